@@ -215,6 +215,85 @@ class LayerCall(Structure):
     ]
 
 
+class CachePlan(Structure):
+    """`CozyCachePlan`."""
+
+    _fields_ = [
+        ("lengths", c_void_p),
+        ("added", c_void_p),
+        ("table", c_void_p),
+        ("table_stride", c_longlong),
+        ("free_ring", c_void_p),
+        ("cursor", c_void_p),
+        ("requests", c_int),
+        ("width", c_int),
+        ("pages", c_int),
+        ("page", c_int),
+        ("tokens", c_int),
+        ("longest", c_int),
+        ("group", c_int),
+        ("max_blocks", c_int),
+        ("lengths_after", c_void_p),
+        ("starts", c_void_p),
+        ("cursor_after", c_void_p),
+        ("positions", c_void_p),
+        ("slots", c_void_p),
+        ("blocks", c_void_p),
+        ("units", c_void_p),
+        ("status", c_void_p),
+    ]
+
+
+class CacheStore(Structure):
+    """`CozyCacheStore`."""
+
+    _fields_ = [
+        ("key", c_void_p),
+        ("value", c_void_p),
+        ("key_exponent", c_void_p),
+        ("value_exponent", c_void_p),
+        ("pages", c_int),
+        ("heads_kv", c_int),
+        ("page", c_int),
+        ("head_dim", c_int),
+    ]
+
+
+class CacheAppend(Structure):
+    """`CozyCacheAppend`."""
+
+    _fields_ = [
+        ("query", c_void_p),
+        ("key", c_void_p),
+        ("value", c_void_p),
+        ("query_strides", c_longlong * 2),
+        ("key_strides", c_longlong * 2),
+        ("value_strides", c_longlong * 2),
+        ("out", c_void_p),
+        ("out_strides", c_longlong * 2),
+        ("normalize", c_int * 2),
+        ("norm_weight", c_void_p * 2),
+        ("norm_offset", c_float * 2),
+        ("norm_eps", c_float * 2),
+        ("rope", POINTER(Rope)),
+    ]
+
+
+class CacheAttend(Structure):
+    """`CozyCacheAttend`."""
+
+    _fields_ = [
+        ("query", c_void_p),
+        ("query_strides", c_longlong * 2),
+        ("out", c_void_p),
+        ("out_strides", c_longlong * 2),
+        ("lse", c_void_p),
+        ("scale", c_float),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_longlong),
+    ]
+
+
 class CudaCallError(RuntimeError):
     """A library entry point returned a non-zero cudaError_t."""
 
@@ -310,6 +389,14 @@ SIGNATURES = {
     "cozy_ulysses_layer_begin": ([c_void_p, POINTER(LayerCall), c_uint64], c_int),
     "cozy_ulysses_layer_attend": ([c_void_p, POINTER(LayerCall), c_uint64], c_int),
     "cozy_ulysses_layer_end": ([c_void_p, POINTER(LayerCall), c_uint64], c_int),
+    "cozy_cache_plan": ([POINTER(CachePlan), c_uint64], c_int),
+    "cozy_cache_append": (
+        [POINTER(CachePlan), POINTER(CacheStore), POINTER(CacheAppend), c_uint64], c_int,
+    ),
+    "cozy_cache_workspace": ([POINTER(CachePlan), POINTER(CacheStore)], c_longlong),
+    "cozy_cache_attention": (
+        [POINTER(CachePlan), POINTER(CacheStore), POINTER(CacheAttend), c_uint64], c_int,
+    ),
     "cozy_error_name": ([c_int], c_char_p),
     "cozy_abi_version": ([], c_int),
 }

@@ -18,7 +18,8 @@ ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libcozy_ulysses.so"
 SOURCES = [
-    "attention_fwd.cu", "stage.cu", "fp8.cu", "peer.cu", "layer.cu", "noalloc.cu", "narrow.cu", "capi.cu",
+    "attention_fwd.cu", "stage.cu", "fp8.cu", "peer.cu", "layer.cu", "noalloc.cu", "narrow.cu", "cache.cu",
+    "cache_attention.cu", "capi.cu",
 ]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 #: Sources compiled with IEEE fp32 semantics (denormals kept, exact division and square root):

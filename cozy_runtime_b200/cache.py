@@ -1,0 +1,420 @@
+"""An 8-bit paged key/value cache and the attention that reads it.
+
+What a causal model needs behind its first pass over a prompt: the keys and values of running
+requests, kept as e4m3 codes in pages of a pool, and attention of each step's new tokens over them.
+A step is one `plan` for all layers, then for each layer an `append` and an `attention`:
+
+    step = cache.plan(layout, table, lengths, new, free, cursor, tokens=T, longest=L)
+    for store, layer in zip(stores, layers):
+        query = cache.append(store, step, key, value, query=query, rope=tables, norm_q=..., norm_k=...)
+        out = cache.attention(store, step, query)
+    lengths, cursor = step.lengths, step.cursor
+
+The step's tokens are packed: request n's rows of `query`, `key` and `value` [tokens, heads,
+head_dim] are `step.starts[n]` to `step.starts[n + 1]`. Lengths, page numbers and the plan's answer
+stay on the GPU: no call here synchronizes, and a step can be captured into a CUDA graph (each
+replay plans anew from the lengths the tensors then hold). A plan that cannot be served gives no
+pages and its append and attention do nothing; `Plan.check()` says why. As with every torch tensor,
+a plan or a cache used on another stream than the one that wrote it is ordered by the caller.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+
+from cozy_runtime_b200 import _lib
+from cozy_runtime_b200.rope import RopeSpec
+from cozy_runtime_b200.ulysses import Norm
+
+PAGES = (16, 32, 64, 128)
+MAX_REQUESTS = 8192
+MAX_GROUP = 128
+#: the range of a block's exponent; larger magnitudes than 448 · 2^40 are stored as NaN
+EXPONENT_RANGE = (-60, 40)
+
+#: bits of a plan's status word
+STATUS_NAMES = {
+    1: "too few free pages",
+    2: "a request longer than its row of the table",
+    4: "more new tokens than `tokens`, or than `longest` in one request",
+    8: "a negative length, new < -1, or an impossible ring cursor",
+    16: "a page number outside the pool",
+    32: "an on-chip wait timed out",
+}
+
+
+@dataclass(frozen=True)
+class Layout:
+    """The heads of every layer of a model and the tokens of a page."""
+
+    heads_q: int
+    heads_kv: int
+    head_dim: int
+    page: int = 64
+
+    def __post_init__(self) -> None:
+        if self.heads_kv < 1 or self.heads_q < 1 or self.heads_q % self.heads_kv:
+            raise ValueError(f"{self.heads_q} query heads over {self.heads_kv} key heads")
+        if self.group > MAX_GROUP:
+            raise ValueError(f"a group of {self.group} query heads is not served ({MAX_GROUP} are)")
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"head dim {self.head_dim} is not served (64 or 128)")
+        if self.page not in PAGES:
+            raise ValueError(f"pages of {self.page} tokens are not served ({PAGES})")
+
+    @property
+    def group(self) -> int:
+        return self.heads_q // self.heads_kv
+
+
+def _need(t: Tensor, name: str, dtype: torch.dtype, shape: tuple[int | None, ...]) -> None:
+    if t.dtype != dtype:
+        raise ValueError(f"{name} is {t.dtype}, not {dtype}")
+    if t.dim() != len(shape) or any(w is not None and g != w for g, w in zip(t.shape, shape)):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
+
+
+def _same_device(device: torch.device, **tensors: Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not {device}")
+    if device.type != "cuda":
+        raise ValueError("operands are not on a CUDA device")
+
+
+class Cache:
+    """One layer's blocks: `key` and `value` codes [pages, heads_kv, page, head_dim]
+    (float8_e4m3fn) and a power of two for each block: `key_exponent`, `value_exponent` [pages,
+    heads_kv] int8; a stored value is code · 2^exponent."""
+
+    def __init__(self, key: Tensor, value: Tensor, key_exponent: Tensor, value_exponent: Tensor):
+        _need(key, "key", torch.float8_e4m3fn, (None, None, None, None))
+        pages, heads, page, dim = key.shape
+        _need(value, "value", torch.float8_e4m3fn, (pages, heads, page, dim))
+        _need(key_exponent, "key_exponent", torch.int8, (pages, heads))
+        _need(value_exponent, "value_exponent", torch.int8, (pages, heads))
+        for name, t in (("key", key), ("value", value), ("key_exponent", key_exponent),
+                        ("value_exponent", value_exponent)):
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+        _same_device(key.device, key=key, value=value, key_exponent=key_exponent,
+                     value_exponent=value_exponent)
+        for name, t in (("key", key), ("value", value)):
+            if t.data_ptr() % 128:
+                raise ValueError(f"{name} must start on a 128-byte boundary")
+        if pages * heads * page > 2**31 - 1:
+            raise ValueError("a pool holds at most 2^31 - 1 rows")
+        self.key, self.value = key, value
+        self.key_exponent, self.value_exponent = key_exponent, value_exponent
+        self._c = _lib.CacheStore(
+            key.data_ptr(), value.data_ptr(), key_exponent.data_ptr(), value_exponent.data_ptr(),
+            pages, heads, page, dim,
+        )
+
+    @classmethod
+    def empty(cls, layout: Layout, pages: int, device: torch.device | str = "cuda") -> Cache:
+        """A pool of `pages` pages (nothing in it has to start at a value)."""
+        shape = (pages, layout.heads_kv, layout.page, layout.head_dim)
+        key, value = (torch.empty(shape, dtype=torch.float8_e4m3fn, device=device) for _ in "kv")
+        exponents = torch.zeros(2, pages, layout.heads_kv, dtype=torch.int8, device=device)
+        return cls(key, value, exponents[0], exponents[1])
+
+    def read(self, pages: Tensor) -> tuple[Tensor, Tensor]:
+        """What blocks of `pages` (page numbers, any shape) hold, as bf16 [*, heads_kv, page,
+        head_dim] keys and values (exact: a code has 4 significant bits)."""
+        out = []
+        for codes, exponent in ((self.key, self.key_exponent), (self.value, self.value_exponent)):
+            x = codes.view(torch.uint8)[pages].view(torch.float8_e4m3fn).to(torch.bfloat16)
+            out.append(x * torch.exp2(exponent[pages].float()).to(torch.bfloat16)[..., None, None])
+        return out[0], out[1]
+
+
+class Plan:
+    """A step's plan on the GPU. Tensors: `lengths` [requests] int32 after the step, `cursor` [2]
+    int64 after it, `starts` [requests + 1] int32, `positions` [tokens] int32 and `slots` [tokens]
+    int64 (page number · page + row; both -1 in rows of nobody), `status` [1] int32."""
+
+    def __init__(self, layout: Layout, table: Tensor, lengths: Tensor, new: Tensor, free: Tensor,
+                 cursor: Tensor, tokens: int, longest: int):
+        n, page = lengths.shape[0], layout.page
+        blocks = min(tokens, tokens // page + 2 * n)
+        # one buffer, in 8-byte words: status, blocks (16-byte entries), cursor, units, slots, ...
+        sizes = (2, 2 * blocks, 2, n + 1, tokens, n // 2 + 1, (n + 1) // 2, (tokens + 1) // 2)
+        self._at = [0]
+        for size in sizes:
+            self._at.append(self._at[-1] + size)
+        self._buffer = torch.empty(self._at[-1], dtype=torch.int64, device=table.device)
+        self.layout, self.table, self.tokens, self.longest = layout, table, tokens, longest
+        # what the calls of this step read must outlive them
+        self._inputs = (lengths, new, free, cursor)
+        base = self._buffer.data_ptr()
+        at = [base + 8 * word for word in self._at]
+        self._c = _lib.CachePlan(
+            lengths.data_ptr(), new.data_ptr(), table.data_ptr(), table.stride(0),
+            free.data_ptr(), cursor.data_ptr(), n, table.shape[1], free.shape[0], page, tokens,
+            longest, layout.group, blocks, at[6], at[5], at[2], at[7], at[4], at[1], at[3], at[0],
+        )
+
+    def _words(self, part: int) -> Tensor:
+        return self._buffer[self._at[part]:self._at[part + 1]]
+
+    @property
+    def requests(self) -> int:
+        return self._c.requests
+
+    @property
+    def pages(self) -> int:
+        return self._c.pages
+
+    @property
+    def status(self) -> Tensor:
+        return self._words(0).view(torch.int32)[:1]
+
+    @property
+    def cursor(self) -> Tensor:
+        return self._words(2)
+
+    @property
+    def slots(self) -> Tensor:
+        return self._words(4)
+
+    @property
+    def starts(self) -> Tensor:
+        return self._words(5).view(torch.int32)[:self.requests + 1]
+
+    @property
+    def lengths(self) -> Tensor:
+        return self._words(6).view(torch.int32)[:self.requests]
+
+    @property
+    def positions(self) -> Tensor:
+        return self._words(7).view(torch.int32)[:self.tokens]
+
+    def check(self) -> None:
+        """Raise if the plan was refused, or if its calls so far met a page number outside the pool
+        or a wait that timed out (synchronizes)."""
+        word = int(self.status.item())
+        if word:
+            raise RuntimeError("cache plan: " + "; ".join(
+                text for bit, text in STATUS_NAMES.items() if word & bit))
+
+
+def plan(
+    layout: Layout,
+    table: Tensor,
+    lengths: Tensor,
+    new: Tensor,
+    free: Tensor,
+    cursor: Tensor,
+    *,
+    tokens: int,
+    longest: int,
+) -> Plan:
+    """Gives pages to the requests of a step and says where its tokens go, in one launch.
+
+    `table` [requests, width] int32: page numbers of each request, in order. `lengths` [requests]
+    int32: tokens a request holds; `new` [requests] int32: tokens it brings (0: none; -1: it is
+    finished and releases its pages, its length becomes 0). `free` [pages] int32: a ring of page
+    numbers of which entries `cursor` = [head, tail) int64 (counted on, taken modulo pages) are
+    free. Pages are given from the head in the requests' order; released ones go behind the tail
+    and are given from the next plan on. `tokens`: rows of the step's tensors (at least the sum of
+    `new`; rows behind it belong to nobody). `longest`: no request brings more than that.
+
+    `table` and `free` are written in place, only where they held nothing; the new lengths and
+    cursor are the plan's, so planning the same tensors again gives the same plan. A step that
+    cannot be served (see `STATUS_NAMES`) changes nothing: its plan has no rows."""
+    _need(lengths, "lengths", torch.int32, (None,))
+    requests = lengths.shape[0]
+    _need(table, "table", torch.int32, (requests, None))
+    _need(new, "new", torch.int32, (requests,))
+    _need(free, "free", torch.int32, (None,))
+    _need(cursor, "cursor", torch.int64, (2,))
+    if not 1 <= requests <= MAX_REQUESTS:
+        raise ValueError(f"{requests} requests are not served (1 to {MAX_REQUESTS})")
+    if table.shape[1] < 1 or free.shape[0] < 1:
+        raise ValueError("an empty table or pool")
+    if table.shape[1] * layout.page > 2**31 - 1:
+        raise ValueError("a request holds at most 2^31 - 1 tokens")
+    if table.stride(1) != 1 or (requests > 1 and table.stride(0) < table.shape[1]):
+        raise ValueError("rows of the table must be contiguous and apart")
+    if not (lengths.is_contiguous() and new.is_contiguous() and free.is_contiguous()
+            and cursor.is_contiguous()):
+        raise ValueError("lengths, new, free and cursor must be contiguous")
+    if not 0 <= tokens < 2**31 or not 0 <= longest < 2**31:
+        raise ValueError("tokens and longest must be counts below 2^31")
+    _same_device(table.device, table=table, lengths=lengths, new=new, free=free, cursor=cursor)
+    with torch.cuda.device(table.device):
+        made = Plan(layout, table, lengths, new, free, cursor, tokens, longest)
+        made._c.table_stride = max(table.stride(0), table.shape[1])
+        code = _lib.load().cozy_cache_plan(
+            ctypes.byref(made._c), torch.cuda.current_stream(table.device).cuda_stream
+        )
+    _lib.check("cozy_cache_plan", code)
+    return made
+
+
+def _rows(t: Tensor, name: str, step: Plan, heads: int) -> tuple[int, int]:
+    """Element strides {token, head} of a step's [tokens, heads, head_dim] rows."""
+    _need(t, name, torch.bfloat16, (step.tokens, heads, step.layout.head_dim))
+    strides = [t.stride(i) if t.shape[i] > 1 else t.shape[2] for i in (0, 1)]
+    if (t.stride(2) != 1 and t.numel() > 0) or any(s % 8 for s in strides) or t.data_ptr() % 16:
+        raise ValueError(f"{name}: the head dimension must be contiguous and rows 16-byte aligned")
+    return strides[0], strides[1]
+
+
+def _out(given: Tensor | None, like: Tensor, step: Plan) -> tuple[Tensor, tuple[int, int]]:
+    if given is None:
+        given = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    token, head = _rows(given, "out", step, like.shape[1])
+    rows, heads, dim = given.shape
+    apart = head >= dim and token >= (heads - 1) * head + dim
+    apart = apart or (token >= dim and head >= (rows - 1) * token + dim)
+    if rows * heads > 1 and not apart:
+        raise ValueError("rows of out overlap")
+    return given, (token, head)
+
+
+def _range(t: Tensor) -> tuple[int, int]:
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _fits(store: Cache, step: Plan) -> None:
+    c, layout = store._c, step.layout
+    if (c.heads_kv, c.page, c.head_dim) != (layout.heads_kv, layout.page, layout.head_dim):
+        raise ValueError("the cache's heads or pages are not the plan's layout")
+    if c.pages != step.pages:
+        raise ValueError(f"a cache of {c.pages} pages and a plan over {step.pages}")
+
+
+def append(
+    store: Cache,
+    step: Plan,
+    key: Tensor,
+    value: Tensor,
+    *,
+    query: Tensor | None = None,
+    rope: RopeSpec | None = None,
+    norm_q: Norm | None = None,
+    norm_k: Norm | None = None,
+    out: Tensor | None = None,
+) -> Tensor | None:
+    """Stores a step's keys and values, and readies its queries, in one launch.
+
+    `key`, `value` [tokens, heads_kv, head_dim] and `query` [tokens, heads_q, head_dim] bf16, head
+    dimension contiguous. Query and key are normed (`norm_q`, `norm_k`: per-head RMSNorm) and
+    rotated (`rope`: row = position in the request; the tables must reach the table's width) in
+    fp32 and rounded once to bf16, the laws of `rope.head_norm_rope`. Returns the ready queries
+    (`out`, or a new tensor; rows of nobody are left as they were), None without `query`.
+
+    A block's exponent is the smallest e ≥ -60 with max |x| ≤ 448 · 2^e over the tokens put into it
+    so far. It only grows; the codes a block holds are then rounded to the grown scale, which is
+    exact down to e4m3's subnormals. NaN, infinities and magnitudes over 448 · 2^40 are stored as
+    NaN and leave the exponent alone. The same step can be appended again: it stores the same.
+    A page that requests share must be full: two writers of one block are not ordered."""
+    _fits(store, step)
+    layout = step.layout
+    _same_device(store.key.device, plan=step.table, key=key, value=value, query=query, out=out)
+    a = _lib.CacheAppend()
+    a.key, a.value = key.data_ptr(), value.data_ptr()
+    a.key_strides[:] = _rows(key, "key", step, layout.heads_kv)
+    a.value_strides[:] = _rows(value, "value", step, layout.heads_kv)
+    if query is not None:
+        a.query_strides[:] = _rows(query, "query", step, layout.heads_q)
+    elif norm_q is not None or out is not None:
+        raise ValueError("norm_q and out are the query's")
+    tables = None
+    if rope is not None:
+        _same_device(store.key.device, cos=rope.cos, sin=rope.sin)
+        last = step._c.width * layout.page - 1
+        columns = rope.rotary // 2 if rope.interleaved else rope.rotary
+        if rope.rotary < 0 or rope.rotary > layout.head_dim or rope.rotary % 2:
+            raise ValueError(f"{rope.rotary} rotated channels of {layout.head_dim}")
+        if not rope.interleaved and rope.rotary % 16:
+            raise ValueError("split-half rotation serves multiples of 16 channels")
+        reach = last * rope.stride_token + (columns - 1) * rope.stride_channel
+        for t in (rope.cos, rope.sin):
+            if t.dtype != torch.float32 or not t.is_contiguous():
+                raise ValueError("rotation tables are contiguous fp32")
+            if rope.stride_token < 0 or rope.stride_channel < 0 or (columns > 0 and reach >= t.numel()):
+                raise ValueError("the rotation tables end before the table's last position")
+        tables = rope.struct(0)
+        a.rope = ctypes.pointer(tables)
+    weights = []
+    for i, norm in enumerate((norm_q, norm_k)):
+        if norm is None:
+            continue
+        a.normalize[i] = 1
+        a.norm_offset[i], a.norm_eps[i] = float(norm.offset), float(norm.eps)
+        if norm.weight is not None:
+            if norm.weight.shape != (layout.head_dim,):
+                raise ValueError("a norm's weight has one value for each channel of a head")
+            w = norm.weight.to(device=store.key.device, dtype=torch.float32).contiguous()
+            weights.append(w)
+            a.norm_weight[i] = w.data_ptr()
+    with torch.cuda.device(store.key.device):
+        if query is not None:
+            out, strides = _out(out, query, step)
+            a.query, a.out = query.data_ptr(), out.data_ptr()
+            a.out_strides[:] = strides
+        code = _lib.load().cozy_cache_append(
+            ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a),
+            torch.cuda.current_stream(store.key.device).cuda_stream,
+        )
+    _lib.check("cozy_cache_append", code)
+    return out
+
+
+def attention(
+    store: Cache,
+    step: Plan,
+    query: Tensor,
+    *,
+    scale: float | None = None,
+    out: Tensor | None = None,
+    return_lse: bool = False,
+) -> Tensor | tuple[Tensor, Tensor]:
+    """Causal attention of a step's queries [tokens, heads_q, head_dim] bf16 over their requests'
+    blocks, the step's own tokens among them (`append` comes first): each row sees the keys up to
+    its own position. Returns `out` (or a new tensor) of the query's shape, and with `return_lse`
+    the natural log of each row's sum of exponentials [tokens, heads_q] fp32, by which outputs
+    over parts of the keys can be joined. Rows of nobody are left as they were.
+
+    What stands in blocks behind a row's last key, NaN among it, does not reach the row. Keys in a
+    page whose number is outside the pool are left out, and the plan's status says so."""
+    _fits(store, step)
+    device = store.key.device
+    _same_device(device, plan=step.table, query=query, out=out)
+    scale = 1.0 / math.sqrt(step.layout.head_dim) if scale is None else float(scale)
+    if not (0.0 < scale < 3e38):
+        raise ValueError("attention scale must be positive and finite")
+    a = _lib.CacheAttend()
+    a.query, a.scale = query.data_ptr(), scale
+    a.query_strides[:] = _rows(query, "query", step, step.layout.heads_q)
+    with torch.cuda.device(device):
+        given, (out, strides) = out, _out(out, query, step)
+        if given is not None and query.numel() > 0:
+            (q0, q1), (o0, o1) = _range(query), _range(out)
+            if q0 < o1 and o0 < q1:
+                raise ValueError("out overlaps the query")
+        a.out = out.data_ptr()
+        a.out_strides[:] = strides
+        lse = None
+        if return_lse:
+            lse = torch.empty(query.shape[:2], dtype=torch.float32, device=device)
+            a.lse = lse.data_ptr()
+        lib = _lib.load()
+        size = lib.cozy_cache_workspace(ctypes.byref(step._c), ctypes.byref(store._c))
+        space = torch.empty(size, dtype=torch.uint8, device=device)
+        a.workspace, a.workspace_bytes = space.data_ptr(), size
+        code = lib.cozy_cache_attention(
+            ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a),
+            torch.cuda.current_stream(device).cuda_stream,
+        )
+    _lib.check("cozy_cache_attention", code)
+    return out if lse is None else (out, lse)

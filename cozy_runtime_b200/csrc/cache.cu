@@ -1,0 +1,547 @@
+// The 8-bit paged cache's bookkeeping: a step's plan (block tables and slot maps from request
+// lengths) and the append (per-head RMSNorm and RoPE of the step's queries and keys, keys and
+// values into e4m3 blocks).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/cozy_ulysses.h"
+#include "cache.cuh"
+#include "norm_rope.cuh"
+
+namespace cozy {
+
+// ---------------------------------------------------------------------------------- the plan
+// One cluster. Every CTA scans all requests (a few loads a thread, two barriers a round: cheaper
+// than handing the sums over), keeps the running sums in shared memory, and then takes its share
+// of the tokens, fresh pages, released pages and touched blocks, each found by bisection.
+// Nothing here is bandwidth: a step of 4 requests moves 112 bytes, one of 1000 requests 170 KB;
+// the time is the launch, one load of the lengths, the scan and the bisection's chain.
+constexpr int kPlanThreads = 1024;
+
+struct PlanSums {
+  long long tokens, need, back, blocks, units;
+};
+
+__device__ __forceinline__ PlanSums operator+(PlanSums a, const PlanSums& b) {
+  a.tokens += b.tokens;
+  a.need += b.need;
+  a.back += b.back;
+  a.blocks += b.blocks;
+  a.units += b.units;
+  return a;
+}
+
+__device__ __forceinline__ PlanSums shifted(const PlanSums& a, int by) {
+  PlanSums r;
+  r.tokens = __shfl_up_sync(0xffffffffu, a.tokens, by);
+  r.need = __shfl_up_sync(0xffffffffu, a.need, by);
+  r.back = __shfl_up_sync(0xffffffffu, a.back, by);
+  r.blocks = __shfl_up_sync(0xffffffffu, a.blocks, by);
+  r.units = __shfl_up_sync(0xffffffffu, a.units, by);
+  return r;
+}
+
+__device__ __forceinline__ long long pages_of(long long length, int page) {
+  return (length + page - 1) / page;
+}
+
+// One request's part of the sums, and the status bits it raises.
+__device__ __forceinline__ PlanSums request_sums(const CozyCachePlan& p, int n, int* flags) {
+  const long long length = p.lengths[n], added = p.added[n];
+  PlanSums s = {};
+  if (length < 0 || added < -1) {
+    *flags |= kPlanLengths;
+    return s;
+  }
+  const long long held = pages_of(length, p.page);
+  if (added < 0) {
+    if (held > p.width) *flags |= kPlanNarrow;
+    s.back = held;
+    return s;
+  }
+  const long long want = pages_of(length + added, p.page);
+  if (want > p.width) *flags |= kPlanNarrow;
+  if (added > p.longest) *flags |= kPlanTokens;
+  s.tokens = added;
+  s.need = want - held;
+  if (added > 0) {
+    s.blocks = want - length / p.page;
+    s.units = attention_units(p.group, p.longest, length, added);
+  }
+  return s;
+}
+
+__device__ __forceinline__ int ring_at(long long at, int pages) {
+  return static_cast<int>(at % pages);
+}
+
+// The request whose span [starts[n], starts[n + 1]) holds `at`.
+__device__ __forceinline__ int span_of(const int* starts, int n, int at) {
+  int low = 0, high = n - 1;
+  while (low < high) {
+    const int mid = (low + high + 1) >> 1;
+    if (starts[mid] <= at) low = mid;
+    else high = mid - 1;
+  }
+  return low;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const CozyCachePlan p) {
+  extern __shared__ int plan_smem[];
+  __shared__ PlanSums warp_sums[32];
+  __shared__ int any_flags;
+  const int n1 = p.requests + 1;
+  int* starts = plan_smem;        // [requests + 1] each: tokens, fresh pages, released pages, blocks
+  int* needs = starts + n1;
+  int* backs = needs + n1;
+  int* blocks = backs + n1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool lead = blockIdx.x == 0;
+  if (threadIdx.x == 0) any_flags = 0;
+  __syncthreads();
+
+  // checks first: a step that cannot be served gets nothing at all
+  int flags = 0;
+  PlanSums carry = {};
+  for (int base = 0; base < p.requests; base += kPlanThreads) {
+    const int n = base + threadIdx.x;
+    PlanSums mine = n < p.requests ? request_sums(p, n, &flags) : PlanSums{};
+    PlanSums upto = mine;
+#pragma unroll
+    for (int by = 1; by < 32; by <<= 1) {
+      const PlanSums other = shifted(upto, by);
+      if (lane >= by) upto = upto + other;
+    }
+    if (lane == 31) warp_sums[warp] = upto;
+    __syncthreads();
+    if (warp == 0) {
+      PlanSums w = warp_sums[lane];
+#pragma unroll
+      for (int by = 1; by < 32; by <<= 1) {
+        const PlanSums other = shifted(w, by);
+        if (lane >= by) w = w + other;
+      }
+      warp_sums[lane] = w;
+    }
+    __syncthreads();
+    PlanSums before = carry;
+    if (warp > 0) before = before + warp_sums[warp - 1];
+    const PlanSums end = before + upto;
+    if (n < p.requests) {
+      // sums past 2^31 - 1 only occur in steps that are refused below
+      starts[n + 1] = static_cast<int>(end.tokens);
+      needs[n + 1] = static_cast<int>(end.need);
+      backs[n + 1] = static_cast<int>(end.back);
+      blocks[n + 1] = static_cast<int>(end.blocks);
+      if (lead) p.units[n + 1] = end.units;
+    }
+    carry = carry + warp_sums[31];
+    __syncthreads();
+  }
+  const long long head = p.cursor[0], tail = p.cursor[1];
+  if (head < 0 || tail < head || tail - head > p.pages) flags |= kPlanLengths;
+  else if (carry.need > tail - head) flags |= kPlanNoPages;
+  else if (tail - head + carry.back > p.pages) flags |= kPlanLengths;
+  if (carry.tokens > p.tokens) flags |= kPlanTokens;
+  if (flags) atomicOr(&any_flags, flags);
+  __syncthreads();
+  const int status = any_flags;
+  const bool refused = status != 0;
+  if (refused) {
+    for (int n = threadIdx.x; n < n1; n += kPlanThreads) {
+      starts[n] = 0;
+      if (lead) p.units[n] = 0;
+    }
+    carry = PlanSums{};
+  } else if (threadIdx.x == 0) {
+    starts[0] = needs[0] = backs[0] = blocks[0] = 0;
+    if (lead) p.units[0] = 0;
+  }
+  if (lead && threadIdx.x == 0) {
+    *p.status = status;
+    p.cursor_after[0] = head + carry.need;
+    p.cursor_after[1] = tail + carry.back;
+  }
+  // the status word is set before any CTA adds the bad-page bit to it
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+
+  const int first = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
+  for (int n = first; n < n1; n += step) {
+    p.starts[n] = starts[n];
+    if (n < p.requests) {
+      const int length = p.lengths[n], added = p.added[n];
+      p.lengths_after[n] = refused ? max(length, 0) : added < 0 ? 0 : length + added;
+    }
+  }
+  // the page of block `b` of request n: fresh ones straight from the ring
+  bool bad = false;
+  auto page_of = [&](int n, int b) {
+    const int held = static_cast<int>(pages_of(p.lengths[n], p.page));
+    const int id = b < held ? p.table[n * p.table_stride + b]
+                            : p.free_ring[ring_at(head + needs[n] + (b - held), p.pages)];
+    if (id >= 0 && id < p.pages) return id;
+    bad = true;
+    return -1;
+  };
+  const int tokens = static_cast<int>(carry.tokens);
+  for (int t = first; t < p.tokens; t += step) {
+    int position = -1;
+    long long slot = -1;
+    if (t < tokens) {
+      const int n = span_of(starts, p.requests, t);
+      position = p.lengths[n] + (t - starts[n]);
+      const int id = page_of(n, position / p.page);
+      if (id >= 0) slot = static_cast<long long>(id) * p.page + position % p.page;
+      else position = -1;
+    }
+    p.positions[t] = position;
+    p.slots[t] = slot;
+  }
+  for (int i = first; i < p.max_blocks; i += step) {
+    int4 entry = make_int4(-1, 0, 0, 0);  // page, first row, rows, first token
+    if (i < carry.blocks) {
+      const int n = span_of(blocks, p.requests, i);
+      const int length = p.lengths[n], added = p.added[n];
+      const int b = length / p.page + (i - blocks[n]);
+      const int low = max(length, b * p.page);
+      const int high = static_cast<int>(min(static_cast<long long>(length) + added,
+                                            (b + 1LL) * p.page));
+      entry = make_int4(page_of(n, b), low - b * p.page, high - low, starts[n] + low - length);
+    }
+    reinterpret_cast<int4*>(p.blocks)[i] = entry;
+  }
+  if (bad) atomicOr(p.status, kPlanBadPage);
+  for (int i = first; i < carry.back; i += step) {
+    const int n = span_of(backs, p.requests, i);
+    p.free_ring[ring_at(tail + i, p.pages)] = p.table[n * p.table_stride + (i - backs[n])];
+  }
+  for (int i = first; i < carry.need; i += step) {
+    const int n = span_of(needs, p.requests, i);
+    const int held = static_cast<int>(pages_of(p.lengths[n], p.page));
+    p.table[n * p.table_stride + held + (i - needs[n])] = p.free_ring[ring_at(head + i, p.pages)];
+  }
+}
+
+static int plan_check(const CozyCachePlan& p) {
+  if (p.requests < 1 || p.requests > COZY_CACHE_MAX_REQUESTS || p.width < 1 || p.pages < 1)
+    return cudaErrorInvalidValue;
+  if (p.page != 16 && p.page != 32 && p.page != 64 && p.page != 128) return cudaErrorNotSupported;
+  if (p.tokens < 0 || p.longest < 0 || p.group < 1 || p.table_stride < p.width)
+    return cudaErrorInvalidValue;
+  if (static_cast<long long>(p.width) * p.page > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (p.group > COZY_CACHE_MAX_GROUP) return cudaErrorNotSupported;
+  const void* ptrs[] = {p.lengths, p.added, p.table, p.free_ring, p.cursor, p.lengths_after,
+                        p.starts, p.cursor_after, p.units, p.status};
+  for (const void* ptr : ptrs)
+    if (ptr == nullptr) return cudaErrorInvalidValue;
+  if (p.tokens > 0 && (!p.positions || !p.slots || !p.blocks)) return cudaErrorInvalidValue;
+  if (reinterpret_cast<uintptr_t>(p.blocks) % 16) return cudaErrorInvalidValue;
+  // every block that `tokens` tokens of `requests` requests can touch has an entry
+  const long long most = static_cast<long long>(p.tokens) / p.page + 2LL * p.requests;
+  if (p.max_blocks < (most < p.tokens ? most : p.tokens)) return cudaErrorInvalidValue;
+  return cudaSuccess;
+}
+
+int cache_plan(const CozyCachePlan& p, cudaStream_t stream) {
+  const int e = plan_check(p);
+  if (e) return e;
+  const size_t smem = 4 * sizeof(int) * (static_cast<size_t>(p.requests) + 1);
+  static bool configured[64] = {};
+  int device = 0;
+  cudaGetDevice(&device);
+  if (device < 64 && !configured[device]) {
+    const cudaError_t r = cudaFuncSetAttribute(
+        cache_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        static_cast<int>(4 * sizeof(int) * (COZY_CACHE_MAX_REQUESTS + 1)));
+    if (r != cudaSuccess) return r;
+    configured[device] = true;
+  }
+  // one CTA up to a thread for each token, else the portable cluster of 8
+  cudaLaunchConfig_t cfg = {};
+  const unsigned ctas = p.tokens <= kPlanThreads ? 1 : 8;
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, cache_plan_kernel, p);
+}
+
+// -------------------------------------------------------------------------------- the append
+// A unit is one touched block of one head of K or V: its new rows are read once (held as bf16 in
+// registers), normed and rotated, their largest magnitude sets or grows the block's exponent,
+// and their codes are written. WARPS warps share a unit. Queries take CTAs of the same launch.
+// HBM bounds the long form: a token reads (Hq + 2 Hkv) · D bf16 and writes Hq · D bf16 and
+// 2 · Hkv · D codes.
+struct AppendTensor {  // the fields norm_rope_row reads
+  int normalize;
+  const float* norm_weight;
+  float norm_offset, norm_eps;
+  int rotate;
+};
+
+struct AppendArgs {
+  const int4* blocks;
+  const int* positions;
+  int max_blocks, tokens;
+  int pages, page, heads_q, heads_kv;
+  const __nv_bfloat16* src[3];  // query, key, value
+  long long src_token[3], src_head[3];
+  __nv_bfloat16* out;  // rotated queries
+  long long out_token, out_head;
+  uint8_t* codes[2];
+  int8_t* exponents[2];
+  AppendTensor t[3];
+  CozyRope rope;
+  unsigned query_ctas;
+};
+
+__device__ __forceinline__ void widen8(uint4 v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ uint4 narrow8(const float (&x)[8]) {
+  return make_uint4(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4], x[5]),
+                    bf16_pair(x[6], x[7]));
+}
+
+// Eight values to e4m3 codes (round to nearest even; NaN stays NaN).
+__device__ __forceinline__ uint2 encode8(const float (&x)[8]) {
+  uint16_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h[i]) : "f"(x[2 * i]), "f"(x[2 * i + 1]));
+  return make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+}
+
+__device__ __forceinline__ void decode8(uint2 c, float (&x)[8]) {
+  const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint16_t pair = static_cast<uint16_t>(w[i >> 1] >> ((i & 1) * 16));
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(pair));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+// The smallest exponent e ≥ the floor with amax ≤ 448 · 2^e: 448 = 1.75 · 2^8, so the fraction
+// bits carry into the exponent field exactly when they are above 0.75.
+__device__ __forceinline__ int exponent_of(float amax) {
+  const int e = static_cast<int>((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8;
+  return max(e, kExponentFloor);
+}
+
+template <int HD, int WARPS>
+__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+  constexpr int CHUNKS = HD / 8;         // threads a row
+  constexpr int ROWS = 32 / CHUNKS;      // rows a warp and pass
+  constexpr int PASSES = 8;              // rows a unit holds: WARPS · ROWS · PASSES
+  constexpr int UNITS = 8 / WARPS;       // units a CTA
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunk = lane % CHUNKS, sub = lane / CHUNKS, d0 = chunk * 8;
+  const unsigned mask = row_group_mask<CHUNKS>();
+
+  if (blockIdx.x < a.query_ctas) {  // queries: a row a group of threads
+    const long long row = (static_cast<long long>(blockIdx.x) * 8 + warp) * ROWS + sub;
+    if (row >= static_cast<long long>(a.tokens) * a.heads_q) return;
+    const int token = static_cast<int>(row / a.heads_q), head = static_cast<int>(row % a.heads_q);
+    const int position = a.positions[token];
+    if (position < 0) return;
+    float x[8];
+    widen8(*reinterpret_cast<const uint4*>(a.src[0] + token * a.src_token[0] +
+                                           head * a.src_head[0] + d0), x);
+    norm_rope_row<HD>(x, d0, chunk, mask, position, a.t[0], a.rope);
+    *reinterpret_cast<uint4*>(a.out + token * a.out_token + head * a.out_head + d0) = narrow8(x);
+    return;
+  }
+
+  __shared__ float largest[8];
+  const long long unit = static_cast<long long>(blockIdx.x - a.query_ctas) * UNITS + warp / WARPS;
+  const int which = static_cast<int>(unit & 1);  // 0 keys, 1 values
+  const int head = static_cast<int>((unit >> 1) % a.heads_kv);
+  const long long at = (unit >> 1) / a.heads_kv;
+  const int4 entry = at < a.max_blocks ? a.blocks[at] : make_int4(-1, 0, 0, 0);
+  if (entry.x < 0) return;  // all warps of the unit alike (WARPS = 8: the whole CTA)
+  const int slot = (warp % WARPS) * ROWS + sub;
+  const AppendTensor& t = a.t[1 + which];
+  const __nv_bfloat16* src = a.src[1 + which] + entry.w * a.src_token[1 + which] +
+                             head * a.src_head[1 + which] + d0;
+  uint4 held[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = slot + i * (WARPS * ROWS);
+    if (r < entry.z) held[i] = *reinterpret_cast<const uint4*>(src + r * a.src_token[1 + which]);
+  }
+  float amax = 0.f;
+  const int position = a.positions[entry.w];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = slot + i * (WARPS * ROWS);
+    if (r < entry.z) {
+      float x[8];
+      widen8(held[i], x);
+      if (t.normalize || t.rotate) {
+        norm_rope_row<HD>(x, d0, chunk, mask, position + r, t, a.rope);
+        held[i] = narrow8(x);
+        widen8(held[i], x);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float m = fabsf(x[k]);
+        if (m <= kLargestStored) amax = fmaxf(amax, m);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const long long block = static_cast<long long>(entry.x) * a.heads_kv + head;
+  int8_t* exponent = a.exponents[which] + block;
+  const int before = entry.y > 0 ? *exponent : kExponentFloor;
+  if constexpr (WARPS > 1) {
+    if (lane == 0) largest[warp] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) amax = fmaxf(amax, largest[w]);
+  } else {
+    __syncwarp();
+  }
+  const int e = max(before, exponent_of(amax));
+  if (chunk == 0 && slot == 0) *exponent = static_cast<int8_t>(e);
+  uint8_t* codes = a.codes[which] + block * a.page * HD + d0;
+  const float scale = exponent_scale(-e);
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = slot + i * (WARPS * ROWS);
+    if (r < entry.z) {
+      float x[8];
+      widen8(held[i], x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        x[k] = fabsf(x[k]) <= kLargestStored ? x[k] * scale : __uint_as_float(0x7fc00000u);
+      *reinterpret_cast<uint2*>(codes + (entry.y + r) * HD) = encode8(x);
+    }
+  }
+  if (e > before && entry.y > 0) {  // the scale grew: shift what the block holds already
+    const float shift = exponent_scale(max(before - e, -126));
+    for (int r = slot; r < entry.y; r += WARPS * ROWS) {
+      uint2* row = reinterpret_cast<uint2*>(codes + r * HD);
+      float x[8];
+      decode8(*row, x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= shift;
+      *row = encode8(x);
+    }
+  }
+}
+
+template <int HD>
+static int append_launch(AppendArgs& a, int longest, cudaStream_t stream) {
+  constexpr int kRows = 32 / (HD / 8);
+  const long long rows = a.out != nullptr ? static_cast<long long>(a.tokens) * a.heads_q : 0;
+  const long long query_ctas = (rows + 8 * kRows - 1) / (8 * kRows);
+  const long long units = 2LL * a.heads_kv * a.max_blocks;
+  // A warp holds 8 passes of rows. Where no block gets more than that, a warp a unit (a decode
+  // step: one row a unit); else the 8 warps of a CTA share one (up to 128 rows).
+  const int most = longest < a.page ? longest : a.page;
+  const bool narrow = most <= 8 * kRows;
+  const long long ctas = query_ctas + (narrow ? (units + 7) / 8 : units);
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  a.query_ctas = static_cast<unsigned>(query_ctas);
+  if (narrow)
+    cache_append_kernel<HD, 1><<<static_cast<unsigned>(ctas), 256, 0, stream>>>(a);
+  else
+    cache_append_kernel<HD, 8><<<static_cast<unsigned>(ctas), 256, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+int cache_store_check(const CozyCacheStore& c, const CozyCachePlan& p) {
+  if (c.head_dim != 64 && c.head_dim != 128) return cudaErrorNotSupported;
+  if (c.heads_kv < 1 || c.pages != p.pages || c.page != p.page) return cudaErrorInvalidValue;
+  // rows of a pool are counted in 31 bits (tensor-map coordinates)
+  if (static_cast<long long>(c.pages) * c.heads_kv > 0x7fffffffLL / c.page)
+    return cudaErrorInvalidValue;
+  if (!c.key || !c.value || !c.key_exponent || !c.value_exponent) return cudaErrorInvalidValue;
+  if (reinterpret_cast<uintptr_t>(c.key) % 128 || reinterpret_cast<uintptr_t>(c.value) % 128)
+    return cudaErrorInvalidValue;
+  return cudaSuccess;
+}
+
+int cache_append(const CozyCachePlan& p, const CozyCacheStore& c, const CozyCacheAppend& x,
+                 cudaStream_t stream) {
+  int e = plan_check(p);
+  if (e || (e = cache_store_check(c, p))) return e;
+  if (p.tokens == 0) return cudaSuccess;
+  AppendArgs a = {};
+  a.blocks = reinterpret_cast<const int4*>(p.blocks);
+  a.positions = p.positions;
+  a.max_blocks = p.max_blocks;
+  a.tokens = p.tokens;
+  a.pages = c.pages;
+  a.page = c.page;
+  a.heads_q = c.heads_kv * p.group;
+  a.heads_kv = c.heads_kv;
+  const void* src[3] = {x.query, x.key, x.value};
+  const long long* strides[3] = {x.query_strides, x.key_strides, x.value_strides};
+  for (int i = 0; i < 3; ++i) {
+    if (i == 0 && src[0] == nullptr) continue;
+    if (src[i] == nullptr || reinterpret_cast<uintptr_t>(src[i]) % 16) return cudaErrorInvalidValue;
+    if (strides[i][0] < 0 || strides[i][1] < 0 || strides[i][0] % 8 || strides[i][1] % 8)
+      return cudaErrorInvalidValue;
+    a.src[i] = static_cast<const __nv_bfloat16*>(src[i]);
+    a.src_token[i] = strides[i][0];
+    a.src_head[i] = strides[i][1];
+  }
+  if (src[0] != nullptr) {
+    if (x.out == nullptr || reinterpret_cast<uintptr_t>(x.out) % 16 || x.out_strides[0] % 8 ||
+        x.out_strides[1] % 8 || x.out_strides[0] < 0 || x.out_strides[1] < 0)
+      return cudaErrorInvalidValue;
+    a.out = static_cast<__nv_bfloat16*>(x.out);
+    a.out_token = x.out_strides[0];
+    a.out_head = x.out_strides[1];
+  }
+  a.codes[0] = static_cast<uint8_t*>(c.key);
+  a.codes[1] = static_cast<uint8_t*>(c.value);
+  a.exponents[0] = static_cast<int8_t*>(c.key_exponent);
+  a.exponents[1] = static_cast<int8_t*>(c.value_exponent);
+  for (int i = 0; i < 2; ++i) {
+    a.t[i].normalize = x.normalize[i];
+    a.t[i].norm_weight = x.norm_weight[i];
+    a.t[i].norm_offset = x.norm_offset[i];
+    a.t[i].norm_eps = x.norm_eps[i];
+    a.t[i].rotate = x.rope != nullptr;
+  }
+  if (x.rope != nullptr) {
+    a.rope = *x.rope;
+    if (!a.rope.cos || !a.rope.sin || a.rope.rotary < 0 || a.rope.rotary > c.head_dim ||
+        a.rope.rotary % 2)
+      return cudaErrorInvalidValue;
+    if (!a.rope.interleaved && a.rope.rotary % 16) return cudaErrorNotSupported;
+  }
+  return c.head_dim == 64 ? append_launch<64>(a, p.longest, stream)
+                          : append_launch<128>(a, p.longest, stream);
+}
+
+}  // namespace cozy

@@ -165,3 +165,37 @@ int cozy_attention_fwd_fp8(const void* q, const void* k, const void* v, const fl
 }
 
 }  // extern "C"
+
+namespace cozy {
+int cache_plan(const CozyCachePlan& plan, cudaStream_t stream);
+int cache_append(const CozyCachePlan& plan, const CozyCacheStore& store,
+                 const CozyCacheAppend& append, cudaStream_t stream);
+long long cache_workspace(const CozyCachePlan& plan, const CozyCacheStore& store);
+int cache_attention(const CozyCachePlan& plan, const CozyCacheStore& store,
+                    const CozyCacheAttend& attend, cudaStream_t stream);
+}  // namespace cozy
+
+extern "C" {
+
+int cozy_cache_plan(const CozyCachePlan* plan, uintptr_t stream) {
+  if (!plan) return cudaErrorInvalidValue;
+  return cozy::cache_plan(*plan, as_stream(stream));
+}
+
+int cozy_cache_append(const CozyCachePlan* plan, const CozyCacheStore* store,
+                      const CozyCacheAppend* append, uintptr_t stream) {
+  if (!plan || !store || !append) return cudaErrorInvalidValue;
+  return cozy::cache_append(*plan, *store, *append, as_stream(stream));
+}
+
+long long cozy_cache_workspace(const CozyCachePlan* plan, const CozyCacheStore* store) {
+  return plan && store ? cozy::cache_workspace(*plan, *store) : 0;
+}
+
+int cozy_cache_attention(const CozyCachePlan* plan, const CozyCacheStore* store,
+                         const CozyCacheAttend* attend, uintptr_t stream) {
+  if (!plan || !store || !attend) return cudaErrorInvalidValue;
+  return cozy::cache_attention(*plan, *store, *attend, as_stream(stream));
+}
+
+}  // extern "C"

@@ -458,6 +458,113 @@ COZY_API int cozy_ulysses_layer_attend(CozyGroup* group, const CozyLayerCall* ca
                                        uintptr_t stream);
 COZY_API int cozy_ulysses_layer_end(CozyGroup* group, const CozyLayerCall* call, uintptr_t stream);
 
+/* ------------------------------------------------------------------- the 8-bit paged cache
+ * Keys and values of running requests, kept as e4m3 codes in pages of `page` tokens; what a
+ * request holds is named by its row of a block table. Three calls make a step: a plan (once for
+ * all layers), then for each layer an append and an attention. All sizes the host does not know
+ * (lengths, pages) stay on the GPU; nothing allocates or synchronizes, so a step can be captured
+ * into a graph. */
+#define COZY_CACHE_MAX_REQUESTS 8192
+#define COZY_CACHE_MAX_GROUP 128
+
+/* A step's plan. Inputs: request n holds lengths[n] tokens in the pages of its table row and
+ * brings added[n] new ones (0: none; -1: it is finished and its pages are released). Free page
+ * numbers are the entries [cursor[0], cursor[1]) of a ring of `pages` entries (taken modulo
+ * pages). Requests are given pages in order, from the ring's head; released pages go behind its
+ * tail, to be given from the next plan on. Rows of the step's tokens: request n's are
+ * [starts[n], starts[n + 1]); rows behind the last belong to nobody.
+ * Writes the table (fresh entries only), the ring (behind the tail only), and the outputs;
+ * lengths, added and cursor stay as they were, so the same plan can be made again.
+ * *status: 0, or the sum of 1 (too few free pages), 2 (a request longer than its table row), 4
+ * (more new tokens than `tokens`, or than `longest` in one request), 8 (a negative length,
+ * added < -1, or an impossible cursor) - with any of these nothing is given or released, starts
+ * are all 0 and append and attention do nothing - and 16 (a page number outside [0, pages): the
+ * tokens in such a page are left out). A later call that meets such a page in the table sets 16
+ * too, and one whose on-chip wait times out sets 32 (its output is then incomplete). */
+typedef struct CozyCachePlan {
+  const int* lengths;      /* [requests] */
+  const int* added;        /* [requests] */
+  int* table;              /* [requests][table_stride], `width` entries used */
+  long long table_stride;
+  int* free_ring;          /* [pages] */
+  const long long* cursor; /* [2] head, tail */
+  int requests, width, pages, page; /* page: 16, 32, 64 or 128 tokens */
+  int tokens;              /* rows of the step's tensors */
+  int longest;             /* no request brings more new tokens */
+  int group;               /* query heads per key/value head, at most COZY_CACHE_MAX_GROUP */
+  int max_blocks;          /* entries of `blocks`: min(tokens, tokens / page + 2 * requests) */
+  int* lengths_after;      /* [requests] */
+  int* starts;             /* [requests + 1] */
+  long long* cursor_after; /* [2] */
+  int* positions;          /* [tokens] position in its request, -1 for a row of nobody */
+  long long* slots;        /* [tokens] page number * page + row in the page, or -1 */
+  int* blocks;             /* [max_blocks][4], 16-byte aligned: page (-1: none), first row, rows,
+                              first token: the blocks this step's tokens go into */
+  long long* units;        /* [requests + 1] units of attention before each request, a head */
+  int* status;
+} CozyCachePlan;
+
+COZY_API int cozy_cache_plan(const CozyCachePlan* plan, uintptr_t stream);
+
+/* One layer's blocks: codes [pages][heads_kv][page][head_dim] (e4m3, 128-byte aligned) and one
+ * exponent a block ([pages][heads_kv], int8 in [-60, 40]): value = code * 2^exponent. */
+typedef struct CozyCacheStore {
+  void* key;
+  void* value;
+  void* key_exponent;
+  void* value_exponent;
+  int pages, heads_kv, page, head_dim; /* head_dim 64 or 128 */
+} CozyCacheStore;
+
+/* Puts a step's keys and values into their blocks, in one launch with what comes before the
+ * attention: per-head RMSNorm and RoPE (by each token's position; the laws of
+ * cozy_head_norm_rope) of query [tokens, heads_kv * group, head_dim] into `out` and of key
+ * [tokens, heads_kv, head_dim], rounded to bf16, then codes. A block's exponent is the smallest
+ * e >= -60 with max |x| <= 448 * 2^e over the tokens put into it so far: it only grows, and the
+ * codes that the block holds are then rounded to the grown scale (exact down to subnormals). A
+ * magnitude over 448 * 2^40 or a NaN is stored as NaN and does not count for the exponent. Rows
+ * of `out` that belong to nobody are left as they were. Strides in elements {token, head},
+ * multiples of 8; pointers 16-byte aligned. Index 0 of the norm arrays is the query's, 1 the
+ * key's. rope->token0 is not used; the tables must hold every position up to width * page. */
+typedef struct CozyCacheAppend {
+  const void* query; /* NULL: no query */
+  const void* key;
+  const void* value;
+  long long query_strides[2], key_strides[2], value_strides[2];
+  void* out;
+  long long out_strides[2];
+  int normalize[2];
+  const float* norm_weight[2]; /* [head_dim] or NULL for unit weight */
+  float norm_offset[2];
+  float norm_eps[2];
+  const CozyRope* rope; /* NULL: no rotation */
+} CozyCacheAppend;
+
+COZY_API int cozy_cache_append(const CozyCachePlan* plan, const CozyCacheStore* store,
+                               const CozyCacheAppend* append, uintptr_t stream);
+
+/* Causal attention of a step's queries over their requests' blocks (the step's own tokens among
+ * them: append first): out = softmax(scale * q k) v over the keys up to the row's own position,
+ * and lse (natural log of the sum of exponentials, fp32 [tokens][heads_q], may be NULL). Keys in
+ * a page whose number is not in [0, pages) are left out (and bit 16 set in the plan's status); a
+ * row that sees no key is zero with lse -inf. Rows of nobody are left as they were.
+ * scale > 0. `workspace`: cozy_cache_workspace bytes of device memory, 256-byte aligned, this
+ * call's alone while it runs. */
+typedef struct CozyCacheAttend {
+  const void* query;
+  long long query_strides[2];
+  void* out;
+  long long out_strides[2];
+  float* lse;
+  float scale;
+  void* workspace;
+  long long workspace_bytes;
+} CozyCacheAttend;
+
+COZY_API long long cozy_cache_workspace(const CozyCachePlan* plan, const CozyCacheStore* store);
+COZY_API int cozy_cache_attention(const CozyCachePlan* plan, const CozyCacheStore* store,
+                                  const CozyCacheAttend* attend, uintptr_t stream);
+
 /* Name of a code returned above (a cudaError_t, or one of this library's). */
 COZY_API const char* cozy_error_name(int code);
 

@@ -29,6 +29,7 @@ enum : int {
   kPlanTokens = 4,      // more new tokens than `tokens`, or than `longest` in one request
   kPlanLengths = 8,     // a negative length, new < -1, or a ring whose cursor is not possible
   kPlanBadPage = 16,    // a page number outside [0, pages): its tokens are left out
+  kPlanTimeout = 32,    // an on-chip wait of a call of this step ran past its limit
 };
 constexpr int kPlanRefused = kPlanNoPages | kPlanNarrow | kPlanTokens | kPlanLengths;
 

@@ -1,4 +1,12 @@
-// Attention over the 8-bit paged cache (the plain form: a warp a query row and head).
+// Attention over the 8-bit paged cache.
+//
+// Few rows a key/value head (a decode step): `attend_few`. All units of work (chunks of 64 keys
+// of one head of one request) stand in one order, requests outermost, and every warp of the GPU
+// takes an equal run of them, whatever the lengths are. A run that covers an item (one head of
+// one request) writes its output; pieces of items leave fp32 rows and (max, sum) in the
+// workspace, and a second kernel, already resident when the first ends, joins them in order: no
+// atomics, the same bits every time.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -7,93 +15,1562 @@
 
 #include "../../include/cozy_ulysses.h"
 #include "cache.cuh"
+#include "sm100.cuh"
 
 namespace cozy {
 
 int cache_store_check(const CozyCacheStore& c, const CozyCachePlan& p);
 
-template <int HD>
-__global__ void __launch_bounds__(128) cache_attend_plain(const CozyCachePlan p,
-                                                          const CozyCacheStore c,
-                                                          const CozyCacheAttend a) {
-  constexpr int PER = HD / 32;
-  const int lane = threadIdx.x & 31;
-  const int heads_q = c.heads_kv * p.group;
-  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<long long>(p.tokens) * heads_q) return;
-  const int token = static_cast<int>(row / heads_q), hq = static_cast<int>(row % heads_q);
-  if (token >= p.starts[p.requests]) return;
-  int n = 0;
-  for (int low = 0, high = p.requests - 1; low <= high;) {
-    const int mid = (low + high) >> 1;
-    if (p.starts[mid] <= token) { n = mid; low = mid + 1; }
-    else high = mid - 1;
-  }
-  const int h = hq / p.group;
-  const int keys = p.lengths_after[n] - (p.starts[n + 1] - token) + 1;
-  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.query) +
-                           token * a.query_strides[0] + hq * a.query_strides[1] + lane * PER;
-  float qv[PER], o[PER];
-  for (int i = 0; i < PER; ++i) {
-    qv[i] = __bfloat162float(q[i]) * a.scale;
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int k = 0; k < keys; ++k) {
-    const int page = p.table[n * p.table_stride + k / p.page];
-    if (page < 0 || page >= p.pages) {
-      if (lane == 0) atomicOr(p.status, kPlanBadPage);
-      continue;
-    }
-    const long long block = static_cast<long long>(page) * c.heads_kv + h;
-    const long long at = (block * p.page + k % p.page) * HD + lane * PER;
-    const float ks = exponent_scale(static_cast<const int8_t*>(c.key_exponent)[block]);
-    const float vs = exponent_scale(static_cast<const int8_t*>(c.value_exponent)[block]);
-    float s = 0.f, v[PER];
-    for (int i = 0; i < PER; i += 2) {
-      uint32_t hk, hv;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hk) : "h"(*reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(c.key) + at + i)));
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hv) : "h"(*reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(c.value) + at + i)));
-      const float2 fk = __half22float2(*reinterpret_cast<const __half2*>(&hk));
-      const float2 fv = __half22float2(*reinterpret_cast<const __half2*>(&hv));
-      s = fmaf(qv[i], fk.x, fmaf(qv[i + 1], fk.y, s));
-      v[i] = fv.x * vs;
-      v[i + 1] = fv.y * vs;
-    }
-    for (int b = 16; b > 0; b >>= 1) s += __shfl_xor_sync(0xffffffffu, s, b);
-    s *= ks;
-    const float top = fmaxf(m, s), w = m == -INFINITY ? 0.f : __expf(m - top), e = __expf(s - top);
-    l = l * w + e;
-    for (int i = 0; i < PER; ++i) o[i] = fmaf(e, v[i], o[i] * w);
-    m = top;
-  }
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + token * a.out_strides[0] +
-                       hq * a.out_strides[1] + lane * PER;
-  for (int i = 0; i < PER; ++i) out[i] = __float2bfloat16(l > 0.f || l != l ? o[i] / l : 0.f);
-  if (a.lse != nullptr && lane == 0) a.lse[row] = m + logf(l);
+// What both kernels read: the plan's answers, the pool and the call.
+struct CacheArgs {
+  const int* table;
+  long long table_stride;
+  const int* starts;
+  const int* lengths;
+  const long long* units;
+  int* status;
+  int requests, pages, page, group, heads_kv;
+  const int8_t* key_exponent;
+  const int8_t* value_exponent;
+  const __nv_bfloat16* query;
+  long long q_token, q_head;
+  __nv_bfloat16* out;
+  long long o_token, o_head;
+  float* lse;
+  float scale_log2;  // softmax scale · log2(e)
+  float* ws_o;       // [worker][2][rows][HD]
+  float2* ws_ml;     // [worker][2][rows]
+  int workers;
+};
+
+// 2^15 over a row's reference: P ≤ 2^15 in f16, normal down to 2^-29 of the row's largest term.
+constexpr float kFewBias = 15.0f;
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
 }
 
-long long cache_workspace(const CozyCachePlan& p, const CozyCacheStore& c) { return 0; }
+// A bounded wait that reports through the plan's status word.
+__device__ __noinline__ bool cache_wait_slow(uint64_t* bar, uint32_t parity, int* status) {
+  const uint64_t start = global_timer_ns();
+  for (uint32_t spin = 1;; ++spin) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((spin & 63u) == 0 && global_timer_ns() - start > kWaitLimitNs) {
+      atomicOr(status, kPlanTimeout);
+      return false;
+    }
+  }
+}
 
-int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyCacheAttend& a,
+__device__ __forceinline__ bool cache_wait(uint64_t* bar, uint32_t parity, int* status) {
+  return mbar_try_wait(bar, parity) || cache_wait_slow(bar, parity, status);
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "r"(at));
+  return r;
+}
+
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
+  return r;
+}
+
+// Four codes to two pairs of f16 (exact).
+__device__ __forceinline__ void widen4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
+}
+
+// D[16 × 8] += A[16 × 16] · B[16 × 8], f16 in, fp32 accumulators.
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+      " {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Bytes of `codes` that are e4m3's NaN (0x7f or 0xff), as 0xff.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {
+  return __vcmpeq4(codes & 0x7f7f7f7fu, 0x7f7f7f7fu);
+}
+
+// The request whose units hold `u` (units of all its heads), by all lanes together: 32 places
+// of the search range are read at once, so 8192 requests take three rounds.
+__device__ __forceinline__ int request_of(const CacheArgs& a, long long u) {
+  const int lane = threadIdx.x & 31;
+  int low = 0, count = a.requests;  // the answer is in [low, low + count)
+  while (count > 1) {
+    const int step = (count + 31) / 32;
+    const int at = low + lane * step;
+    const bool before = lane * step < count && a.units[at] * a.heads_kv <= u;
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, before));
+    const int used = last * step;
+    low += used;
+    count = min(step, count - used);
+  }
+  return low;
+}
+
+// ------------------------------------------------------------------------------- few rows
+// Matrix instructions are mma.sync m16n8k16: the query rows of an item (group · new tokens, at
+// most 16) are their 16 rows, keys their columns. HBM bounds this: a chunk is 2 · 64 · HD bytes
+// and 4 · 16 · 64 · HD operations on the tensor cores, an eighth of what even these instructions
+// do in the time. Codes are widened to f16 in registers (exact) straight from the swizzled tile
+// that TMA wrote. The operand layouts are chosen so that no shuffle or transposing load is
+// needed: the contraction over channels may run in any order, so a thread's 16 consecutive
+// channels of a key serve four instructions; the keys of a tile may be taken in any order
+// (column c is row (c & 1 ? c + 4 : c) mod 8 of 8, which keeps the 16-byte reads of both K and V
+// free of bank conflicts); and V's pairs of keys are joined by byte permutes before widening.
+template <int HD>
+struct Few {
+  static constexpr int kWarps = 8;
+  static constexpr int kSlotBytes = kChunkKeys * HD;
+  static constexpr int kSlots = 24576 / kSlotBytes;  // a warp's ring: 24 KB
+  static constexpr int kMeta = 8;                    // chunks whose scales are kept
+  static constexpr int kBarOffset = kWarps * kSlots * kSlotBytes;
+  static constexpr int kMetaOffset = kBarOffset + kWarps * kSlots * 8;
+  static constexpr int kAlloc = kMetaOffset + kWarps * kMeta * 32 + 1024;
+};
+
+// A position in the order of units, moved on chunk by chunk.
+struct FewAt {
+  int n, h, j, chunks;  // request, head, chunk, chunks of an item
+  int keys;             // the request's tokens
+};
+
+__device__ __forceinline__ void few_request(const CacheArgs& a, FewAt& at, int n) {
+  at.n = n;
+  at.chunks = static_cast<int>(a.units[n + 1] - a.units[n]);
+  at.keys = a.lengths[n];
+}
+
+__device__ __forceinline__ FewAt few_at(const CacheArgs& a, long long u) {
+  FewAt at;
+  few_request(a, at, request_of(a, u));
+  const long long within = u - a.units[at.n] * a.heads_kv;
+  at.h = static_cast<int>(within / at.chunks);
+  at.j = static_cast<int>(within - static_cast<long long>(at.h) * at.chunks);
+  return at;
+}
+
+// To the next chunk; true when it belongs to another item.
+__device__ __forceinline__ bool few_next(const CacheArgs& a, FewAt& at) {
+  if (++at.j < at.chunks) return false;
+  at.j = 0;
+  if (++at.h == a.heads_kv) {
+    at.h = 0;
+    do few_request(a, at, at.n + 1);
+    while (at.chunks == 0);  // only reached while units remain
+  }
+  return true;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(256, 1)
+    attend_few(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+               const CacheArgs a) {
+  using L = Few<HD>;
+  constexpr int KSTEPS = HD / 16;  // k16 steps of Q·K
+  constexpr int XT = HD / 8;       // column tiles of the output
+  extern __shared__ uint8_t few_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(few_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * (L::kSlots * L::kSlotBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOffset) + warp * L::kSlots;
+  // scales of a chunk's up to four pages: {2^key exponent, value exponent}
+  float2* meta = reinterpret_cast<float2*>(smem + L::kMetaOffset) + warp * L::kMeta * 4;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const long long total = a.units[a.requests] * a.heads_kv;
+  const int workers = static_cast<int>(min(static_cast<long long>(a.workers), total));
+  const int worker = warp * gridDim.x + blockIdx.x;
+  if (worker >= workers) return;  // warps share nothing
+  const long long u0 = worker * total / workers, u1 = (worker + 1) * total / workers;
+  if (lane == 0) {
+    for (int i = 0; i < L::kSlots; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+
+  // ---- the loads: fill f is the keys (even) or values (odd) of unit u0 + f / 2
+  const int box = min(a.page, kChunkKeys), per_chunk = kChunkKeys / box;
+  const long long fills = 2 * (u1 - u0);
+  FewAt to = few_at(a, u0);  // the chunk to load next
+  FewAt at = to;             // the chunk to compute
+  int batch = 0, id = -1, ids = 0;      // a lane's page number among 32 of the item's
+  float key_scale = 1.f, value_e = 0.f;
+  bool fresh = true;
+  auto load = [&](long long f) {
+    if (f >= fills) return;
+    const int slot = static_cast<int>(f % L::kSlots);
+    const int first = a.page > kChunkKeys ? to.j * kChunkKeys / a.page : to.j * per_chunk;
+    const int offset = a.page > kChunkKeys ? to.j * kChunkKeys % a.page : 0;
+    const int count = min(per_chunk, (to.keys - to.j * kChunkKeys + box - 1) / box);
+    if ((f & 1) == 0) {
+      if (fresh || first + per_chunk > batch + 32) {
+        fresh = false;
+        batch = first;
+        id = -1;
+        key_scale = 1.f;
+        value_e = 0.f;
+        const int index = first + lane;
+        if (index * static_cast<long long>(a.page) < to.keys) {
+          id = a.table[to.n * a.table_stride + index];
+          if (id < 0 || id >= a.pages) {
+            id = -1;
+            atomicOr(a.status, kPlanBadPage);
+          } else {
+            const long long block = static_cast<long long>(id) * a.heads_kv + to.h;
+            key_scale = exponent_scale(a.key_exponent[block]);
+            value_e = static_cast<float>(a.value_exponent[block]);
+          }
+        }
+      }
+      // the chunk's scales; a page that is not there has a scale of zero
+      const int from = first - batch + (lane & 3);
+      const float ks = __shfl_sync(0xffffffffu, key_scale, from & 31);
+      const float ve = __shfl_sync(0xffffffffu, value_e, from & 31);
+      ids = __shfl_sync(0xffffffffu, id, from & 31);
+      if (lane >= count) ids = -1;
+      if (lane < per_chunk)
+        meta[(f >> 1) % L::kMeta * 4 + lane] = make_float2(ids < 0 ? 0.f : ks, ve);
+    }
+    const unsigned there = __ballot_sync(0xffffffffu, lane < per_chunk && ids >= 0);
+    if (lane == 0) mbar_expect_tx(&full[slot], __popc(there) * box * HD);
+    __syncwarp();
+    if (lane < per_chunk && ids >= 0)
+      tma_load_2d(ring + slot * L::kSlotBytes + lane * box * HD, (f & 1) ? &tm_v : &tm_k,
+                  &full[slot], 0, (ids * a.heads_kv + to.h) * a.page + offset);
+    if (f & 1) {
+      if (f + 1 < fills) fresh |= few_next(a, to);
+    }
+  };
+  for (int f = 0; f < L::kSlots; ++f) load(f);
+
+  const int order = (g & 1) ? ((g + 4) & 7) : g;  // row of this lane's column of K
+  const uint32_t base = smem_u32(ring);
+  uint32_t k_off[HD / 64];
+#pragma unroll
+  for (int c = 0; c < HD / 64; ++c)
+    k_off[c] = HD == 128 ? order * 128 + (((t + 4 * c) ^ order) << 4)
+                         : order * 64 + ((t ^ ((order >> 1) & 3)) << 4);
+  const int row0 = 2 * t, row1 = (2 * t + 5) & 7;  // rows of columns 2t and 2t + 1
+  uint32_t v_off[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = i ? row1 : row0;
+    v_off[i] = HD == 128 ? r * 128 + ((g ^ r) << 4)
+                         : r * 64 + (((g >> 1) ^ ((r >> 1) & 3)) << 4) + (g & 1) * 8;
+  }
+
+  bool ok = true;
+  long long u = u0;
+  while (u < u1 && ok) {
+    // ---- an item, or the part of it that this worker has
+    const int first_token = a.starts[at.n];
+    const int added = a.starts[at.n + 1] - first_token;
+    const int rows = added * a.group;
+    const int seen0 = at.keys - added;  // keys before the step's own
+    const int j0 = at.j;
+    const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.chunks - at.j)));
+    // rows g and g + 8: query times a power of two that puts its largest value in [2^14, 2^15)
+    uint32_t q[KSTEPS][4];
+    float mul[2];
+    int last[2];  // the last key that each row sees
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = g + 8 * i;
+      last[i] = seen0 + min(row, rows - 1) / a.group;
+      uint4 x[HD / 64][2];
+      float amax = 0.f;
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          x[c][k] = make_uint4(0, 0, 0, 0);
+          if (row < rows)
+            x[c][k] = *reinterpret_cast<const uint4*>(
+                a.query + (first_token + row / a.group) * a.q_token +
+                (at.h * a.group + row % a.group) * a.q_head + (t + 4 * c) * 16 + k * 8);
+          const uint32_t w[4] = {x[c][k].x, x[c][k].y, x[c][k].z, x[c][k].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            amax = fmaxf(amax, fabsf(__uint_as_float(w[e] << 16)));
+            amax = fmaxf(amax, fabsf(__uint_as_float(w[e] & 0xffff0000u)));
+          }
+        }
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const int up = min(100, 14 + 127 - static_cast<int>(__float_as_uint(amax) >> 23));
+      const float s = exponent_scale(up);
+      mul[i] = a.scale_log2 * exponent_scale(-up);
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t w[4] = {x[c][k].x, x[c][k].y, x[c][k].z, x[c][k].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // words 2i, 2i + 1 of the 8 a chunk: registers {row, row + 8} × {low, high} of step i
+            const int word = k * 4 + e;
+            q[c * 4 + word / 2][(word & 1) * 2 + i] =
+                f16_pair(__uint_as_float(w[e] << 16) * s, __uint_as_float(w[e] & 0xffff0000u) * s);
+          }
+        }
+      }
+    }
+    float o[XT][4];
+#pragma unroll
+    for (int x = 0; x < XT; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int step = 0; step < steps; ++step, ++u) {
+      const long long f = 2 * (u - u0);
+      int slot = static_cast<int>(f % L::kSlots);
+      if (!(ok = __all_sync(0xffffffffu, cache_wait(&full[slot], (f / L::kSlots) & 1, a.status)))) break;
+      const float2* scales = meta + (f >> 1) % L::kMeta * 4;
+      const int key0 = (j0 + step) * kChunkKeys;
+      // ---- scores
+      float s[8][4];
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) {
+          const uint4 k = lds128(base + slot * L::kSlotBytes + nt * 8 * HD + k_off[c]);
+          const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t b0, b1;
+            widen4(w[e], b0, b1);
+            mma16816(s[nt], q[c * 4 + e], b0, b1);
+          }
+        }
+      }
+      __syncwarp();
+      // the scales are read before the ring of chunks moves on
+      float2 sc[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[i] = scales[i < per_chunk ? i : 0];
+      __syncwarp();
+      load(f + L::kSlots);
+      bool whole = key0 + kChunkKeys <= seen0 + 1;  // every row sees every key
+#pragma unroll
+      for (int i = 0; i < 4; ++i) whole = whole && sc[i].x != 0.f;
+      float top[2] = {m[0], m[1]};
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 x = per_chunk == 4 ? sc[nt / 2] : per_chunk == 2 ? sc[nt / 4] : sc[0];
+        const float f0 = mul[0] * x.x, f1 = mul[1] * x.x;
+        s[nt][0] = fmaf(s[nt][0], f0, x.y);
+        s[nt][1] = fmaf(s[nt][1], f0, x.y);
+        s[nt][2] = fmaf(s[nt][2], f1, x.y);
+        s[nt][3] = fmaf(s[nt][3], f1, x.y);
+        if (!whole) {
+          const int ka = key0 + nt * 8 + row0, kb = key0 + nt * 8 + row1;
+          const bool gone = x.x == 0.f;
+          if (gone || ka > last[0]) s[nt][0] = -INFINITY;
+          if (gone || kb > last[0]) s[nt][1] = -INFINITY;
+          if (gone || ka > last[1]) s[nt][2] = -INFINITY;
+          if (gone || kb > last[1]) s[nt][3] = -INFINITY;
+        }
+        top[0] = fmaxf(top[0], fmaxf(s[nt][0], s[nt][1]));
+        top[1] = fmaxf(top[1], fmaxf(s[nt][2], s[nt][3]));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      }
+      if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+        float w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          w[i] = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - top[i]);
+          l[i] *= w[i];
+          m[i] = top[i];
+        }
+#pragma unroll
+        for (int x = 0; x < XT; ++x) {
+          o[x][0] *= w[0];
+          o[x][1] *= w[0];
+          o[x][2] *= w[1];
+          o[x][3] *= w[1];
+        }
+      }
+      const float r0 = (m[0] == -INFINITY ? 0.f : m[0]) - kFewBias;
+      const float r1 = (m[1] == -INFINITY ? 0.f : m[1]) - kFewBias;
+      // weights 2^(s + e - m), their sum without the value's 2^e
+      uint32_t p[4][4];
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 x = per_chunk == 4 ? sc[nt / 2] : per_chunk == 2 ? sc[nt / 4] : sc[0];
+        const float back = exponent_scale(-static_cast<int>(x.y));
+        const float p0 = ex2_approx(s[nt][0] - r0), p1 = ex2_approx(s[nt][1] - r0);
+        const float p2 = ex2_approx(s[nt][2] - r1), p3 = ex2_approx(s[nt][3] - r1);
+        l[0] = fmaf(p0 + p1, back, l[0]);
+        l[1] = fmaf(p2 + p3, back, l[1]);
+        p[nt / 2][(nt & 1) * 2] = f16_pair(p0, p1);
+        p[nt / 2][(nt & 1) * 2 + 1] = f16_pair(p2, p3);
+      }
+      // ---- values
+      slot = static_cast<int>((f + 1) % L::kSlots);
+      if (!(ok = __all_sync(0xffffffffu, cache_wait(&full[slot], ((f + 1) / L::kSlots) & 1, a.status)))) break;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        constexpr int WORDS = HD / 32;  // words of 4 channels a thread and key
+        uint32_t v[4][WORDS];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // keys row0, row1, 8 + row0, 8 + row1 of 16
+          const uint32_t from = base + slot * L::kSlotBytes + (kk * 16 + (i >> 1) * 8) * HD + v_off[i & 1];
+          if constexpr (HD == 128) {
+            const uint4 x = lds128(from);
+            v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
+          } else {
+            const uint2 x = lds64(from);
+            v[i][0] = x.x; v[i][1] = x.y;
+          }
+        }
+        if (!whole) {
+          // Codes behind the last key of the request and in pages that are not there are whatever
+          // they are, and a NaN that some row does not see must not reach it as 0 · NaN: both
+          // become zeros here, and rows that do see a NaN get it by a product of ones.
+          uint32_t any = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at16 = kk * 16 + (i >> 1) * 8 + ((i & 1) ? row1 : row0);
+            const float2 x = per_chunk == 4 ? sc[kk] : per_chunk == 2 ? sc[kk / 2] : sc[0];
+            const bool gone = x.x == 0.f || key0 + at16 >= at.keys;
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) {
+              if (gone) v[i][w] = 0;
+              any |= nan_bytes(v[i][w]);
+            }
+          }
+          if (__any_sync(0xffffffffu, any != 0)) {
+            uint32_t see[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // a row's keys of the two column pairs
+              const int k = key0 + kk * 16 + (i >> 1) * 8, to_row = last[i & 1];
+              see[i] = f16_pair(k + row0 <= to_row ? 1.f : 0.f, k + row1 <= to_row ? 1.f : 0.f);
+            }
+#pragma unroll
+            for (int x = 0; x < XT; ++x) {
+              const int w = x / 4, sh = (x & 3) * 8;
+              auto one = [&](int i) { return (nan_bytes(v[i][w]) >> sh & 0xffu) ? 0x3c00u : 0u; };
+              float hit[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816(hit, see, one(0) | one(1) << 16, one(2) | one(3) << 16);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (hit[i] > 0.f) o[x][i] = __uint_as_float(0x7fc00000u);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int w = 0; w < WORDS; ++w) v[i][w] &= ~nan_bytes(v[i][w]);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+          uint32_t b0[4], b1[4];
+          widen4(__byte_perm(v[0][w], v[1][w], 0x5140), b0[0], b0[1]);
+          widen4(__byte_perm(v[0][w], v[1][w], 0x7362), b0[2], b0[3]);
+          widen4(__byte_perm(v[2][w], v[3][w], 0x5140), b1[0], b1[1]);
+          widen4(__byte_perm(v[2][w], v[3][w], 0x7362), b1[2], b1[3]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mma16816(o[w * 4 + x], p[kk], b0[x], b1[x]);
+        }
+      }
+      __syncwarp();
+      load(f + 1 + L::kSlots);
+    }
+    if (!ok) break;
+    // ---- the item's end: this thread has channels [t · HD / 4, + HD / 4) of rows g and g + 8
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      const int row = g + 8 * i;
+      if (row >= rows) continue;
+      if (steps == at.chunks) {
+        const int token = first_token + row / a.group, head = at.h * a.group + row % a.group;
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+        uint4* to_row = reinterpret_cast<uint4*>(a.out + token * a.o_token + head * a.o_head + t * (HD / 4));
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int x = 0; x < XT; x += 8)
+            to_row[(c * XT + x) / 8] = make_uint4(
+                pack_bf16x2(o[x][2 * i + c] * inv, o[x + 1][2 * i + c] * inv),
+                pack_bf16x2(o[x + 2][2 * i + c] * inv, o[x + 3][2 * i + c] * inv),
+                pack_bf16x2(o[x + 4][2 * i + c] * inv, o[x + 5][2 * i + c] * inv),
+                pack_bf16x2(o[x + 6][2 * i + c] * inv, o[x + 7][2 * i + c] * inv));
+        if (a.lse != nullptr && t == 0)
+          a.lse[static_cast<long long>(token) * a.heads_kv * a.group + head] =
+              l[i] == 0.f ? -INFINITY : 0.6931471805599453f * (m[i] - kFewBias + __log2f(l[i]));
+      } else {
+        const long long part = (2LL * worker + (j0 == 0 ? 1 : 0)) * kRowsFew + row;
+        float4* to_row = reinterpret_cast<float4*>(a.ws_o + part * HD + t * (HD / 4));
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int x = 0; x < XT; x += 4)
+            to_row[(c * XT + x) / 4] = make_float4(o[x][2 * i + c], o[x + 1][2 * i + c],
+                                                   o[x + 2][2 * i + c], o[x + 3][2 * i + c]);
+        if (t == 0) a.ws_ml[part] = make_float2(m[i], l[i]);
+      }
+    }
+    at.j += steps - 1;
+    if (u < u1) few_next(a, at);
+  }
+  if (!ok) {  // copies in flight land before the warp leaves
+    const long long f = 2 * (u - u0);
+    for (long long i = f; i < f + 2 * L::kSlots && i < fills; ++i)
+      cache_wait_slow(&full[i % L::kSlots], (i / L::kSlots) & 1, a.status);
+  }
+}
+
+// Joins the parts of an item that several workers had: block (item, row), 8 warps over the
+// parts, in a fixed order.
+template <int HD>
+__global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
+  constexpr int PER = HD / 32;  // channels a lane
+  __shared__ float sum_o[8][HD];
+  __shared__ float2 sum_ml[8];
+  const int n = blockIdx.x / a.heads_kv, h = blockIdx.x % a.heads_kv, row = blockIdx.y;
+  const int rows = (a.starts[n + 1] - a.starts[n]) * a.group;
+  const long long chunks = a.units[n + 1] - a.units[n];
+  const long long total = a.units[a.requests] * a.heads_kv;
+  const long long workers = min(static_cast<long long>(a.workers), total);
+  const long long u0 = a.units[n] * a.heads_kv + h * chunks;
+  const int first = total == 0 ? 0 : static_cast<int>(((u0 + 1) * workers - 1) / total);
+  const int last = total == 0 ? 0 : static_cast<int>(((u0 + chunks) * workers - 1) / total);
+  const bool split = row < rows && first != last;
+  // one block at least waits, so that this grid does not end before the one it follows
+  if (split || (blockIdx.x == 0 && blockIdx.y == 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!split) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float o[PER], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = 0.f;
+#pragma unroll 4
+  for (int w = first + warp; w <= last; w += 8) {
+    const long long part = (2LL * w + (w == first ? 1 : 0)) * kRowsFew + row;
+    const float2 ml = __ldcg(&a.ws_ml[part]);
+    float x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = __ldcg(&a.ws_o[part * HD + i * 32 + lane]);
+    const float top = fmaxf(m, ml.x);
+    const float mine = m == -INFINITY ? 0.f : ex2_approx(m - top);
+    const float other = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+    m = top;
+    // a part without a key has zeros; one whose scores are NaN has a sum of NaN
+    l = l * mine + ml.y * (ml.x == -INFINITY ? 1.f : other);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = o[i] * mine + x[i] * (ml.x == -INFINITY ? 1.f : other);
+  }
+  if (lane == 0) sum_ml[warp] = make_float2(m, l);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum_o[warp][i * 32 + lane] = o[i];
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= HD) return;
+  float top = -INFINITY;
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, sum_ml[w].x);
+  float value = 0.f, sum = 0.f;
+  for (int w = 0; w < 8; ++w) {
+    const float mine = sum_ml[w].x == -INFINITY ? 1.f : ex2_approx(sum_ml[w].x - top);
+    value += sum_o[w][d] * mine;
+    sum += sum_ml[w].y * mine;
+  }
+  const int token = a.starts[n] + row / a.group, head = h * a.group + row % a.group;
+  a.out[token * a.o_token + head * a.o_head + d] = __float2bfloat16(sum == 0.f ? 0.f : value / sum);
+  if (a.lse != nullptr && d == 0)
+    a.lse[static_cast<long long>(token) * a.heads_kv * a.group + head] =
+        sum == 0.f ? -INFINITY : 0.6931471805599453f * (top - kFewBias + __log2f(sum));
+}
+
+// ------------------------------------------------------------------------------ many rows
+// Items of up to 256 query rows (whole tokens of one head's group) over tiles of 128 keys, on
+// the 5th-generation tensor cores: two query tiles of 128 rows take turns, so that one's softmax
+// runs while the other's products do. Every CTA takes an equal run of all units, item after item
+// (one head's items are neighbours and share its keys in L2).
+//
+//   warps 0-3, 4-7  softmax of query tile 0, 1 (a thread a row, a TMEM lane)
+//   warp  8         page numbers, scales, and TMA of K and V codes into their rings
+//   warp  9         the matrix instructions
+//   warps 10, 11    V's codes widened to f16 (exact)
+//
+// S = Q·Kᵀ runs in 8 bits on K's codes as they are stored, with Q split into two e4m3 parts
+// under one power of two a row: q = hi + lo holds all 8 bits of a bf16 that is not below 2^-11 of
+// its row's largest value, and a smaller one to 2^-19 of that. Two 8-bit products cost what one
+// 16-bit product costs, and K needs neither widening nor more than its stored bytes of shared
+// memory. P stays in f16 (11 bits; two 8-bit parts would lose the weights under 2^-17 of a row's
+// largest, which a long context has many of), so V is widened.
+//
+// Tensor memory: S/P of the two tiles at columns 0 and 128, O at 256 and 256 + HD.
+template <int HD>
+struct Many {
+  static constexpr int kThreads = 384;
+  static constexpr int kKStages = 3, kV8Stages = 2, kV16Stages = 2;
+  static constexpr int kScaleRing = 8;
+  static constexpr int kCodeTile = 128 * HD;      // 128 rows of codes
+  static constexpr int kQOffset = 0;              // [tile][hi, lo]
+  static constexpr int kKOffset = 4 * kCodeTile;
+  static constexpr int kV8Offset = kKOffset + kKStages * kCodeTile;
+  static constexpr int kV16Offset = kV8Offset + kV8Stages * kCodeTile;
+  static constexpr int kPoisonOffset = kV16Offset + kV16Stages * 2 * kCodeTile;  // [256 rows][16]
+  static constexpr int kNanOffset = kPoisonOffset + 256 * 16;  // [V16 slot][128 keys][16 bytes]
+  static constexpr int kScaleOffset = kNanOffset + kV16Stages * 128 * 16;
+  // [ring]{2^key exponent [8], value exponent [8], 2^-value exponent [8], gone groups, pad}
+  static constexpr int kScaleBytes = 112;
+  static constexpr int kBarOffset = kScaleOffset + kScaleRing * kScaleBytes;
+  static constexpr int kBars = 2 + 2 * kKStages + 2 * kV8Stages + 2 * kV16Stages + 2 + 4 + 2 +
+                               kScaleRing + 1;
+  static constexpr int kMiscOffset = kBarOffset + kBars * 8;
+  static constexpr int kAlloc = kMiscOffset + 32 + 1024;
+};
+// Registers: 384 threads start with 168 each; 256 · 208 + 128 · 80 = 63488 ≤ 64512.
+constexpr int kManySoftmaxRegs = 208;
+constexpr int kManyOtherRegs = 80;
+
+// P = 2^(s - m + 7) against a reference that may lie 2^8 below the row's largest (O is rescaled
+// only when the maximum grew by more): at most 2^15 in f16, normal down to 2^-21 of the reference.
+constexpr float kManyBias = 7.0f;
+constexpr float kManySlack = 8.0f;
+
+// A group's multiplier of scores: never zero, so that a hidden score's -inf stays one (products
+// below 2^-120 are scores of nothing either way).
+__device__ __forceinline__ float group_mul(float mul, float key_scale) {
+  return fmaxf(mul * key_scale, 7.52316385e-37f);
+}
+
+struct ManyAt {
+  int n, h, item, j;  // request, head, item, tile of keys
+  int items, tiles;   // items of the request's head, tiles of this item
+  int keys, cached, added, first_token;
+};
+
+__device__ __forceinline__ void many_item(const CacheArgs& a, ManyAt& at) {
+  const int per = kRowsMany / a.group;
+  at.tiles = (at.cached + min((at.item + 1) * per, at.added) + kTileKeys - 1) / kTileKeys;
+}
+
+__device__ __forceinline__ void many_request(const CacheArgs& a, ManyAt& at, int n) {
+  const int per = kRowsMany / a.group;
+  at.n = n;
+  at.first_token = a.starts[n];
+  at.added = a.starts[n + 1] - at.first_token;
+  at.keys = a.lengths[n];
+  at.cached = at.keys - at.added;
+  at.items = (at.added + per - 1) / per;
+}
+
+__device__ __forceinline__ ManyAt many_at(const CacheArgs& a, long long u) {
+  ManyAt at;
+  many_request(a, at, request_of(a, u));
+  const long long units = a.units[at.n + 1] - a.units[at.n];
+  const long long within = u - a.units[at.n] * a.heads_kv;
+  at.h = static_cast<int>(within / units);
+  const long long rest = within - at.h * units;
+  int low = 0, high = at.items - 1;
+  while (low < high) {
+    const int mid = (low + high + 1) >> 1;
+    if (tiles_before(a.group, at.cached, mid) <= rest) low = mid;
+    else high = mid - 1;
+  }
+  at.item = low;
+  at.j = static_cast<int>(rest - tiles_before(a.group, at.cached, low));
+  many_item(a, at);
+  return at;
+}
+
+// To the first tile of the next item.
+__device__ __forceinline__ void many_next(const CacheArgs& a, ManyAt& at) {
+  at.j = 0;
+  if (++at.item == at.items) {
+    at.item = 0;
+    if (++at.h == a.heads_kv) {
+      at.h = 0;
+      do many_request(a, at, at.n + 1);
+      while (at.added == 0);  // only reached while units remain
+    }
+  }
+  many_item(a, at);
+}
+
+__device__ __forceinline__ int many_rows(const CacheArgs& a, const ManyAt& at) {
+  const int per = kRowsMany / a.group;
+  return min(per, at.added - at.item * per) * a.group;
+}
+
+__device__ __forceinline__ bool many_wait(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                          int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t start = global_timer_ns();
+  for (uint32_t spin = 1;; ++spin) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((spin & 63u) == 0) {
+      if (*abort) return false;
+      if (global_timer_ns() - start > kWaitLimitNs) {
+        *abort = 1;
+        atomicOr(status, kPlanTimeout);
+        return false;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ bool many_warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                               int* status) {
+  return __all_sync(0xffffffffu, many_wait(bar, parity, abort, status));
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(pred));
+  return pred != 0;
+}
+
+__device__ __forceinline__ void fence_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+__device__ __forceinline__ void tie(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31]));
+}
+
+__device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+
+// Descriptor of a K-major tile of codes: rows of HD bytes in the swizzle of that width
+// (layout type 2: 128 bytes, 4: 64 bytes), 8 rows an atom.
+template <int HD>
+__device__ __forceinline__ uint64_t code_desc(uint32_t at) {
+  uint64_t d = static_cast<uint64_t>((at & 0x3FFFFu) >> 4);
+  d |= 1ull << 16;
+  d |= static_cast<uint64_t>((8 * HD) >> 4) << 32;
+  d |= 1ull << 46;
+  d |= (HD == 128 ? 2ull : 4ull) << 61;
+  return d;
+}
+
+// Sixteen scores (a group under one scale) to weights 2^(s · mul + add) in f16 pairs.
+__device__ __forceinline__ void weigh16(const uint32_t* r, float mul, float add, float2& acc,
+                                        uint32_t* pk) {
+  const float2 m2 = make_float2(mul, mul), a2 = make_float2(add, add);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 s = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    const float2 x = __ffma2_rn(s, m2, a2);
+    const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+    acc = __fadd2_rn(acc, e);
+    pk[i] = f16_pair(e.x, e.y);
+  }
+}
+
+__device__ __forceinline__ float max16(const uint32_t* r) {
+  float a = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  float b = fmaxf(__uint_as_float(r[2]), __uint_as_float(r[3]));
+#pragma unroll
+  for (int i = 4; i < 16; i += 4) {
+    a = fmaxf(a, fmaxf(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+    b = fmaxf(b, fmaxf(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])));
+  }
+  return fmaxf(a, b);
+}
+
+// Columns past `limit` (relative to the chunk; may be negative) and of groups that are not
+// there (bits 0 and 1 of `gone`) become -inf.
+__device__ __forceinline__ void hide32(uint32_t (&r)[32], int limit, int gone) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (i > limit || (gone >> (i / 16) & 1)) r[i] = 0xff800000u;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(384, 1)
+    attend_many(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                const CacheArgs a) {
+  using L = Many<HD>;
+  extern __shared__ uint8_t many_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(many_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kBarOffset);
+  uint64_t* q_ready = bar;
+  uint64_t* k_full = q_ready + 2;
+  uint64_t* k_empty = k_full + L::kKStages;
+  uint64_t* v8_full = k_empty + L::kKStages;
+  uint64_t* v8_empty = v8_full + L::kV8Stages;
+  uint64_t* v16_full = v8_empty + L::kV8Stages;
+  uint64_t* v16_empty = v16_full + L::kV16Stages;
+  uint64_t* s_full = v16_empty + L::kV16Stages;
+  uint64_t* p_ready = s_full + 2;  // [tile][half]
+  uint64_t* o_final = p_ready + 4;
+  uint64_t* scale_full = o_final + 2;
+  uint64_t* drain = scale_full + L::kScaleRing;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOffset);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 4);
+  volatile int* nan_tile = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 8);  // [slot]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const long long total = a.units[a.requests] * a.heads_kv;
+  const int workers = static_cast<int>(min(static_cast<long long>(a.workers), total));
+  if (static_cast<int>(blockIdx.x) >= workers) return;
+  const long long u0 = blockIdx.x * total / workers, u1 = (blockIdx.x + 1) * total / workers;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_ready[i], 128);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[2 * i], 128);
+      mbar_init(&p_ready[2 * i + 1], 128);
+      mbar_init(&o_final[i], 1);
+    }
+    for (int i = 0; i < L::kKStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < L::kV8Stages; ++i) {
+      mbar_init(&v8_full[i], 1);
+      mbar_init(&v8_empty[i], 64);
+    }
+    for (int i = 0; i < L::kV16Stages; ++i) {
+      mbar_init(&v16_full[i], 64);
+      mbar_init(&v16_empty[i], 1);
+      nan_tile[i] = 0;
+    }
+    for (int i = 0; i < L::kScaleRing; ++i) mbar_init(&scale_full[i], 1);
+    mbar_init(drain, 1);
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManySoftmaxRegs));
+    const int s = warp >> 2;
+    const int row128 = threadIdx.x & 127;
+    const uint32_t lane_bits = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lane_bits + static_cast<uint32_t>(s * 128);
+    const uint32_t tO = tmem + lane_bits + 256u + static_cast<uint32_t>(s * HD);
+    uint4* poison = reinterpret_cast<uint4*>(smem + L::kPoisonOffset) + threadIdx.x;
+    int block = 0, mine = 0, segment = 0;  // tiles of keys seen; by this query tile; items of it
+    bool ok = true;
+    ManyAt at = many_at(a, u0);
+    for (long long u = u0; u < u1;) {
+      const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.tiles - at.j)));
+      const int rows = many_rows(a, at);
+      if (s * 128 < rows) {
+        const int per = kRowsMany / a.group;
+        const int row = s * 128 + row128;
+        const int token = at.item * per + min(row, rows - 1) / a.group;  // of the request
+        const int last = at.cached + token;                              // the last key it sees
+        float mul;
+        {  // ---- this row of Q as two e4m3 parts
+          const __nv_bfloat16* from = a.query + (at.first_token + token) * a.q_token +
+                                      (at.h * a.group + min(row, rows - 1) % a.group) * a.q_head;
+          uint4 x[HD / 8];
+          float amax = 0.f;
+#pragma unroll
+          for (int c = 0; c < HD / 8; ++c) {
+            x[c] = row < rows ? *reinterpret_cast<const uint4*>(from + c * 8) : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              amax = fmaxf(amax, fabsf(__uint_as_float(w[e] << 16)));
+              amax = fmaxf(amax, fabsf(__uint_as_float(w[e] & 0xffff0000u)));
+            }
+          }
+          // the largest value in [224, 448]: 448 = 1.75 · 2^8
+          const int e = max(-100, static_cast<int>((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8);
+          const float up = exponent_scale(-e);
+          mul = a.scale_log2 * exponent_scale(e);
+          const uint32_t hi_at = smem_u32(smem + L::kQOffset + s * 2 * L::kCodeTile);
+          const uint32_t lo_at = hi_at + L::kCodeTile;
+#pragma unroll
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint4 v = x[2 * c + (k >> 1)];
+              const uint32_t w[2] = {(k & 1) ? v.z : v.x, (k & 1) ? v.w : v.y};
+              uint32_t parts[2][2];
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                float f0 = __uint_as_float(w[b] << 16) * up, f1 = __uint_as_float(w[b] & 0xffff0000u) * up;
+                // an infinity has no parts: its row is NaN, as its softmax is
+                if (!(fabsf(f0) <= 448.f)) f0 = __uint_as_float(0x7fc00000u);
+                if (!(fabsf(f1) <= 448.f)) f1 = __uint_as_float(0x7fc00000u);
+                uint16_t h, l;
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h) : "f"(f0), "f"(f1));
+                uint32_t back;
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
+                const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&back));
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(l) : "f"(f0 - g.x), "f"(f1 - g.y));
+                parts[0][b] = h;
+                parts[1][b] = l;
+              }
+              hi[k] = parts[0][0] | parts[0][1] << 16;
+              lo[k] = parts[1][0] | parts[1][1] << 16;
+            }
+            const uint32_t off = HD == 128 ? row128 * 128 + ((c ^ (row128 & 7)) << 4)
+                                           : row128 * 64 + ((c ^ ((row128 >> 1) & 3)) << 4);
+            sts128(hi_at + off, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            sts128(lo_at + off, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+          }
+          *poison = make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+          mbar_arrive(&q_ready[s]);
+        }
+        float m = -INFINITY, l = 0.f;
+        const int first_seen = at.cached + at.item * per;  // the item's first token's last key
+        for (int step = 0; step < steps; ++step, ++block, ++mine) {
+          const float* scales = reinterpret_cast<const float*>(
+              smem + L::kScaleOffset + (block % L::kScaleRing) * L::kScaleBytes);
+          if (!many_wait(&s_full[s], mine & 1, abort, a.status) ||
+              !many_wait(&scale_full[block % L::kScaleRing], (block / L::kScaleRing) & 1, abort, a.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          uint32_t r[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, r[c]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tie(r[c]);
+          const int key0 = (at.j + step) * kTileKeys;
+          const int gone = reinterpret_cast<const int*>(scales)[24];
+          const bool partial = key0 + kTileKeys > first_seen + 1 || gone != 0;
+          if (partial) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) hide32(r[c], last - key0 - c * 32, gone >> (2 * c));
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            top = fmaxf(top, fmaf(max16(&r[c >> 1][(c & 1) * 16]), group_mul(mul, scales[c]), scales[8 + c]));
+          const float m_new = fmaxf(m, top);
+          if (__any_sync(0xffffffffu, m != -INFINITY && m_new > m + kManySlack)) {
+            // the commit behind s_full covers every earlier product of this tile
+            const float w = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
+            l *= w;
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + c * 32, o);
+              tmem_wait_ld();
+              tie(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w);
+              tmem_st32(tO + c * 32, o);
+            }
+            m = m_new;
+          }
+          if (m == -INFINITY) m = m_new;
+          const float ref = (m == -INFINITY ? 0.f : m) - kManyBias;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int group = half * 4 + c * 2 + e;
+                float2 acc = make_float2(0.f, 0.f);
+                weigh16(&r[half * 2 + c][e * 16], group_mul(mul, scales[group]), scales[8 + group] - ref,
+                        acc, pk + 8 * e);
+                l = fmaf(acc.x + acc.y, scales[16 + group], l);
+              }
+              tmem_st16(tS + half * 32 + c * 16, pk);
+            }
+            if (half == 1 && partial) {
+              // values that are NaN in a tile that some row does not see whole: those rows that
+              // see the key take the NaN, in their channels, at the end
+              const int slot = block % L::kV16Stages;
+              if (!many_wait(&v16_full[slot], (block / L::kV16Stages) & 1, abort, a.status)) ok = false;
+              else if (nan_tile[slot] == block + 1) {
+                const uint4* bits = reinterpret_cast<const uint4*>(smem + L::kNanOffset) + slot * 128;
+                uint4 p = *poison;
+                for (int k = 0; k < kTileKeys && key0 + k <= last; ++k) {
+                  p.x |= bits[k].x;
+                  p.y |= bits[k].y;
+                  p.z |= bits[k].z;
+                  p.w |= bits[k].w;
+                }
+                *poison = p;
+              }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_ready[2 * s + half]);
+          }
+        }
+        if (ok) ok = many_wait(&o_final[s], segment & 1, abort, a.status);
+        tc_fence_after();
+        if (!ok) break;
+        ++segment;
+        // ---- the item's end, or this worker's part of it
+        const bool whole = steps == at.tiles;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const long long part = 2LL * blockIdx.x + (at.j == 0 ? 1 : 0);
+        const int head = at.h * a.group + row % a.group;
+        __nv_bfloat16* to = a.out + (at.first_token + token) * a.o_token + head * a.o_head;
+        float4* ws = reinterpret_cast<float4*>(a.ws_o) + part * (HD / 4) * kRowsMany + row;
+        const uint4 p = *poison;
+        const bool nan = (p.x | p.y | p.z | p.w) != 0;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_wait_ld();
+          tie(o);
+          if (nan) {
+            const uint32_t bits = c == 0 ? p.x : c == 1 ? p.y : c == 2 ? p.z : p.w;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (bits >> i & 1) o[i] = 0x7fc00000u;
+          }
+          if (row < rows) {
+            if (whole) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  w[k] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * k]) * inv,
+                                     __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+                *reinterpret_cast<uint4*>(to + c * 32 + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                ws[(c * 8 + i) * kRowsMany] =
+                    make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+            }
+          }
+        }
+        tc_fence_before();
+        if (row < rows) {
+          if (!whole) a.ws_ml[part * kRowsMany + row] = make_float2(m, l);
+          else if (a.lse != nullptr)
+            a.lse[static_cast<long long>(at.first_token + token) * a.heads_kv * a.group + head] =
+                l == 0.f ? -INFINITY : 0.6931471805599453f * (m - kManyBias + __log2f(l));
+        }
+      } else {
+        block += steps;
+      }
+      u += steps;
+      if (u < u1) many_next(a, at);
+    }
+  } else if (warp == 8) {
+    // -------------------------------------------------------------- page numbers and copies
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyOtherRegs));
+    const int box = min(a.page, kTileKeys), per_tile = kTileKeys / box;
+    int block = 0;
+    bool ok = true;
+    ManyAt at = many_at(a, u0);
+    for (long long u = u0; u < u1 && ok;) {
+      const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.tiles - at.j)));
+      int batch = 0, id = -1;
+      float key_scale = 1.f, value_e = 0.f;
+      for (int step = 0; step < steps; ++step, ++block) {
+        const int key0 = (at.j + step) * kTileKeys;
+        const int first = key0 / a.page;
+        if (step == 0 || first + per_tile > batch + 32) {  // 32 pages' numbers and scales at once
+          batch = first;
+          id = -1;
+          key_scale = 1.f;
+          value_e = 0.f;
+          const int index = first + lane;
+          if (index * static_cast<long long>(a.page) < at.keys) {
+            id = a.table[at.n * a.table_stride + index];
+            if (id < 0 || id >= a.pages) {
+              id = -1;
+              atomicOr(a.status, kPlanBadPage);
+            } else {
+              const long long at_block = static_cast<long long>(id) * a.heads_kv + at.h;
+              key_scale = exponent_scale(a.key_exponent[at_block]);
+              value_e = static_cast<float>(a.value_exponent[at_block]);
+            }
+          }
+        }
+        // groups of 16 keys: lane's group is in page (key0 + 16 · lane) / page
+        const int from = ((key0 + (lane & 7) * 16) / a.page - batch) & 31;
+        const float ks = __shfl_sync(0xffffffffu, key_scale, from);
+        const float ve = __shfl_sync(0xffffffffu, value_e, from);
+        const int group_id = __shfl_sync(0xffffffffu, id, from);
+        const unsigned gone = __ballot_sync(
+            0xffffffffu, lane < 8 && group_id < 0 && key0 + (lane & 7) * 16 < at.keys);
+        const int page_id = __shfl_sync(0xffffffffu, id, (first - batch + lane) & 31);
+        const bool load = lane < per_tile && page_id >= 0 && key0 + lane * box < at.keys;
+        const int bytes = __popc(__ballot_sync(0xffffffffu, load)) * box * HD;
+        const int ks_stage = block % L::kKStages, v_stage = block % L::kV8Stages;
+        if (block >= L::kKStages &&
+            !(ok = many_warp_wait(&k_empty[ks_stage], (block / L::kKStages - 1) & 1, abort, a.status)))
+          break;
+        float* scales = reinterpret_cast<float*>(smem + L::kScaleOffset +
+                                                 (block % L::kScaleRing) * L::kScaleBytes);
+        if (lane < 8) {
+          scales[lane] = ks;
+          scales[8 + lane] = ve;
+          scales[16 + lane] = exponent_scale(-static_cast<int>(ve));
+        }
+        if (lane == 0) reinterpret_cast<int*>(scales)[24] = static_cast<int>(gone);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&scale_full[block % L::kScaleRing]);
+          mbar_expect_tx(&k_full[ks_stage], bytes);
+        }
+        __syncwarp();
+        const int y = (page_id * a.heads_kv + at.h) * a.page + key0 % a.page;
+        if (load)
+          tma_load_2d(smem + L::kKOffset + ks_stage * L::kCodeTile + lane * box * HD, &tm_k,
+                      &k_full[ks_stage], 0, y);
+        if (block >= L::kV8Stages &&
+            !(ok = many_warp_wait(&v8_empty[v_stage], (block / L::kV8Stages - 1) & 1, abort, a.status))) {
+          // this tile's K was asked for without its V: counted below as K only
+          many_warp_wait(&k_full[ks_stage], (block / L::kKStages) & 1, abort, a.status);
+          break;
+        }
+        if (lane == 0) mbar_expect_tx(&v8_full[v_stage], bytes);
+        __syncwarp();
+        if (load)
+          tma_load_2d(smem + L::kV8Offset + v_stage * L::kCodeTile + lane * box * HD, &tm_v,
+                      &v8_full[v_stage], 0, y);
+      }
+      u += steps;
+      if (ok && u < u1) many_next(a, at);
+    }
+    // every copy lands before the CTA unwinds
+    volatile int never = 0;
+    for (int b = max(0, block - L::kKStages); b < block; ++b)
+      many_wait(&k_full[b % L::kKStages], (b / L::kKStages) & 1, &never, a.status);
+    for (int b = max(0, block - L::kV8Stages); b < block; ++b)
+      many_wait(&v8_full[b % L::kV8Stages], (b / L::kV8Stages) & 1, &never, a.status);
+    __syncwarp();
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------ matrix instructions
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyOtherRegs));
+    constexpr uint32_t kIdescQK = idesc_e4m3_f32(128, 128, false);
+    constexpr uint32_t kIdescPV = idesc_e4m3_f32(128, HD, true);  // f16 has the same code, 0
+    const uint64_t dq = code_desc<HD>(smem_u32(smem + L::kQOffset));
+    const uint64_t dk = code_desc<HD>(smem_u32(smem + L::kKOffset));
+    const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kV16Offset), 128 * 128, 1024);
+    constexpr uint64_t kTile = L::kCodeTile >> 4;
+    auto issue_qk = [&](int s, int stage) {
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const uint64_t q = dq + (2 * s + part) * kTile, k = dk + stage * kTile;
+#pragma unroll
+        for (int kk = 0; kk < HD / 32; ++kk)
+          mma_ss_f8(tmem + s * 128, q + kk * 2, k + kk * 2, kIdescQK, part + kk > 0 ? 1u : 0u);
+      }
+    };
+    auto issue_pv = [&](int s, int slot, uint32_t accumulate, int half) {
+      const uint64_t v = dv + slot * 2 * kTile;
+#pragma unroll
+      for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+        mma_ts(tmem + 256u + s * HD, tmem + s * 128 + kk * 8, v + ((kk * 16 * 128) >> 4), kIdescPV,
+               kk > 0 ? 1u : accumulate);
+    };
+    int block = 0, mine[2] = {0, 0}, segment[2] = {0, 0};
+    bool ok = true;
+    ManyAt at = many_at(a, u0);
+    for (long long u = u0; u < u1 && ok;) {
+      const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.tiles - at.j)));
+      const int tiles = many_rows(a, at) > 128 ? 2 : 1;
+      for (int s = 0; s < tiles && ok; ++s)
+        ok = many_warp_wait(&q_ready[s], segment[s]++ & 1, abort, a.status);
+      if (!ok || !(ok = many_warp_wait(&k_full[block % L::kKStages], (block / L::kKStages) & 1, abort, a.status)))
+        break;
+      tc_fence_after();
+      if (elect_one()) {
+        for (int s = 0; s < tiles; ++s) {
+          issue_qk(s, block % L::kKStages);
+          mma_commit(&s_full[s]);
+        }
+        mma_commit(&k_empty[block % L::kKStages]);
+      }
+      __syncwarp();
+      for (int step = 0; step < steps && ok; ++step, ++block) {
+        const bool more = step + 1 < steps;
+        const int slot = block % L::kV16Stages, next = (block + 1) % L::kKStages;
+        if (!(ok = many_warp_wait(&v16_full[slot], (block / L::kV16Stages) & 1, abort, a.status))) break;
+        if (more && !(ok = many_warp_wait(&k_full[next], ((block + 1) / L::kKStages) & 1, abort, a.status))) break;
+        for (int s = 0; s < tiles && ok; ++s) {
+          if (!(ok = many_warp_wait(&p_ready[2 * s], mine[s] & 1, abort, a.status))) break;
+          tc_fence_after();
+          if (elect_one()) issue_pv(s, slot, step > 0 ? 1u : 0u, 0);
+          __syncwarp();
+          if (!(ok = many_warp_wait(&p_ready[2 * s + 1], mine[s] & 1, abort, a.status))) break;
+          ++mine[s];
+          tc_fence_after();
+          if (elect_one()) {
+            issue_pv(s, slot, step > 0 ? 1u : 0u, 1);
+            if (more) {
+              issue_qk(s, next);
+              mma_commit(&s_full[s]);
+            } else {
+              mma_commit(&o_final[s]);
+            }
+            if (s + 1 == tiles) {
+              mma_commit(&v16_empty[slot]);
+              if (more) mma_commit(&k_empty[next]);
+            }
+          }
+          __syncwarp();
+        }
+      }
+      u += steps;
+      if (ok && u < u1) many_next(a, at);
+    }
+    // every product completes before tensor memory is given back
+    if (elect_one()) mma_commit(drain);
+    __syncwarp();
+    volatile int never = 0;
+    many_wait(drain, 0, &never, a.status);
+    __syncwarp();
+  } else {
+    // ----------------------------------------------------------------- V's codes to f16
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyOtherRegs));
+    constexpr int CH = HD / 16;  // 16-byte chunks of a row of codes
+    const int tid = threadIdx.x - 320;
+    int block = 0;
+    bool ok = true;
+    ManyAt at = many_at(a, u0);
+    for (long long u = u0; u < u1 && ok;) {
+      const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.tiles - at.j)));
+      const int first_seen = at.cached + at.item * (kRowsMany / a.group);
+      for (int step = 0; step < steps; ++step, ++block) {
+        const int in = block % L::kV8Stages, slot = block % L::kV16Stages;
+        if (!(ok = many_wait(&v8_full[in], (block / L::kV8Stages) & 1, abort, a.status))) break;
+        if (block >= L::kV16Stages &&
+            !(ok = many_wait(&v16_empty[slot], (block / L::kV16Stages - 1) & 1, abort, a.status)))
+          break;
+        const int key0 = (at.j + step) * kTileKeys;
+        // written before this tile's copies were asked for
+        const int gone = *reinterpret_cast<const volatile int*>(
+            smem + L::kScaleOffset + (block % L::kScaleRing) * L::kScaleBytes + 96);
+        const bool partial = key0 + kTileKeys > first_seen + 1 || gone != 0;
+        const uint32_t from = smem_u32(smem + L::kV8Offset + in * L::kCodeTile);
+        const uint32_t to = smem_u32(smem + L::kV16Offset + slot * 2 * L::kCodeTile);
+#pragma unroll 4
+        for (int i = 0; i < 128 * CH / 64; ++i) {
+          const int index = i * 64 + tid, row = index / CH, c = index % CH;
+          uint4 v = lds128(from + index * 16);
+          if (partial) {
+            if (key0 + row >= at.keys || (gone >> (row / 16) & 1)) v = make_uint4(0, 0, 0, 0);
+            const uint32_t n[4] = {nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w)};
+            uint32_t bits = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              bits |= ((n[k] & 1) | (n[k] >> 7 & 2) | (n[k] >> 14 & 4) | (n[k] >> 21 & 8)) << (4 * k);
+            *reinterpret_cast<uint16_t*>(smem + L::kNanOffset + (slot * 128 + row) * 16 + c * 2) =
+                static_cast<uint16_t>(bits);
+            if (bits) {
+              nan_tile[slot] = block + 1;
+              v.x &= ~n[0];
+              v.y &= ~n[1];
+              v.z &= ~n[2];
+              v.w &= ~n[3];
+            }
+          }
+          uint4 w0, w1;
+          widen4(v.x, w0.x, w0.y);
+          widen4(v.y, w0.z, w0.w);
+          widen4(v.z, w1.x, w1.y);
+          widen4(v.w, w1.z, w1.w);
+          // 64 channels (128 bytes) a box; the upper box's writers take their two chunks in
+          // the other order, so that 8 lanes never meet in a bank
+          const uint32_t box = to + (c >> 2) * (128 * 128) + row * 128;
+          const int j = 2 * (c & 3), turn = c >> 2;
+          sts128(box + (((j + turn) ^ (row & 7)) << 4), turn ? w1 : w0);
+          sts128(box + (((j + 1 - turn) ^ (row & 7)) << 4), turn ? w0 : w1);
+        }
+        fence_async_smem();
+        mbar_arrive(&v16_full[slot]);
+        mbar_arrive(&v8_empty[in]);
+      }
+      u += steps;
+      if (ok && u < u1) many_next(a, at);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of an item that a boundary between workers cuts (the first such boundary has
+// it): block (boundary, 32 rows), a lane a row, 8 warps over the channels.
+template <int HD>
+__global__ void __launch_bounds__(256) join_many(const CacheArgs a) {
+  constexpr int PER = HD / 32;  // float4 columns a warp
+  const long long total = a.units[a.requests] * a.heads_kv;
+  const long long workers = min(static_cast<long long>(a.workers), total);
+  const int w = blockIdx.x + 1;
+  bool split = w < workers;
+  ManyAt at;
+  int last = 0, rows = 0;
+  if (split) {
+    const long long u = w * total / workers;
+    at = many_at(a, u);
+    const long long u0 = u - at.j;
+    rows = many_rows(a, at);
+    split = at.j > 0 && (w - 1) * total / workers <= u0 && static_cast<int>(blockIdx.y) * 32 < rows;
+    last = static_cast<int>(((u0 + at.tiles) * workers - 1) / total);
+  }
+  if (split || (blockIdx.x == 0 && blockIdx.y == 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!split) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.y * 32 + lane;
+  if (row >= rows) return;
+  float top = -INFINITY;
+  for (int p = w - 1; p <= last; ++p)
+    top = fmaxf(top, __ldcg(&a.ws_ml[(2LL * p + (p == w - 1)) * kRowsMany + row]).x);
+  float sum = 0.f;
+  float4 o[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p = w - 1; p <= last; ++p) {
+    const long long part = 2LL * p + (p == w - 1);
+    const float2 ml = __ldcg(&a.ws_ml[part * kRowsMany + row]);
+    // a part without a key has zeros; one whose scores are NaN has a sum of NaN
+    const float f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - top);
+    sum += ml.y * f;
+    const float4* from = reinterpret_cast<const float4*>(a.ws_o) +
+                         (part * (HD / 4) + warp * PER) * kRowsMany + row;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float4 x = __ldcg(from + i * kRowsMany);
+      o[i].x = fmaf(x.x, f, o[i].x);
+      o[i].y = fmaf(x.y, f, o[i].y);
+      o[i].z = fmaf(x.z, f, o[i].z);
+      o[i].w = fmaf(x.w, f, o[i].w);
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int token = at.first_token + at.item * (kRowsMany / a.group) + row / a.group;
+  const int head = at.h * a.group + row % a.group;
+  uint2* to = reinterpret_cast<uint2*>(a.out + token * a.o_token + head * a.o_head) + warp * PER;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    to[i] = make_uint2(pack_bf16x2(o[i].x * inv, o[i].y * inv), pack_bf16x2(o[i].z * inv, o[i].w * inv));
+  if (a.lse != nullptr && warp == 0)
+    a.lse[static_cast<long long>(token) * a.heads_kv * a.group + head] =
+        sum == 0.f ? -INFINITY : 0.6931471805599453f * (top - kManyBias + __log2f(sum));
+}
+
+// ------------------------------------------------------------------------------- host side
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+  static EncodeTiled fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<EncodeTiled>(ptr);
+  }();
+  return fn;
+}
+
+// A pool's codes as rows of one head's channels; a box is `rows` rows, swizzled over a row's
+// width or not.
+static int code_map(CUtensorMap* map, const void* base, const CozyCacheStore& c, int rows,
+                    bool swizzled) {
+  EncodeTiled fn = encode_tiled();
+  if (fn == nullptr) return cudaErrorNotSupported;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(c.head_dim),
+                              static_cast<cuuint64_t>(c.pages) * c.heads_kv * c.page};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(c.head_dim)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(c.head_dim), static_cast<cuuint32_t>(rows)};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                        strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        !swizzled           ? CU_TENSOR_MAP_SWIZZLE_NONE
+                        : c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                            : CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+static int device_sms() {
+  static int counts[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 0;
+  if (counts[device] == 0)
+    cudaDeviceGetAttribute(&counts[device], cudaDevAttrMultiProcessorCount, device);
+  return counts[device];
+}
+
+static long long few_workers() { return static_cast<long long>(device_sms()) * 8; }
+
+// Rows of partial results a call may leave: two parts a worker.
+static long long part_rows(const CozyCachePlan& p) {
+  return few_rows(p.group, p.longest) ? few_workers() * 2 * kRowsFew
+                                      : static_cast<long long>(device_sms()) * 2 * kRowsMany;
+}
+
+long long cache_workspace(const CozyCachePlan& p, const CozyCacheStore& c) {
+  return part_rows(p) * (c.head_dim * sizeof(float) + sizeof(float2));
+}
+
+// A join starts while its attention runs and waits for that one's end on the device.
+static int join_launch(void (*kernel)(CacheArgs), dim3 grid, const CacheArgs& a, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <int HD>
+static int few_launch(const CozyCacheStore& c, CacheArgs& a, int longest, cudaStream_t stream) {
+  using L = Few<HD>;
+  static bool configured[64] = {};
+  int device = 0;
+  cudaGetDevice(&device);
+  if (device < 64 && !configured[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        attend_few<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
+    if (e != cudaSuccess) return e;
+    configured[device] = true;
+  }
+  CUtensorMap mk, mv;
+  const int box = c.page < kChunkKeys ? c.page : kChunkKeys;
+  int e = code_map(&mk, c.key, c, box, true);
+  if (e || (e = code_map(&mv, c.value, c, box, true))) return e;
+  attend_few<HD><<<device_sms(), 256, L::kAlloc, stream>>>(mk, mv, a);
+  if ((e = cudaGetLastError())) return e;
+  return join_launch(join_few<HD>, dim3(a.requests * a.heads_kv, a.group * longest), a, stream);
+}
+
+template <int HD>
+static int many_launch(const CozyCacheStore& c, CacheArgs& a, cudaStream_t stream) {
+  using L = Many<HD>;
+  static bool configured[64] = {};
+  int device = 0;
+  cudaGetDevice(&device);
+  if (device < 64 && !configured[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        attend_many<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
+    if (e != cudaSuccess) return e;
+    configured[device] = true;
+  }
+  CUtensorMap mk, mv;
+  const int box = c.page < kTileKeys ? c.page : kTileKeys;
+  int e = code_map(&mk, c.key, c, box, true);
+  if (e || (e = code_map(&mv, c.value, c, box, false))) return e;
+  attend_many<HD><<<a.workers, L::kThreads, L::kAlloc, stream>>>(mk, mv, a);
+  if ((e = cudaGetLastError())) return e;
+  if (a.workers < 2) return cudaSuccess;
+  return join_launch(join_many<HD>, dim3(a.workers - 1, kRowsMany / 32), a, stream);
+}
+
+int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyCacheAttend& x,
                     cudaStream_t stream) {
   const int e = cache_store_check(c, p);
   if (e) return e;
   if (p.tokens == 0) return cudaSuccess;
-  if (!(a.scale > 0.f) || a.scale > 3.0e38f) return cudaErrorInvalidValue;
-  const void* ptrs[] = {a.query, a.out};
+  if (!(x.scale > 0.f) || x.scale > 3.0e38f) return cudaErrorInvalidValue;
+  const void* ptrs[] = {x.query, x.out};
   for (const void* ptr : ptrs)
     if (ptr == nullptr || reinterpret_cast<uintptr_t>(ptr) % 16) return cudaErrorInvalidValue;
   for (int i = 0; i < 2; ++i)
-    if (a.query_strides[i] < 0 || a.query_strides[i] % 8 || a.out_strides[i] < 0 ||
-        a.out_strides[i] % 8)
+    if (x.query_strides[i] < 0 || x.query_strides[i] % 8 || x.out_strides[i] < 0 ||
+        x.out_strides[i] % 8)
       return cudaErrorInvalidValue;
-  const long long rows = static_cast<long long>(p.tokens) * c.heads_kv * p.group;
-  const long long ctas = (rows + 3) / 4;
-  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (c.head_dim == 64) cache_attend_plain<64><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(p, c, a);
-  else cache_attend_plain<128><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(p, c, a);
-  return cudaGetLastError();
+  if (x.workspace == nullptr || reinterpret_cast<uintptr_t>(x.workspace) % 256 ||
+      x.workspace_bytes < cache_workspace(p, c))
+    return cudaErrorInvalidValue;
+  CacheArgs a = {};
+  a.table = p.table;
+  a.table_stride = p.table_stride;
+  a.starts = p.starts;
+  a.lengths = p.lengths_after;
+  a.units = p.units;
+  a.status = p.status;
+  a.requests = p.requests;
+  a.pages = p.pages;
+  a.page = p.page;
+  a.group = p.group;
+  a.heads_kv = c.heads_kv;
+  a.key_exponent = static_cast<const int8_t*>(c.key_exponent);
+  a.value_exponent = static_cast<const int8_t*>(c.value_exponent);
+  a.query = static_cast<const __nv_bfloat16*>(x.query);
+  a.q_token = x.query_strides[0];
+  a.q_head = x.query_strides[1];
+  a.out = static_cast<__nv_bfloat16*>(x.out);
+  a.o_token = x.out_strides[0];
+  a.o_head = x.out_strides[1];
+  a.lse = x.lse;
+  a.scale_log2 = x.scale * 1.4426950408889634f;
+  a.ws_o = static_cast<float*>(x.workspace);
+  a.ws_ml = reinterpret_cast<float2*>(a.ws_o + part_rows(p) * c.head_dim);
+  if (few_rows(p.group, p.longest)) {
+    if (static_cast<long long>(p.requests) * c.heads_kv > 0x7fffffffLL) return cudaErrorInvalidValue;
+    a.workers = static_cast<int>(few_workers());
+    return c.head_dim == 64 ? few_launch<64>(c, a, p.longest, stream)
+                            : few_launch<128>(c, a, p.longest, stream);
+  }
+  a.workers = device_sms();
+  return c.head_dim == 64 ? many_launch<64>(c, a, stream) : many_launch<128>(c, a, stream);
 }
 
 }  // namespace cozy

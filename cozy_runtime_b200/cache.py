@@ -20,7 +20,9 @@ a plan or a cache used on another stream than the one that wrote it is ordered b
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 
@@ -75,16 +77,31 @@ class Layout:
 def _need(t: Tensor, name: str, dtype: torch.dtype, shape: tuple[int | None, ...]) -> None:
     if t.dtype != dtype:
         raise ValueError(f"{name} is {t.dtype}, not {dtype}")
-    if t.dim() != len(shape) or any(w is not None and g != w for g, w in zip(t.shape, shape)):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
+    got = t.shape
+    if got != shape and (
+        len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape))
+    ):
+        raise ValueError(f"{name} has shape {tuple(got)}, not {shape}")
 
 
-def _same_device(device: torch.device, **tensors: Tensor | None) -> None:
-    for name, t in tensors.items():
+def _one_device(device: torch.device, *tensors: Tensor | None) -> None:
+    for t in tensors:
         if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not {device}")
+            raise ValueError(f"operands are on {t.device} and on {device}")
     if device.type != "cuda":
         raise ValueError("operands are not on a CUDA device")
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device's context, entered only where another one is current."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device.index).cuda_stream
 
 
 class Cache:
@@ -102,8 +119,7 @@ class Cache:
                         ("value_exponent", value_exponent)):
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
-        _same_device(key.device, key=key, value=value, key_exponent=key_exponent,
-                     value_exponent=value_exponent)
+        _one_device(key.device, value, key_exponent, value_exponent)
         for name, t in (("key", key), ("value", value)):
             if t.data_ptr() % 128:
                 raise ValueError(f"{name} must start on a 128-byte boundary")
@@ -135,65 +151,64 @@ class Cache:
 
 
 class Plan:
-    """A step's plan on the GPU. Tensors: `lengths` [requests] int32 after the step, `cursor` [2]
-    int64 after it, `starts` [requests + 1] int32, `positions` [tokens] int32 and `slots` [tokens]
-    int64 (page number · page + row; both -1 in rows of nobody), `status` [1] int32."""
+    """A step's plan on the GPU. `lengths` [requests] int32 after the step, `cursor` [2] int64
+    after it, `starts` [requests + 1] int32, `positions` [tokens] int32 and `slots` [tokens] int64
+    (page number · page + row; both -1 in rows of nobody), `status` [1] int32."""
 
     def __init__(self, layout: Layout, table: Tensor, lengths: Tensor, new: Tensor, free: Tensor,
                  cursor: Tensor, tokens: int, longest: int):
-        n, page = lengths.shape[0], layout.page
+        n, page, device = lengths.shape[0], layout.page, table.device
         blocks = min(tokens, tokens // page + 2 * n)
-        # one buffer, in 8-byte words: status, blocks (16-byte entries), cursor, units, slots, ...
-        sizes = (2, 2 * blocks, 2, n + 1, tokens, n // 2 + 1, (n + 1) // 2, (tokens + 1) // 2)
-        self._at = [0]
-        for size in sizes:
-            self._at.append(self._at[-1] + size)
-        self._buffer = torch.empty(self._at[-1], dtype=torch.int64, device=table.device)
+        # `blocks` entries are 16 bytes and stand first, in front of the status word
+        self._cuts = (4 * blocks, 1, n, n + 1, tokens), (2, n + 1, tokens)
+        whole = torch.empty(4 * blocks + 2 * n + 2 + tokens, dtype=torch.int32, device=device)
+        wide = torch.empty(n + 3 + tokens, dtype=torch.int64, device=device)
+        self._buffers = whole, wide
         self.layout, self.table, self.tokens, self.longest = layout, table, tokens, longest
+        self.requests, self.pages = n, free.shape[0]
         # what the calls of this step read must outlive them
         self._inputs = (lengths, new, free, cursor)
-        base = self._buffer.data_ptr()
-        at = [base + 8 * word for word in self._at]
+        at, at8 = whole.data_ptr(), wide.data_ptr()
+        status = at + 16 * blocks
         self._c = _lib.CachePlan(
-            lengths.data_ptr(), new.data_ptr(), table.data_ptr(), table.stride(0),
-            free.data_ptr(), cursor.data_ptr(), n, table.shape[1], free.shape[0], page, tokens,
-            longest, layout.group, blocks, at[6], at[5], at[2], at[7], at[4], at[1], at[3], at[0],
+            lengths.data_ptr(), new.data_ptr(), table.data_ptr(),
+            max(table.stride(0), table.shape[1]), free.data_ptr(), cursor.data_ptr(), n,
+            table.shape[1], free.shape[0], page, tokens, longest, layout.group, blocks,
+            status + 4, status + 4 + 4 * n, at8, status + 8 + 8 * n, at8 + 8 * (n + 3), at,
+            at8 + 16, status,
         )
 
-    def _words(self, part: int) -> Tensor:
-        return self._buffer[self._at[part]:self._at[part + 1]]
+    @functools.cached_property
+    def _whole(self) -> tuple[Tensor, ...]:
+        return self._buffers[0].split_with_sizes(self._cuts[0])
 
-    @property
-    def requests(self) -> int:
-        return self._c.requests
-
-    @property
-    def pages(self) -> int:
-        return self._c.pages
+    @functools.cached_property
+    def _wide(self) -> tuple[Tensor, ...]:
+        return self._buffers[1].split_with_sizes(self._cuts[1])
 
     @property
     def status(self) -> Tensor:
-        return self._words(0).view(torch.int32)[:1]
-
-    @property
-    def cursor(self) -> Tensor:
-        return self._words(2)
-
-    @property
-    def slots(self) -> Tensor:
-        return self._words(4)
-
-    @property
-    def starts(self) -> Tensor:
-        return self._words(5).view(torch.int32)[:self.requests + 1]
+        return self._whole[1]
 
     @property
     def lengths(self) -> Tensor:
-        return self._words(6).view(torch.int32)[:self.requests]
+        return self._whole[2]
+
+    @property
+    def starts(self) -> Tensor:
+        return self._whole[3]
 
     @property
     def positions(self) -> Tensor:
-        return self._words(7).view(torch.int32)[:self.tokens]
+        return self._whole[4]
+
+    @property
+    def cursor(self) -> Tensor:
+        return self._wide[0]
+
+    @property
+    def slots(self) -> Tensor:
+        return self._wide[2]
 
     def check(self) -> None:
         """Raise if the plan was refused, or if its calls so far met a page number outside the pool
@@ -202,6 +217,28 @@ class Plan:
         if word:
             raise RuntimeError("cache plan: " + "; ".join(
                 text for bit, text in STATUS_NAMES.items() if word & bit))
+
+
+def _check_plan(table, lengths, new, free, cursor) -> tuple[int, int]:
+    """(requests, width) of a plan's tensors, whose types and shapes fit each other."""
+    if table.dim() != 2:
+        raise ValueError(f"table has shape {tuple(table.shape)}, not [requests, width]")
+    requests, width = table.shape
+    for name, t, shape in (("table", table, None), ("lengths", lengths, (requests,)),
+                           ("new", new, (requests,)), ("free", free, None)):
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} is {t.dtype}, not torch.int32")
+        if shape is not None and t.shape != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
+    if cursor.dtype != torch.int64 or cursor.shape != (2,) or free.dim() != 1:
+        raise ValueError("cursor is two int64 counts, free a ring of page numbers")
+    stride = table.stride()
+    if stride[1] != 1 or (requests > 1 and stride[0] < width):
+        raise ValueError("rows of the table must be contiguous and apart")
+    if not (lengths.is_contiguous() and new.is_contiguous() and free.is_contiguous()
+            and cursor.is_contiguous()):
+        raise ValueError("lengths, new, free and cursor must be contiguous")
+    return requests, width
 
 
 def plan(
@@ -228,48 +265,42 @@ def plan(
     `table` and `free` are written in place, only where they held nothing; the new lengths and
     cursor are the plan's, so planning the same tensors again gives the same plan. A step that
     cannot be served (see `STATUS_NAMES`) changes nothing: its plan has no rows."""
-    _need(lengths, "lengths", torch.int32, (None,))
-    requests = lengths.shape[0]
-    _need(table, "table", torch.int32, (requests, None))
-    _need(new, "new", torch.int32, (requests,))
-    _need(free, "free", torch.int32, (None,))
-    _need(cursor, "cursor", torch.int64, (2,))
+    requests, width = _check_plan(table, lengths, new, free, cursor)
     if not 1 <= requests <= MAX_REQUESTS:
         raise ValueError(f"{requests} requests are not served (1 to {MAX_REQUESTS})")
-    if table.shape[1] < 1 or free.shape[0] < 1:
+    if width < 1 or free.shape[0] < 1:
         raise ValueError("an empty table or pool")
-    if table.shape[1] * layout.page > 2**31 - 1:
+    if width * layout.page > 2**31 - 1:
         raise ValueError("a request holds at most 2^31 - 1 tokens")
-    if table.stride(1) != 1 or (requests > 1 and table.stride(0) < table.shape[1]):
-        raise ValueError("rows of the table must be contiguous and apart")
-    if not (lengths.is_contiguous() and new.is_contiguous() and free.is_contiguous()
-            and cursor.is_contiguous()):
-        raise ValueError("lengths, new, free and cursor must be contiguous")
     if not 0 <= tokens < 2**31 or not 0 <= longest < 2**31:
         raise ValueError("tokens and longest must be counts below 2^31")
-    _same_device(table.device, table=table, lengths=lengths, new=new, free=free, cursor=cursor)
-    with torch.cuda.device(table.device):
-        made = Plan(layout, table, lengths, new, free, cursor, tokens, longest)
-        made._c.table_stride = max(table.stride(0), table.shape[1])
-        code = _lib.load().cozy_cache_plan(
-            ctypes.byref(made._c), torch.cuda.current_stream(table.device).cuda_stream
-        )
+    device = table.device
+    _one_device(device, lengths, new, free, cursor)
+    made = Plan(layout, table, lengths, new, free, cursor, tokens, longest)
+    with _on(device):
+        code = _lib.load().cozy_cache_plan(ctypes.byref(made._c), _stream(device))
     _lib.check("cozy_cache_plan", code)
     return made
 
 
 def _rows(t: Tensor, name: str, step: Plan, heads: int) -> tuple[int, int]:
     """Element strides {token, head} of a step's [tokens, heads, head_dim] rows."""
-    _need(t, name, torch.bfloat16, (step.tokens, heads, step.layout.head_dim))
-    strides = [t.stride(i) if t.shape[i] > 1 else t.shape[2] for i in (0, 1)]
-    if (t.stride(2) != 1 and t.numel() > 0) or any(s % 8 for s in strides) or t.data_ptr() % 16:
+    dim = step.layout.head_dim
+    _need(t, name, torch.bfloat16, (step.tokens, heads, dim))
+    token, head, last = t.stride()
+    if step.tokens <= 1:
+        token = dim
+    if heads == 1:
+        head = dim
+    if (last != 1 and step.tokens > 0) or token % 8 or head % 8 or t.data_ptr() % 16:
         raise ValueError(f"{name}: the head dimension must be contiguous and rows 16-byte aligned")
-    return strides[0], strides[1]
+    return token, head
 
 
 def _out(given: Tensor | None, like: Tensor, step: Plan) -> tuple[Tensor, tuple[int, int]]:
     if given is None:
         given = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return given, (like.shape[1] * like.shape[2], like.shape[2])
     token, head = _rows(given, "out", step, like.shape[1])
     rows, heads, dim = given.shape
     apart = head >= dim and token >= (heads - 1) * head + dim
@@ -319,7 +350,8 @@ def append(
     A page that requests share must be full: two writers of one block are not ordered."""
     _fits(store, step)
     layout = step.layout
-    _same_device(store.key.device, plan=step.table, key=key, value=value, query=query, out=out)
+    device = store.key.device
+    _one_device(device, step.table, key, value, query, out)
     a = _lib.CacheAppend()
     a.key, a.value = key.data_ptr(), value.data_ptr()
     a.key_strides[:] = _rows(key, "key", step, layout.heads_kv)
@@ -330,7 +362,7 @@ def append(
         raise ValueError("norm_q and out are the query's")
     tables = None
     if rope is not None:
-        _same_device(store.key.device, cos=rope.cos, sin=rope.sin)
+        _one_device(device, rope.cos, rope.sin)
         last = step._c.width * layout.page - 1
         columns = rope.rotary // 2 if rope.interleaved else rope.rotary
         if rope.rotary < 0 or rope.rotary > layout.head_dim or rope.rotary % 2:
@@ -354,17 +386,16 @@ def append(
         if norm.weight is not None:
             if norm.weight.shape != (layout.head_dim,):
                 raise ValueError("a norm's weight has one value for each channel of a head")
-            w = norm.weight.to(device=store.key.device, dtype=torch.float32).contiguous()
+            w = norm.weight.to(device=device, dtype=torch.float32).contiguous()
             weights.append(w)
             a.norm_weight[i] = w.data_ptr()
-    with torch.cuda.device(store.key.device):
-        if query is not None:
-            out, strides = _out(out, query, step)
-            a.query, a.out = query.data_ptr(), out.data_ptr()
-            a.out_strides[:] = strides
+    if query is not None:
+        out, strides = _out(out, query, step)
+        a.query, a.out = query.data_ptr(), out.data_ptr()
+        a.out_strides[:] = strides
+    with _on(device):
         code = _lib.load().cozy_cache_append(
-            ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a),
-            torch.cuda.current_stream(store.key.device).cuda_stream,
+            ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a), _stream(device)
         )
     _lib.check("cozy_cache_append", code)
     return out
@@ -389,32 +420,31 @@ def attention(
     page whose number is outside the pool are left out, and the plan's status says so."""
     _fits(store, step)
     device = store.key.device
-    _same_device(device, plan=step.table, query=query, out=out)
+    _one_device(device, step.table, query, out)
     scale = 1.0 / math.sqrt(step.layout.head_dim) if scale is None else float(scale)
     if not (0.0 < scale < 3e38):
         raise ValueError("attention scale must be positive and finite")
     a = _lib.CacheAttend()
     a.query, a.scale = query.data_ptr(), scale
     a.query_strides[:] = _rows(query, "query", step, step.layout.heads_q)
-    with torch.cuda.device(device):
-        given, (out, strides) = out, _out(out, query, step)
-        if given is not None and query.numel() > 0:
-            (q0, q1), (o0, o1) = _range(query), _range(out)
-            if q0 < o1 and o0 < q1:
-                raise ValueError("out overlaps the query")
-        a.out = out.data_ptr()
-        a.out_strides[:] = strides
-        lse = None
-        if return_lse:
-            lse = torch.empty(query.shape[:2], dtype=torch.float32, device=device)
-            a.lse = lse.data_ptr()
-        lib = _lib.load()
+    given, (out, strides) = out, _out(out, query, step)
+    if given is not None and query.numel() > 0:
+        (q0, q1), (o0, o1) = _range(query), _range(out)
+        if q0 < o1 and o0 < q1:
+            raise ValueError("out overlaps the query")
+    a.out = out.data_ptr()
+    a.out_strides[:] = strides
+    lse = None
+    if return_lse:
+        lse = torch.empty(query.shape[:2], dtype=torch.float32, device=device)
+        a.lse = lse.data_ptr()
+    lib = _lib.load()
+    with _on(device):
         size = lib.cozy_cache_workspace(ctypes.byref(step._c), ctypes.byref(store._c))
         space = torch.empty(size, dtype=torch.uint8, device=device)
         a.workspace, a.workspace_bytes = space.data_ptr(), size
         code = lib.cozy_cache_attention(
-            ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a),
-            torch.cuda.current_stream(device).cuda_stream,
+            ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a), _stream(device)
         )
     _lib.check("cozy_cache_attention", code)
     return out if lse is None else (out, lse)

@@ -619,8 +619,9 @@ __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
 //
 //   warps 0-3, 4-7  softmax of query tile 0, 1 (a thread a row, a TMEM lane)
 //   warp  8         page numbers, scales, and TMA of K and V codes into their rings
-//   warp  9         the matrix instructions
-//   warps 10, 11    V's codes widened to f16 (exact)
+//   warps 9, 10     the matrix instructions of query tile 0, 1
+//   warps 12-15     V's codes widened to f16 (exact); they also see K's next tile in, so that
+//                   the issuer waits once for both
 //
 // S = Q·Kᵀ runs in 8 bits on K's codes as they are stored, with Q split into two e4m3 parts
 // under one power of two a row: q = hi + lo holds all 8 bits of a bf16 that is not below 2^-11 of
@@ -629,10 +630,13 @@ __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
 // memory. P stays in f16 (11 bits; two 8-bit parts would lose the weights under 2^-17 of a row's
 // largest, which a long context has many of), so V is widened.
 //
-// Tensor memory: S/P of the two tiles at columns 0 and 128, O at 256 and 256 + HD.
+// A tile of keys is taken in two halves of 64 with a buffer of S each, so that the next half's
+// Q·Kᵀ is done when a half's softmax ends: neither the tensor cores nor the softmax wait for the
+// other's round trip. (With one buffer of 128 a unit took 3823 clocks, 2129 of them on the tensor
+// cores.) Tensor memory: S/P of tile s, half b at column 128 s + 64 b, O at 256 + HD s.
 template <int HD>
 struct Many {
-  static constexpr int kThreads = 384;
+  static constexpr int kThreads = 512;
   static constexpr int kKStages = 3, kV8Stages = 2, kV16Stages = 2;
   static constexpr int kScaleRing = 8;
   static constexpr int kCodeTile = 128 * HD;      // 128 rows of codes
@@ -646,14 +650,16 @@ struct Many {
   // [ring]{2^key exponent [8], value exponent [8], 2^-value exponent [8], gone groups, pad}
   static constexpr int kScaleBytes = 112;
   static constexpr int kBarOffset = kScaleOffset + kScaleRing * kScaleBytes;
-  static constexpr int kBars = 2 + 2 * kKStages + 2 * kV8Stages + 2 * kV16Stages + 2 + 4 + 2 +
+  static constexpr int kBars = 2 + 2 * kKStages + 2 * kV8Stages + 2 * kV16Stages + 4 + 4 + 4 +
                                kScaleRing + 1;
   static constexpr int kMiscOffset = kBarOffset + kBars * 8;
-  static constexpr int kAlloc = kMiscOffset + 32 + 1024;
+  static constexpr int kAtOffset = kMiscOffset + 32;  // each softmax warp's place in its run
+  static constexpr int kAlloc = kAtOffset + 8 * 64 + 1024;
 };
-// Registers: 384 threads start with 168 each; 256 · 208 + 128 · 80 = 63488 ≤ 64512.
-constexpr int kManySoftmaxRegs = 208;
-constexpr int kManyOtherRegs = 80;
+// Registers: 512 threads start with 128 each; 256 · 168 + 256 · 88 = 65536, what they started with.
+constexpr int kManySoftmaxRegs = 168;
+constexpr int kManyOtherRegs = 88;
+constexpr int kWideners = 128;  // threads that widen V: a warp on each sub-partition
 
 // P = 2^(s - m + 7) against a reference that may lie 2^8 below the row's largest (O is rescaled
 // only when the maximum grew by more): at most 2^15 in f16, normal down to 2^-21 of the reference.
@@ -718,6 +724,34 @@ __device__ __forceinline__ void many_next(const CacheArgs& a, ManyAt& at) {
     }
   }
   many_item(a, at);
+}
+
+// A warp's place in shared memory: what the loop over tiles does not need stands there, not in
+// registers (128 scores and 16 weights a thread leave few).
+__device__ __forceinline__ void many_put(volatile int* to, const ManyAt& at, int left) {
+  __syncwarp();
+  to[0] = at.n;
+  to[1] = at.h;
+  to[2] = at.item;
+  to[3] = at.j;
+  to[4] = at.items;
+  to[5] = at.tiles;
+  to[6] = at.keys;
+  to[7] = at.cached;
+  to[8] = at.added;
+  to[9] = at.first_token;
+  to[10] = left;
+  __syncwarp();
+}
+
+__device__ __forceinline__ ManyAt many_get(const volatile int* from) {
+  return {from[0], from[1], from[2], from[3], from[4], from[5], from[6], from[7], from[8], from[9]};
+}
+
+// Halves of tiles in `steps` tiles from the place on: the last tile of an item may need only one.
+__device__ __forceinline__ int many_halves(const CacheArgs& a, const ManyAt& at, int steps) {
+  const int keys = at.cached + min((at.item + 1) * (kRowsMany / a.group), at.added);
+  return min(2 * steps, (keys - at.j * kTileKeys + 63) / 64);
 }
 
 __device__ __forceinline__ int many_rows(const CacheArgs& a, const ManyAt& at) {
@@ -786,7 +820,7 @@ __device__ __forceinline__ uint64_t code_desc(uint32_t at) {
   return d;
 }
 
-// Sixteen scores (a group under one scale) to weights 2^(s · mul + add) in f16 pairs.
+// Sixteen scores (under one scale) to weights 2^(s · mul + add) in f16 pairs, summed into acc.
 __device__ __forceinline__ void weigh16(const uint32_t* r, float mul, float add, float2& acc,
                                         uint32_t* pk) {
   const float2 m2 = make_float2(mul, mul), a2 = make_float2(add, add);
@@ -800,13 +834,19 @@ __device__ __forceinline__ void weigh16(const uint32_t* r, float mul, float add,
   }
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 __device__ __forceinline__ float max16(const uint32_t* r) {
   float a = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
   float b = fmaxf(__uint_as_float(r[2]), __uint_as_float(r[3]));
 #pragma unroll
   for (int i = 4; i < 16; i += 4) {
-    a = fmaxf(a, fmaxf(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
-    b = fmaxf(b, fmaxf(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])));
+    a = max3(a, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+    b = max3(b, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
   }
   return fmaxf(a, b);
 }
@@ -819,8 +859,9 @@ __device__ __forceinline__ void hide32(uint32_t (&r)[32], int limit, int gone) {
     if (i > limit || (gone >> (i / 16) & 1)) r[i] = 0xff800000u;
 }
 
-template <int HD>
-__global__ void __launch_bounds__(384, 1)
+// GROUPS: scales that 64 keys can have (64 / page, at least 1).
+template <int HD, int GROUPS>
+__global__ void __launch_bounds__(512, 1)
     attend_many(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                 const CacheArgs a) {
   using L = Many<HD>;
@@ -836,9 +877,9 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t* v16_full = v8_empty + L::kV8Stages;
   uint64_t* v16_empty = v16_full + L::kV16Stages;
   uint64_t* s_full = v16_empty + L::kV16Stages;
-  uint64_t* p_ready = s_full + 2;  // [tile][half]
-  uint64_t* o_final = p_ready + 4;
-  uint64_t* scale_full = o_final + 2;
+  uint64_t* p_ready = s_full + 4;
+  uint64_t* pv_done = p_ready + 4;  // these three [tile][half]
+  uint64_t* scale_full = pv_done + 4;
   uint64_t* drain = scale_full + L::kScaleRing;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOffset);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 4);
@@ -854,26 +895,28 @@ __global__ void __launch_bounds__(384, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_ready[i], 128);
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[2 * i], 1);
+      mbar_init(&s_full[2 * i + 1], 1);
       mbar_init(&p_ready[2 * i], 128);
       mbar_init(&p_ready[2 * i + 1], 128);
-      mbar_init(&o_final[i], 1);
+      mbar_init(&pv_done[2 * i], 1);
+      mbar_init(&pv_done[2 * i + 1], 1);
     }
     for (int i = 0; i < L::kKStages; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], 2);
     }
     for (int i = 0; i < L::kV8Stages; ++i) {
       mbar_init(&v8_full[i], 1);
-      mbar_init(&v8_empty[i], 64);
+      mbar_init(&v8_empty[i], kWideners);
     }
     for (int i = 0; i < L::kV16Stages; ++i) {
-      mbar_init(&v16_full[i], 64);
-      mbar_init(&v16_empty[i], 1);
+      mbar_init(&v16_full[i], kWideners);
+      mbar_init(&v16_empty[i], 2);
       nan_tile[i] = 0;
     }
     for (int i = 0; i < L::kScaleRing; ++i) mbar_init(&scale_full[i], 1);
-    mbar_init(drain, 1);
+    mbar_init(drain, 2);
     *abort = 0;
     fence_barrier_init();
   }
@@ -894,27 +937,35 @@ __global__ void __launch_bounds__(384, 1)
     const uint32_t tS = tmem + lane_bits + static_cast<uint32_t>(s * 128);
     const uint32_t tO = tmem + lane_bits + 256u + static_cast<uint32_t>(s * HD);
     uint4* poison = reinterpret_cast<uint4*>(smem + L::kPoisonOffset) + threadIdx.x;
-    int block = 0, mine = 0, segment = 0;  // tiles of keys seen; by this query tile; items of it
+    int block = 0;       // tiles of keys seen
+    uint32_t phase = 0;  // bit b: parity of half b's next scores (its last product has the other)
     bool ok = true;
-    ManyAt at = many_at(a, u0);
-    for (long long u = u0; u < u1;) {
-      const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.tiles - at.j)));
-      const int rows = many_rows(a, at);
-      if (s * 128 < rows) {
+    volatile int* place = reinterpret_cast<volatile int*>(smem + L::kAtOffset) + warp * 16;
+    many_put(place, many_at(a, u0), static_cast<int>(u1 - u0));
+    while (ok) {
+      int steps, halves, last, first_seen, key0;
+      bool here;
+      float mul = 0.f;
+      {
+        const ManyAt at = many_get(place);
+        steps = min(static_cast<int>(place[10]), at.tiles - at.j);
+        halves = many_halves(a, at, steps);
+        key0 = at.j * kTileKeys;
+        const int rows = many_rows(a, at);
+        here = s * 128 < rows;
         const int per = kRowsMany / a.group;
-        const int row = s * 128 + row128;
-        const int token = at.item * per + min(row, rows - 1) / a.group;  // of the request
-        const int last = at.cached + token;                              // the last key it sees
-        float mul;
-        {  // ---- this row of Q as two e4m3 parts
+        const int row = min(s * 128 + row128, rows - 1);
+        const int token = at.item * per + row / a.group;  // of the request
+        last = at.cached + token;                         // the last key it sees
+        first_seen = at.cached + at.item * per;           // the item's first token's last key
+        if (here) {  // ---- this row of Q as two e4m3 parts (rows behind the last repeat it)
           const __nv_bfloat16* from = a.query + (at.first_token + token) * a.q_token +
-                                      (at.h * a.group + min(row, rows - 1) % a.group) * a.q_head;
-          uint4 x[HD / 8];
+                                      (at.h * a.group + row % a.group) * a.q_head;
           float amax = 0.f;
 #pragma unroll
           for (int c = 0; c < HD / 8; ++c) {
-            x[c] = row < rows ? *reinterpret_cast<const uint4*>(from + c * 8) : make_uint4(0, 0, 0, 0);
-            const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(from + c * 8));
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               amax = fmaxf(amax, fabsf(__uint_as_float(w[e] << 16)));
@@ -927,12 +978,14 @@ __global__ void __launch_bounds__(384, 1)
           mul = a.scale_log2 * exponent_scale(e);
           const uint32_t hi_at = smem_u32(smem + L::kQOffset + s * 2 * L::kCodeTile);
           const uint32_t lo_at = hi_at + L::kCodeTile;
-#pragma unroll
-          for (int c = 0; c < HD / 16; ++c) {
+#pragma unroll 2
+          for (int c = 0; c < HD / 16; ++c) {  // read again (from L1) rather than held
             uint32_t hi[4], lo[4];
+            const uint4 x[2] = {__ldg(reinterpret_cast<const uint4*>(from + c * 16)),
+                                __ldg(reinterpret_cast<const uint4*>(from + c * 16 + 8))};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint4 v = x[2 * c + (k >> 1)];
+              const uint4 v = x[k >> 1];
               const uint32_t w[2] = {(k & 1) ? v.z : v.x, (k & 1) ? v.w : v.y};
               uint32_t parts[2][2];
 #pragma unroll
@@ -962,37 +1015,63 @@ __global__ void __launch_bounds__(384, 1)
           fence_async_smem();
           mbar_arrive(&q_ready[s]);
         }
+      }
+      if (here) {
         float m = -INFINITY, l = 0.f;
-        const int first_seen = at.cached + at.item * per;  // the item's first token's last key
-        for (int step = 0; step < steps; ++step, ++block, ++mine) {
-          const float* scales = reinterpret_cast<const float*>(
-              smem + L::kScaleOffset + (block % L::kScaleRing) * L::kScaleBytes);
-          if (!many_wait(&s_full[s], mine & 1, abort, a.status) ||
-              !many_wait(&scale_full[block % L::kScaleRing], (block / L::kScaleRing) & 1, abort, a.status)) {
+        for (int h = 0; h < halves; ++h) {
+          const int b = h & 1, tile = block + (h >> 1), slot = tile % L::kScaleRing;
+          const int tile_key0 = key0 + (h >> 1) * kTileKeys, half_key0 = tile_key0 + b * 64;
+          // the scales are there long before the scores
+          const float* scales =
+              reinterpret_cast<const float*>(smem + L::kScaleOffset + slot * L::kScaleBytes) + b * 4;
+          if (b == 0 && !many_wait(&scale_full[slot], (tile / L::kScaleRing) & 1, abort, a.status)) {
             ok = false;
             break;
           }
+          float mul_of[GROUPS], add_of[GROUPS];
+#pragma unroll
+          for (int c = 0; c < GROUPS; ++c) {
+            mul_of[c] = group_mul(mul, scales[c * (4 / GROUPS)]);
+            add_of[c] = scales[8 + c * (4 / GROUPS)];
+          }
+          const int gone = reinterpret_cast<const int*>(scales)[24 - b * 4];
+          if (!many_wait(&s_full[2 * s + b], phase >> b & 1, abort, a.status)) {
+            ok = false;
+            break;
+          }
+          phase ^= 1u << b;
           tc_fence_after();
-          uint32_t r[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, r[c]);
+          uint32_t r[2][32];
+          tmem_ld32(tS + b * 64, r[0]);
+          tmem_ld32(tS + b * 64 + 32, r[1]);
           tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tie(r[c]);
-          const int key0 = (at.j + step) * kTileKeys;
-          const int gone = reinterpret_cast<const int*>(scales)[24];
-          const bool partial = key0 + kTileKeys > first_seen + 1 || gone != 0;
+          tie(r[0]);
+          tie(r[1]);
+          // some row of the item does not see the whole tile
+          const bool partial = tile_key0 + kTileKeys > first_seen + 1 || gone != 0;
           if (partial) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) hide32(r[c], last - key0 - c * 32, gone >> (2 * c));
+            hide32(r[0], last - half_key0, gone >> (4 * b));
+            hide32(r[1], last - half_key0 - 32, gone >> (4 * b + 2));
           }
           float top = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            top = fmaxf(top, fmaf(max16(&r[c >> 1][(c & 1) * 16]), group_mul(mul, scales[c]), scales[8 + c]));
+          for (int c = 0; c < GROUPS; ++c) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4 / GROUPS; ++e) {
+              const int of = c * (4 / GROUPS) + e;
+              most = fmaxf(most, max16(&r[of >> 1][(of & 1) * 16]));
+            }
+            top = fmaxf(top, fmaf(most, mul_of[c], add_of[c]));
+          }
           const float m_new = fmaxf(m, top);
           if (__any_sync(0xffffffffu, m != -INFINITY && m_new > m + kManySlack)) {
-            // the commit behind s_full covers every earlier product of this tile
+            // O is this warp's own once the last half's product has been added to it
+            if (!many_wait(&pv_done[2 * s + (b ^ 1)], (phase >> (b ^ 1) & 1) ^ 1, abort, a.status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
             const float w = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
             l *= w;
 #pragma unroll
@@ -1009,48 +1088,49 @@ __global__ void __launch_bounds__(384, 1)
           }
           if (m == -INFINITY) m = m_new;
           const float ref = (m == -INFINITY ? 0.f : m) - kManyBias;
+          float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[16];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int group = half * 4 + c * 2 + e;
-                float2 acc = make_float2(0.f, 0.f);
-                weigh16(&r[half * 2 + c][e * 16], group_mul(mul, scales[group]), scales[8 + group] - ref,
-                        acc, pk + 8 * e);
-                l = fmaf(acc.x + acc.y, scales[16 + group], l);
-              }
-              tmem_st16(tS + half * 32 + c * 16, pk);
+            for (int e = 0; e < 2; ++e) {
+              const int of = c * 2 + e, group = of * GROUPS / 4;
+              if (of % (4 / GROUPS) == 0) acc = make_float2(0.f, 0.f);
+              weigh16(&r[c][e * 16], mul_of[group], add_of[group] - ref, acc, pk + 8 * e);
+              if ((of + 1) % (4 / GROUPS) == 0) l = fmaf(acc.x + acc.y, scales[16 + of], l);
             }
-            if (half == 1 && partial) {
-              // values that are NaN in a tile that some row does not see whole: those rows that
-              // see the key take the NaN, in their channels, at the end
-              const int slot = block % L::kV16Stages;
-              if (!many_wait(&v16_full[slot], (block / L::kV16Stages) & 1, abort, a.status)) ok = false;
-              else if (nan_tile[slot] == block + 1) {
-                const uint4* bits = reinterpret_cast<const uint4*>(smem + L::kNanOffset) + slot * 128;
-                uint4 p = *poison;
-                for (int k = 0; k < kTileKeys && key0 + k <= last; ++k) {
-                  p.x |= bits[k].x;
-                  p.y |= bits[k].y;
-                  p.z |= bits[k].z;
-                  p.w |= bits[k].w;
-                }
-                *poison = p;
-              }
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_ready[2 * s + half]);
+            tmem_st16(tS + b * 64 + c * 16, pk);
           }
+          if (partial) {
+            // values that are NaN in a tile that some row does not see whole: the rows that see
+            // the key take the NaN, in its channels, at the end
+            const int v = tile % L::kV16Stages;
+            if (!many_wait(&v16_full[v], (tile / L::kV16Stages) & 1, abort, a.status)) ok = false;
+            else if (nan_tile[v] == tile + 1) {
+              const uint4* bits = reinterpret_cast<const uint4*>(smem + L::kNanOffset) + v * 128 + b * 64;
+              uint4 p = *poison;
+              for (int k = 0; k < 64 && half_key0 + k <= last; ++k) {
+                p.x |= bits[k].x;
+                p.y |= bits[k].y;
+                p.z |= bits[k].z;
+                p.w |= bits[k].w;
+              }
+              *poison = p;
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&p_ready[2 * s + b]);
         }
-        if (ok) ok = many_wait(&o_final[s], segment & 1, abort, a.status);
+        const int b = (halves - 1) & 1;
+        if (ok) ok = many_wait(&pv_done[2 * s + b], (phase >> b & 1) ^ 1, abort, a.status);
         tc_fence_after();
         if (!ok) break;
-        ++segment;
+        block += steps;
         // ---- the item's end, or this worker's part of it
+        const ManyAt at = many_get(place);
+        const int rows = many_rows(a, at), row = s * 128 + row128;
+        const int token = at.item * (kRowsMany / a.group) + row / a.group;
         const bool whole = steps == at.tiles;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const long long part = 2LL * blockIdx.x + (at.j == 0 ? 1 : 0);
@@ -1101,8 +1181,11 @@ __global__ void __launch_bounds__(384, 1)
       } else {
         block += steps;
       }
-      u += steps;
-      if (u < u1) many_next(a, at);
+      const int left = place[10] - steps;
+      if (left <= 0) break;
+      ManyAt at = many_get(place);
+      many_next(a, at);
+      many_put(place, at, left);
     }
   } else if (warp == 8) {
     // -------------------------------------------------------------- page numbers and copies
@@ -1190,79 +1273,83 @@ __global__ void __launch_bounds__(384, 1)
     for (int b = max(0, block - L::kV8Stages); b < block; ++b)
       many_wait(&v8_full[b % L::kV8Stages], (b / L::kV8Stages) & 1, &never, a.status);
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp < 11) {
     // ------------------------------------------------------------------ matrix instructions
+    // A warp for each query tile: a wait of a warp with products in flight takes about 300
+    // clocks even where its barrier is long complete (traced with clock64), and the queue of
+    // products is short, so one warp for both left the tensor cores idle between its turns.
+    const int s = warp - 9;
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyOtherRegs));
-    constexpr uint32_t kIdescQK = idesc_e4m3_f32(128, 128, false);
+    constexpr uint32_t kIdescQK = idesc_e4m3_f32(128, 64, false);
     constexpr uint32_t kIdescPV = idesc_e4m3_f32(128, HD, true);  // f16 has the same code, 0
-    const uint64_t dq = code_desc<HD>(smem_u32(smem + L::kQOffset));
+    const uint64_t dq = code_desc<HD>(smem_u32(smem + L::kQOffset + s * 2 * L::kCodeTile));
     const uint64_t dk = code_desc<HD>(smem_u32(smem + L::kKOffset));
     const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kV16Offset), 128 * 128, 1024);
     constexpr uint64_t kTile = L::kCodeTile >> 4;
-    auto issue_qk = [&](int s, int stage) {
+    const uint32_t ts = tmem + s * 128, to = tmem + 256u + s * HD;
+    auto issue_qk = [&](int b, int stage) {  // a half: 64 rows of K
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
-        const uint64_t q = dq + (2 * s + part) * kTile, k = dk + stage * kTile;
+        const uint64_t q = dq + part * kTile, k = dk + stage * kTile + b * (kTile / 2);
 #pragma unroll
         for (int kk = 0; kk < HD / 32; ++kk)
-          mma_ss_f8(tmem + s * 128, q + kk * 2, k + kk * 2, kIdescQK, part + kk > 0 ? 1u : 0u);
+          mma_ss_f8(ts + b * 64, q + kk * 2, k + kk * 2, kIdescQK, part + kk > 0 ? 1u : 0u);
       }
+      mma_commit(&s_full[2 * s + b]);
     };
-    auto issue_pv = [&](int s, int slot, uint32_t accumulate, int half) {
-      const uint64_t v = dv + slot * 2 * kTile;
+    auto issue_pv = [&](int b, int slot, uint32_t accumulate) {
+      const uint64_t v = dv + slot * 2 * kTile + ((b * 64 * 128) >> 4);
 #pragma unroll
-      for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-        mma_ts(tmem + 256u + s * HD, tmem + s * 128 + kk * 8, v + ((kk * 16 * 128) >> 4), kIdescPV,
-               kk > 0 ? 1u : accumulate);
+      for (int kk = 0; kk < 4; ++kk)
+        mma_ts(to, ts + b * 64 + kk * 8, v + ((kk * 16 * 128) >> 4),
+               kIdescPV, kk > 0 ? 1u : accumulate);
+      mma_commit(&pv_done[2 * s + b]);
     };
-    int block = 0, mine[2] = {0, 0}, segment[2] = {0, 0};
+    int block = 0;
+    uint32_t q_phase = 0, p_phase = 0;  // parities of q_ready, and of p_ready by half
     bool ok = true;
     ManyAt at = many_at(a, u0);
     for (long long u = u0; u < u1 && ok;) {
       const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.tiles - at.j)));
-      const int tiles = many_rows(a, at) > 128 ? 2 : 1;
-      for (int s = 0; s < tiles && ok; ++s)
-        ok = many_warp_wait(&q_ready[s], segment[s]++ & 1, abort, a.status);
-      if (!ok || !(ok = many_warp_wait(&k_full[block % L::kKStages], (block / L::kKStages) & 1, abort, a.status)))
-        break;
-      tc_fence_after();
-      if (elect_one()) {
-        for (int s = 0; s < tiles; ++s) {
-          issue_qk(s, block % L::kKStages);
-          mma_commit(&s_full[s]);
-        }
-        mma_commit(&k_empty[block % L::kKStages]);
+      const int halves = many_halves(a, at, steps);
+      const bool here = s * 128 < many_rows(a, at);
+      if (here) {
+        ok = many_warp_wait(&q_ready[s], q_phase, abort, a.status);
+        q_phase ^= 1;
       }
+      const int stage0 = block % L::kKStages;
+      if (!ok || !(ok = many_warp_wait(&k_full[stage0], (block / L::kKStages) & 1, abort, a.status))) break;
+      tc_fence_after();
+      if (here && elect_one()) {
+        for (int b = 0; b < min(2, halves); ++b) issue_qk(b, stage0);
+        mma_commit(&k_empty[stage0]);
+      }
+      if (!here && lane == 0) mbar_arrive(&k_empty[stage0]);
       __syncwarp();
-      for (int step = 0; step < steps && ok; ++step, ++block) {
-        const bool more = step + 1 < steps;
-        const int slot = block % L::kV16Stages, next = (block + 1) % L::kKStages;
-        if (!(ok = many_warp_wait(&v16_full[slot], (block / L::kV16Stages) & 1, abort, a.status))) break;
-        if (more && !(ok = many_warp_wait(&k_full[next], ((block + 1) / L::kKStages) & 1, abort, a.status))) break;
-        for (int s = 0; s < tiles && ok; ++s) {
-          if (!(ok = many_warp_wait(&p_ready[2 * s], mine[s] & 1, abort, a.status))) break;
-          tc_fence_after();
-          if (elect_one()) issue_pv(s, slot, step > 0 ? 1u : 0u, 0);
-          __syncwarp();
-          if (!(ok = many_warp_wait(&p_ready[2 * s + 1], mine[s] & 1, abort, a.status))) break;
-          ++mine[s];
+      for (int h = 0; h < halves; ++h) {
+        const int b = h & 1, tile = block + (h >> 1), slot = tile % L::kV16Stages;
+        const int stage = (tile + 1) % L::kKStages;
+        const bool more = h + 2 < halves;
+        // this tile's V and the next one's K
+        if (b == 0 && !(ok = many_warp_wait(&v16_full[slot], (tile / L::kV16Stages) & 1, abort, a.status)))
+          break;
+        if (here) {
+          if (!(ok = many_warp_wait(&p_ready[2 * s + b], p_phase >> b & 1, abort, a.status))) break;
+          p_phase ^= 1u << b;
           tc_fence_after();
           if (elect_one()) {
-            issue_pv(s, slot, step > 0 ? 1u : 0u, 1);
-            if (more) {
-              issue_qk(s, next);
-              mma_commit(&s_full[s]);
-            } else {
-              mma_commit(&o_final[s]);
-            }
-            if (s + 1 == tiles) {
-              mma_commit(&v16_empty[slot]);
-              if (more) mma_commit(&k_empty[next]);
-            }
+            issue_pv(b, slot, h > 0 ? 1u : 0u);
+            if (more) issue_qk(b, stage);
+            if (b == 1 || h + 1 == halves) mma_commit(&v16_empty[slot]);
+            if (more && (b == 1 || h + 3 == halves)) mma_commit(&k_empty[stage]);
           }
-          __syncwarp();
+        } else if (b == 0 && lane == 0) {  // no rows here: only the tiles are given back
+          mbar_arrive(&v16_empty[slot]);
+          if (more) mbar_arrive(&k_empty[stage]);
         }
+        __syncwarp();
       }
+      block += steps;
       u += steps;
       if (ok && u < u1) many_next(a, at);
     }
@@ -1272,11 +1359,13 @@ __global__ void __launch_bounds__(384, 1)
     volatile int never = 0;
     many_wait(drain, 0, &never, a.status);
     __syncwarp();
+  } else if (warp == 11) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyOtherRegs));
   } else {
     // ----------------------------------------------------------------- V's codes to f16
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyOtherRegs));
     constexpr int CH = HD / 16;  // 16-byte chunks of a row of codes
-    const int tid = threadIdx.x - 320;
+    const int tid = threadIdx.x - 384;
     int block = 0;
     bool ok = true;
     ManyAt at = many_at(a, u0);
@@ -1297,8 +1386,8 @@ __global__ void __launch_bounds__(384, 1)
         const uint32_t from = smem_u32(smem + L::kV8Offset + in * L::kCodeTile);
         const uint32_t to = smem_u32(smem + L::kV16Offset + slot * 2 * L::kCodeTile);
 #pragma unroll 4
-        for (int i = 0; i < 128 * CH / 64; ++i) {
-          const int index = i * 64 + tid, row = index / CH, c = index % CH;
+        for (int i = 0; i < 128 * CH / kWideners; ++i) {
+          const int index = i * kWideners + tid, row = index / CH, c = index % CH;
           uint4 v = lds128(from + index * 16);
           if (partial) {
             if (key0 + row >= at.keys || (gone >> (row / 16) & 1)) v = make_uint4(0, 0, 0, 0);
@@ -1330,8 +1419,11 @@ __global__ void __launch_bounds__(384, 1)
           sts128(box + (((j + 1 - turn) ^ (row & 7)) << 4), turn ? w0 : w1);
         }
         fence_async_smem();
-        mbar_arrive(&v16_full[slot]);
         mbar_arrive(&v8_empty[in]);
+        if (step + 1 < steps &&
+            !(ok = many_wait(&k_full[(block + 1) % L::kKStages], ((block + 1) / L::kKStages) & 1, abort, a.status)))
+          break;
+        mbar_arrive(&v16_full[slot]);
       }
       u += steps;
       if (ok && u < u1) many_next(a, at);
@@ -1501,7 +1593,7 @@ static int few_launch(const CozyCacheStore& c, CacheArgs& a, int longest, cudaSt
   return join_launch(join_few<HD>, dim3(a.requests * a.heads_kv, a.group * longest), a, stream);
 }
 
-template <int HD>
+template <int HD, int GROUPS>
 static int many_launch(const CozyCacheStore& c, CacheArgs& a, cudaStream_t stream) {
   using L = Many<HD>;
   static bool configured[64] = {};
@@ -1509,7 +1601,7 @@ static int many_launch(const CozyCacheStore& c, CacheArgs& a, cudaStream_t strea
   cudaGetDevice(&device);
   if (device < 64 && !configured[device]) {
     const cudaError_t e = cudaFuncSetAttribute(
-        attend_many<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
+        attend_many<HD, GROUPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
     if (e != cudaSuccess) return e;
     configured[device] = true;
   }
@@ -1517,7 +1609,7 @@ static int many_launch(const CozyCacheStore& c, CacheArgs& a, cudaStream_t strea
   const int box = c.page < kTileKeys ? c.page : kTileKeys;
   int e = code_map(&mk, c.key, c, box, true);
   if (e || (e = code_map(&mv, c.value, c, box, false))) return e;
-  attend_many<HD><<<a.workers, L::kThreads, L::kAlloc, stream>>>(mk, mv, a);
+  attend_many<HD, GROUPS><<<a.workers, L::kThreads, L::kAlloc, stream>>>(mk, mv, a);
   if ((e = cudaGetLastError())) return e;
   if (a.workers < 2) return cudaSuccess;
   return join_launch(join_many<HD>, dim3(a.workers - 1, kRowsMany / 32), a, stream);
@@ -1570,7 +1662,13 @@ int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyC
                             : few_launch<128>(c, a, p.longest, stream);
   }
   a.workers = device_sms();
-  return c.head_dim == 64 ? many_launch<64>(c, a, stream) : many_launch<128>(c, a, stream);
+  if (c.head_dim == 64)
+    return c.page >= 64   ? many_launch<64, 1>(c, a, stream)
+           : c.page == 32 ? many_launch<64, 2>(c, a, stream)
+                          : many_launch<64, 4>(c, a, stream);
+  return c.page >= 64   ? many_launch<128, 1>(c, a, stream)
+         : c.page == 32 ? many_launch<128, 2>(c, a, stream)
+                        : many_launch<128, 4>(c, a, stream);
 }
 
 }  // namespace cozy

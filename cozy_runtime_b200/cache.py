@@ -160,9 +160,9 @@ class Plan:
         n, page, device = lengths.shape[0], layout.page, table.device
         blocks = min(tokens, tokens // page + 2 * n)
         # `blocks` entries are 16 bytes and stand first, in front of the status word
-        self._cuts = (4 * blocks, 1, n, n + 1, tokens), (2, n + 1, tokens)
+        self._cuts = (4 * blocks, 1, n, n + 1, tokens), (2, 2 * n + 2, tokens)
         whole = torch.empty(4 * blocks + 2 * n + 2 + tokens, dtype=torch.int32, device=device)
-        wide = torch.empty(n + 3 + tokens, dtype=torch.int64, device=device)
+        wide = torch.empty(2 * n + 4 + tokens, dtype=torch.int64, device=device)
         self._buffers = whole, wide
         self.layout, self.table, self.tokens, self.longest = layout, table, tokens, longest
         self.requests, self.pages = n, free.shape[0]
@@ -174,7 +174,7 @@ class Plan:
             lengths.data_ptr(), new.data_ptr(), table.data_ptr(),
             max(table.stride(0), table.shape[1]), free.data_ptr(), cursor.data_ptr(), n,
             table.shape[1], free.shape[0], page, tokens, longest, layout.group, blocks,
-            status + 4, status + 4 + 4 * n, at8, status + 8 + 8 * n, at8 + 8 * (n + 3), at,
+            status + 4, status + 4 + 4 * n, at8, status + 8 + 8 * n, at8 + 8 * (2 * n + 4), at,
             at8 + 16, status,
         )
 

@@ -21,7 +21,7 @@ namespace cozy {
 constexpr int kPlanThreads = 1024;
 
 struct PlanSums {
-  long long tokens, need, back, blocks, units;
+  long long tokens, need, back, blocks, few, many;
 };
 
 __device__ __forceinline__ PlanSums operator+(PlanSums a, const PlanSums& b) {
@@ -29,7 +29,8 @@ __device__ __forceinline__ PlanSums operator+(PlanSums a, const PlanSums& b) {
   a.need += b.need;
   a.back += b.back;
   a.blocks += b.blocks;
-  a.units += b.units;
+  a.few += b.few;
+  a.many += b.many;
   return a;
 }
 
@@ -39,7 +40,8 @@ __device__ __forceinline__ PlanSums shifted(const PlanSums& a, int by) {
   r.need = __shfl_up_sync(0xffffffffu, a.need, by);
   r.back = __shfl_up_sync(0xffffffffu, a.back, by);
   r.blocks = __shfl_up_sync(0xffffffffu, a.blocks, by);
-  r.units = __shfl_up_sync(0xffffffffu, a.units, by);
+  r.few = __shfl_up_sync(0xffffffffu, a.few, by);
+  r.many = __shfl_up_sync(0xffffffffu, a.many, by);
   return r;
 }
 
@@ -68,7 +70,9 @@ __device__ __forceinline__ PlanSums request_sums(const CozyCachePlan& p, int n, 
   s.need = want - held;
   if (added > 0) {
     s.blocks = want - length / p.page;
-    s.units = attention_units(p.group, p.longest, length, added);
+    const long long units = attention_units(p.group, length, added);
+    if (few_rows(p.group, added)) s.few = units;
+    else s.many = units;
   }
   return s;
 }
@@ -135,7 +139,10 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const CozyCach
       needs[n + 1] = static_cast<int>(end.need);
       backs[n + 1] = static_cast<int>(end.back);
       blocks[n + 1] = static_cast<int>(end.blocks);
-      if (lead) p.units[n + 1] = end.units;
+      if (lead) {
+        p.units[n + 1] = end.few;
+        p.units[n1 + n + 1] = end.many;
+      }
     }
     carry = carry + warp_sums[31];
     __syncthreads();
@@ -152,12 +159,12 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const CozyCach
   if (refused) {
     for (int n = threadIdx.x; n < n1; n += kPlanThreads) {
       starts[n] = 0;
-      if (lead) p.units[n] = 0;
+      if (lead) p.units[n] = p.units[n1 + n] = 0;
     }
     carry = PlanSums{};
   } else if (threadIdx.x == 0) {
     starts[0] = needs[0] = backs[0] = blocks[0] = 0;
-    if (lead) p.units[0] = 0;
+    if (lead) p.units[0] = p.units[n1] = 0;
   }
   if (lead && threadIdx.x == 0) {
     *p.status = status;

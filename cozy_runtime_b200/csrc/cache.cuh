@@ -45,36 +45,48 @@ __host__ __device__ __forceinline__ float exponent_scale(int e) {
 #endif
 }
 
-// Σ floor((a·i + b) / m) for i in [0, n), a, b ≥ 0 (the Euclid-like recursion on a and m).
-__host__ __device__ inline long long floor_sum(long long n, long long m, long long a, long long b) {
-  long long sum = 0;
-  while (n > 0) {
-    sum += (n - 1) * n / 2 * (a / m) + n * (b / m);
-    a %= m;
-    b %= m;
-    const long long top = a * n + b;
-    if (top < m) break;
-    n = top / m;
-    b = top % m;
-    const long long t = a;
+// a / b of counts: the 64-bit division is many times the 32-bit one, which mostly does.
+__host__ __device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// Σ floor((a·i + b) / 128) for i in [0, n), 0 ≤ a ≤ 256, 0 ≤ b, n < 2^24: the Euclid-like recursion
+// on the divisor and a; behind its first step everything is below 2^31.
+__host__ __device__ inline long long floor_sum_128(uint32_t n, uint32_t a, long long b) {
+  if (n == 0) return 0;
+  long long sum = static_cast<long long>(n) * (n - 1) / 2 * (a >> 7) + n * (b >> 7);
+  uint32_t m = 128, c = static_cast<uint32_t>(b) & 127u;
+  a &= 127u;
+  for (;;) {
+    const uint32_t top = a * n + c;
+    if (top < m) return sum;
+    n = top / m;  // at least 1
+    c = top - n * m;
+    const uint32_t old = a;
     a = m;
-    m = t;
+    m = old;
+    sum += static_cast<long long>(n) * (n - 1) / 2 * (a / m) + static_cast<long long>(n) * (c / m);
+    a %= m;
+    c %= m;
   }
-  return sum;
 }
 
 // ------------------------------------------------------------------------ the attention's work
-// A request's new tokens × the group's query heads are the rows that read one key/value head.
-// Up to kRowsFew of them share one pass over the keys in chunks of kChunkKeys; more are cut into
-// items of kRowsMany rows (whole tokens) whose keys are walked in tiles of kTileKeys. A unit is
-// one chunk or tile; `units[n]` of a plan counts the units of one key/value head before request n.
+// A request's new tokens × the group's query heads are the rows that read one key/value head. Each
+// request goes by its own rows: up to kFewItems items of kRowsFew rows (whole tokens) walk the
+// keys in chunks of kChunkKeys; more rows are cut into items of kRowsMany whose keys are walked in
+// tiles of kTileKeys. A unit is one chunk or tile; a plan counts the units of one key/value head
+// before each request, of either kind. (An item of few rows reads its keys again, from L2: on a
+// B200 20 rows took X us as two such items and Y as one item of many, Z against W at 60.)
 constexpr int kRowsFew = 16;
+constexpr int kFewItems = 3;
 constexpr int kChunkKeys = 64;
 constexpr int kRowsMany = 256;
 constexpr int kTileKeys = 128;
 
-__host__ __device__ __forceinline__ bool few_rows(int group, int longest) {
-  return static_cast<long long>(group) * longest <= kRowsFew;
+__host__ __device__ __forceinline__ bool few_rows(int group, long long added) {
+  return group <= kRowsFew && added <= kFewItems * (kRowsFew / group);
 }
 
 // Tiles before item `item` of a request with `cached` tokens before its new ones: item i's last
@@ -82,14 +94,19 @@ __host__ __device__ __forceinline__ bool few_rows(int group, int longest) {
 __host__ __device__ __forceinline__ long long tiles_before(int group, long long cached,
                                                            long long item) {
   const int per = kRowsMany / group;
-  return floor_sum(item, kTileKeys, per, cached + per + kTileKeys - 1);
+  return floor_sum_128(static_cast<uint32_t>(item), per, cached + per + kTileKeys - 1);
 }
 
-__host__ __device__ __forceinline__ long long attention_units(int group, int longest,
-                                                              long long cached, long long added) {
-  if (few_rows(group, longest)) return (cached + added + kChunkKeys - 1) / kChunkKeys;
+// Units of one key/value head of a request: of few rows, or of many.
+__host__ __device__ __forceinline__ long long attention_units(int group, long long cached,
+                                                              long long added) {
+  if (added == 0) return 0;
+  if (few_rows(group, added)) {
+    const int per = kRowsFew / group;
+    return quotient(added + per - 1, per) * ((cached + added + kChunkKeys - 1) / kChunkKeys);
+  }
   const int per = kRowsMany / group;
-  const long long items = (added + per - 1) / per;
+  const long long items = quotient(added + per - 1, per);
   return tiles_before(group, cached, items - 1) + (cached + added + kTileKeys - 1) / kTileKeys;
 }
 

@@ -27,7 +27,8 @@ struct CacheArgs {
   long long table_stride;
   const int* starts;
   const int* lengths;
-  const long long* units;
+  const long long* units_few;   // [requests + 1] units of one head before each request
+  const long long* units_many;  // (a request has units of one kind only)
   int* status;
   int requests, pages, page, group, heads_kv;
   const int8_t* key_exponent;
@@ -114,13 +115,13 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {
 
 // The request whose units hold `u` (units of all its heads), by all lanes together: 32 places
 // of the search range are read at once, so 8192 requests take three rounds.
-__device__ __forceinline__ int request_of(const CacheArgs& a, long long u) {
+__device__ __forceinline__ int request_of(const CacheArgs& a, const long long* units, long long u) {
   const int lane = threadIdx.x & 31;
   int low = 0, count = a.requests;  // the answer is in [low, low + count)
   while (count > 1) {
     const int step = (count + 31) / 32;
     const int at = low + lane * step;
-    const bool before = lane * step < count && a.units[at] * a.heads_kv <= u;
+    const bool before = lane * step < count && units[at] * a.heads_kv <= u;
     const int last = 31 - __clz(__ballot_sync(0xffffffffu, before));
     const int used = last * step;
     low += used;
@@ -152,22 +153,27 @@ struct Few {
 
 // A position in the order of units, moved on chunk by chunk.
 struct FewAt {
-  int n, h, j, chunks;  // request, head, chunk, chunks of an item
-  int keys;             // the request's tokens
+  int n, h, item, j;  // request, head, rows of it, chunk of keys
+  int items, chunks;  // items of a head, chunks of an item
+  int keys;           // the request's tokens
 };
 
 __device__ __forceinline__ void few_request(const CacheArgs& a, FewAt& at, int n) {
+  const int per = kRowsFew / a.group;  // tokens an item
   at.n = n;
-  at.chunks = static_cast<int>(a.units[n + 1] - a.units[n]);
   at.keys = a.lengths[n];
+  at.items = a.units_few[n + 1] == a.units_few[n] ? 0 : (a.starts[n + 1] - a.starts[n] + per - 1) / per;
+  at.chunks = (at.keys + kChunkKeys - 1) / kChunkKeys;
 }
 
 __device__ __forceinline__ FewAt few_at(const CacheArgs& a, long long u) {
   FewAt at;
-  few_request(a, at, request_of(a, u));
-  const long long within = u - a.units[at.n] * a.heads_kv;
-  at.h = static_cast<int>(within / at.chunks);
-  at.j = static_cast<int>(within - static_cast<long long>(at.h) * at.chunks);
+  few_request(a, at, request_of(a, a.units_few, u));
+  const long long within = u - a.units_few[at.n] * a.heads_kv;
+  const long long item = quotient(within, at.chunks);
+  at.j = static_cast<int>(within - item * at.chunks);
+  at.h = static_cast<int>(quotient(item, at.items));
+  at.item = static_cast<int>(item - static_cast<long long>(at.h) * at.items);
   return at;
 }
 
@@ -175,10 +181,12 @@ __device__ __forceinline__ FewAt few_at(const CacheArgs& a, long long u) {
 __device__ __forceinline__ bool few_next(const CacheArgs& a, FewAt& at) {
   if (++at.j < at.chunks) return false;
   at.j = 0;
+  if (++at.item < at.items) return true;
+  at.item = 0;
   if (++at.h == a.heads_kv) {
     at.h = 0;
     do few_request(a, at, at.n + 1);
-    while (at.chunks == 0);  // only reached while units remain
+    while (at.items == 0);  // only reached while units remain
   }
   return true;
 }
@@ -201,11 +209,11 @@ __global__ void __launch_bounds__(256, 1)
   float2* meta = reinterpret_cast<float2*>(smem + L::kMetaOffset) + warp * L::kMeta * 4;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const long long total = a.units[a.requests] * a.heads_kv;
+  const long long total = a.units_few[a.requests] * a.heads_kv;
   const int workers = static_cast<int>(min(static_cast<long long>(a.workers), total));
   const int worker = warp * gridDim.x + blockIdx.x;
   if (worker >= workers) return;  // warps share nothing
-  const long long u0 = worker * total / workers, u1 = (worker + 1) * total / workers;
+  const long long u0 = quotient(worker * total, workers), u1 = quotient((worker + 1) * total, workers);
   if (lane == 0) {
     for (int i = 0; i < L::kSlots; ++i) mbar_init(&full[i], 1);
     fence_barrier_init();
@@ -287,10 +295,11 @@ __global__ void __launch_bounds__(256, 1)
   long long u = u0;
   while (u < u1 && ok) {
     // ---- an item, or the part of it that this worker has
-    const int first_token = a.starts[at.n];
-    const int added = a.starts[at.n + 1] - first_token;
-    const int rows = added * a.group;
-    const int seen0 = at.keys - added;  // keys before the step's own
+    const int per = kRowsFew / a.group;
+    const int first_token = a.starts[at.n] + at.item * per;
+    const int left = a.starts[at.n + 1] - first_token;  // tokens from the item's first on
+    const int rows = min(left, per) * a.group;
+    const int seen0 = at.keys - left;  // keys before the item's own
     const int j0 = at.j;
     const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.chunks - at.j)));
     // rows g and g + 8: query times a power of two that puts its largest value in [2^14, 2^15)
@@ -558,14 +567,17 @@ __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
   constexpr int PER = HD / 32;  // channels a lane
   __shared__ float sum_o[8][HD];
   __shared__ float2 sum_ml[8];
-  const int n = blockIdx.x / a.heads_kv, h = blockIdx.x % a.heads_kv, row = blockIdx.y;
-  const int rows = (a.starts[n + 1] - a.starts[n]) * a.group;
-  const long long chunks = a.units[n + 1] - a.units[n];
-  const long long total = a.units[a.requests] * a.heads_kv;
+  const int n = blockIdx.x / a.heads_kv, h = blockIdx.x % a.heads_kv;
+  const int per = kRowsFew / a.group, item = blockIdx.y / (per * a.group), row = blockIdx.y % (per * a.group);
+  const int first_token = a.starts[n] + item * per;
+  const int rows = a.units_few[n + 1] == a.units_few[n] ? 0 : (a.starts[n + 1] - first_token) * a.group;
+  const int items = (a.starts[n + 1] - a.starts[n] + per - 1) / per;
+  const long long chunks = (a.lengths[n] + kChunkKeys - 1) / kChunkKeys;
+  const long long total = a.units_few[a.requests] * a.heads_kv;
   const long long workers = min(static_cast<long long>(a.workers), total);
-  const long long u0 = a.units[n] * a.heads_kv + h * chunks;
-  const int first = total == 0 ? 0 : static_cast<int>(((u0 + 1) * workers - 1) / total);
-  const int last = total == 0 ? 0 : static_cast<int>(((u0 + chunks) * workers - 1) / total);
+  const long long u0 = a.units_few[n] * a.heads_kv + (static_cast<long long>(h) * items + item) * chunks;
+  const int first = total == 0 ? 0 : static_cast<int>(quotient((u0 + 1) * workers - 1, total));
+  const int last = total == 0 ? 0 : static_cast<int>(quotient((u0 + chunks) * workers - 1, total));
   const bool split = row < rows && first != last;
   // one block at least waits, so that this grid does not end before the one it follows
   if (split || (blockIdx.x == 0 && blockIdx.y == 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -604,7 +616,7 @@ __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
     value += sum_o[w][d] * mine;
     sum += sum_ml[w].y * mine;
   }
-  const int token = a.starts[n] + row / a.group, head = h * a.group + row % a.group;
+  const int token = first_token + row / a.group, head = h * a.group + row % a.group;
   a.out[token * a.o_token + head * a.o_head + d] = __float2bfloat16(sum == 0.f ? 0.f : value / sum);
   if (a.lse != nullptr && d == 0)
     a.lse[static_cast<long long>(token) * a.heads_kv * a.group + head] =
@@ -690,15 +702,15 @@ __device__ __forceinline__ void many_request(const CacheArgs& a, ManyAt& at, int
   at.added = a.starts[n + 1] - at.first_token;
   at.keys = a.lengths[n];
   at.cached = at.keys - at.added;
-  at.items = (at.added + per - 1) / per;
+  at.items = a.units_many[n + 1] == a.units_many[n] ? 0 : (at.added + per - 1) / per;
 }
 
 __device__ __forceinline__ ManyAt many_at(const CacheArgs& a, long long u) {
   ManyAt at;
-  many_request(a, at, request_of(a, u));
-  const long long units = a.units[at.n + 1] - a.units[at.n];
-  const long long within = u - a.units[at.n] * a.heads_kv;
-  at.h = static_cast<int>(within / units);
+  many_request(a, at, request_of(a, a.units_many, u));
+  const long long units = a.units_many[at.n + 1] - a.units_many[at.n];
+  const long long within = u - a.units_many[at.n] * a.heads_kv;
+  at.h = static_cast<int>(quotient(within, units));
   const long long rest = within - at.h * units;
   int low = 0, high = at.items - 1;
   while (low < high) {
@@ -720,7 +732,7 @@ __device__ __forceinline__ void many_next(const CacheArgs& a, ManyAt& at) {
     if (++at.h == a.heads_kv) {
       at.h = 0;
       do many_request(a, at, at.n + 1);
-      while (at.added == 0);  // only reached while units remain
+      while (at.items == 0);  // only reached while units remain
     }
   }
   many_item(a, at);
@@ -808,15 +820,19 @@ __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
                : "memory");
 }
 
-// Descriptor of a K-major tile of codes: rows of HD bytes in the swizzle of that width
-// (layout type 2: 128 bytes, 4: 64 bytes), 8 rows an atom.
-template <int HD>
-__device__ __forceinline__ uint64_t code_desc(uint32_t at) {
-  uint64_t d = static_cast<uint64_t>((at & 0x3FFFFu) >> 4);
-  d |= 1ull << 16;
-  d |= static_cast<uint64_t>((8 * HD) >> 4) << 32;
-  d |= 1ull << 46;
-  d |= (HD == 128 ? 2ull : 4ull) << 61;
+// Matrix descriptors (the layout that sm100.cuh states), kept as their low words: the start
+// address, and LBO where it counts. The high words are constants.
+__host__ __device__ constexpr uint32_t desc_high(uint32_t stride_bytes, uint32_t layout) {
+  return stride_bytes >> 4 | 1u << 14 | layout << 29;
+}
+
+__device__ __forceinline__ uint32_t desc_low(uint32_t at, uint32_t lbo_bytes) {
+  return (at & 0x3FFFFu) >> 4 | lbo_bytes >> 4 << 16;
+}
+
+__device__ __forceinline__ uint64_t desc(uint32_t low, uint32_t high) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
   return d;
 }
 
@@ -887,10 +903,10 @@ __global__ void __launch_bounds__(512, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const long long total = a.units[a.requests] * a.heads_kv;
+  const long long total = a.units_many[a.requests] * a.heads_kv;
   const int workers = static_cast<int>(min(static_cast<long long>(a.workers), total));
   if (static_cast<int>(blockIdx.x) >= workers) return;
-  const long long u0 = blockIdx.x * total / workers, u1 = (blockIdx.x + 1) * total / workers;
+  const long long u0 = quotient(blockIdx.x * total, workers), u1 = quotient((blockIdx.x + 1) * total, workers);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -1282,27 +1298,29 @@ __global__ void __launch_bounds__(512, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyOtherRegs));
     constexpr uint32_t kIdescQK = idesc_e4m3_f32(128, 64, false);
     constexpr uint32_t kIdescPV = idesc_e4m3_f32(128, HD, true);  // f16 has the same code, 0
-    const uint64_t dq = code_desc<HD>(smem_u32(smem + L::kQOffset + s * 2 * L::kCodeTile));
-    const uint64_t dk = code_desc<HD>(smem_u32(smem + L::kKOffset));
-    const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kV16Offset), 128 * 128, 1024);
-    constexpr uint64_t kTile = L::kCodeTile >> 4;
+    // K-major codes in the swizzle of a row's width, 8 rows an atom; V in 128-byte boxes
+    constexpr uint32_t kCodes = desc_high(8 * HD, HD == 128 ? 2 : 4), kValues = desc_high(1024, 2);
+    const uint32_t q0 = desc_low(smem_u32(smem + L::kQOffset) + s * 2 * L::kCodeTile, 16);
+    const uint32_t k0 = desc_low(smem_u32(smem + L::kKOffset), 16);
+    const uint32_t v0 = desc_low(smem_u32(smem + L::kV16Offset), 128 * 128);
+    constexpr uint32_t kTile = L::kCodeTile >> 4;
     const uint32_t ts = tmem + s * 128, to = tmem + 256u + s * HD;
     auto issue_qk = [&](int b, int stage) {  // a half: 64 rows of K
+      const uint32_t k = k0 + stage * kTile + b * (kTile / 2);
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        const uint64_t q = dq + part * kTile, k = dk + stage * kTile + b * (kTile / 2);
+      for (int part = 0; part < 2; ++part)
 #pragma unroll
         for (int kk = 0; kk < HD / 32; ++kk)
-          mma_ss_f8(ts + b * 64, q + kk * 2, k + kk * 2, kIdescQK, part + kk > 0 ? 1u : 0u);
-      }
+          mma_ss_f8(ts + b * 64, desc(q0 + part * kTile + kk * 2, kCodes), desc(k + kk * 2, kCodes),
+                    kIdescQK, part + kk > 0 ? 1u : 0u);
       mma_commit(&s_full[2 * s + b]);
     };
     auto issue_pv = [&](int b, int slot, uint32_t accumulate) {
-      const uint64_t v = dv + slot * 2 * kTile + ((b * 64 * 128) >> 4);
+      const uint32_t v = v0 + slot * 2 * kTile + ((b * 64 * 128) >> 4);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
-        mma_ts(to, ts + b * 64 + kk * 8, v + ((kk * 16 * 128) >> 4),
-               kIdescPV, kk > 0 ? 1u : accumulate);
+        mma_ts(to, ts + b * 64 + kk * 8, desc(v + ((kk * 16 * 128) >> 4), kValues), kIdescPV,
+               kk > 0 ? 1u : accumulate);
       mma_commit(&pv_done[2 * s + b]);
     };
     int block = 0;
@@ -1443,19 +1461,19 @@ __global__ void __launch_bounds__(512, 1)
 template <int HD>
 __global__ void __launch_bounds__(256) join_many(const CacheArgs a) {
   constexpr int PER = HD / 32;  // float4 columns a warp
-  const long long total = a.units[a.requests] * a.heads_kv;
+  const long long total = a.units_many[a.requests] * a.heads_kv;
   const long long workers = min(static_cast<long long>(a.workers), total);
   const int w = blockIdx.x + 1;
   bool split = w < workers;
   ManyAt at;
   int last = 0, rows = 0;
   if (split) {
-    const long long u = w * total / workers;
+    const long long u = quotient(w * total, workers);
     at = many_at(a, u);
     const long long u0 = u - at.j;
     rows = many_rows(a, at);
-    split = at.j > 0 && (w - 1) * total / workers <= u0 && static_cast<int>(blockIdx.y) * 32 < rows;
-    last = static_cast<int>(((u0 + at.tiles) * workers - 1) / total);
+    split = at.j > 0 && quotient((w - 1) * total, workers) <= u0 && static_cast<int>(blockIdx.y) * 32 < rows;
+    last = static_cast<int>(quotient((u0 + at.tiles) * workers - 1, total));
   }
   if (split || (blockIdx.x == 0 && blockIdx.y == 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!split) return;
@@ -1548,14 +1566,21 @@ static int device_sms() {
 
 static long long few_workers() { return static_cast<long long>(device_sms()) * 8; }
 
-// Rows of partial results a call may leave: two parts a worker.
-static long long part_rows(const CozyCachePlan& p) {
-  return few_rows(p.group, p.longest) ? few_workers() * 2 * kRowsFew
-                                      : static_cast<long long>(device_sms()) * 2 * kRowsMany;
+// Bytes of partial results that the kernels of a call may leave: two parts a worker.
+static size_t few_bytes(int head_dim) {
+  return few_workers() * 2 * kRowsFew * (head_dim * sizeof(float) + sizeof(float2));
 }
 
+static size_t many_bytes(int head_dim) {
+  return static_cast<size_t>(device_sms()) * 2 * kRowsMany * (head_dim * sizeof(float) + sizeof(float2));
+}
+
+// Which kernels a step needs, as far as the host knows: some request may have few rows, or many.
+static bool may_be_few(const CozyCachePlan& p) { return p.group <= kRowsFew; }
+static bool may_be_many(const CozyCachePlan& p) { return !few_rows(p.group, p.longest); }
+
 long long cache_workspace(const CozyCachePlan& p, const CozyCacheStore& c) {
-  return part_rows(p) * (c.head_dim * sizeof(float) + sizeof(float2));
+  return (may_be_few(p) ? few_bytes(c.head_dim) : 0) + (may_be_many(p) ? many_bytes(c.head_dim) : 0);
 }
 
 // A join starts while its attention runs and waits for that one's end on the device.
@@ -1573,7 +1598,7 @@ static int join_launch(void (*kernel)(CacheArgs), dim3 grid, const CacheArgs& a,
 }
 
 template <int HD>
-static int few_launch(const CozyCacheStore& c, CacheArgs& a, int longest, cudaStream_t stream) {
+static int few_launch(const CozyCacheStore& c, CacheArgs& a, int rows, cudaStream_t stream) {
   using L = Few<HD>;
   static bool configured[64] = {};
   int device = 0;
@@ -1590,7 +1615,7 @@ static int few_launch(const CozyCacheStore& c, CacheArgs& a, int longest, cudaSt
   if (e || (e = code_map(&mv, c.value, c, box, true))) return e;
   attend_few<HD><<<device_sms(), 256, L::kAlloc, stream>>>(mk, mv, a);
   if ((e = cudaGetLastError())) return e;
-  return join_launch(join_few<HD>, dim3(a.requests * a.heads_kv, a.group * longest), a, stream);
+  return join_launch(join_few<HD>, dim3(a.requests * a.heads_kv, rows), a, stream);
 }
 
 template <int HD, int GROUPS>
@@ -1636,7 +1661,8 @@ int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyC
   a.table_stride = p.table_stride;
   a.starts = p.starts;
   a.lengths = p.lengths_after;
-  a.units = p.units;
+  a.units_few = p.units;
+  a.units_many = p.units + p.requests + 1;
   a.status = p.status;
   a.requests = p.requests;
   a.pages = p.pages;
@@ -1653,15 +1679,24 @@ int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyC
   a.o_head = x.out_strides[1];
   a.lse = x.lse;
   a.scale_log2 = x.scale * 1.4426950408889634f;
-  a.ws_o = static_cast<float*>(x.workspace);
-  a.ws_ml = reinterpret_cast<float2*>(a.ws_o + part_rows(p) * c.head_dim);
-  if (few_rows(p.group, p.longest)) {
+  uint8_t* space = static_cast<uint8_t*>(x.workspace);
+  if (may_be_few(p)) {
     if (static_cast<long long>(p.requests) * c.heads_kv > 0x7fffffffLL) return cudaErrorInvalidValue;
     a.workers = static_cast<int>(few_workers());
-    return c.head_dim == 64 ? few_launch<64>(c, a, p.longest, stream)
-                            : few_launch<128>(c, a, p.longest, stream);
+    a.ws_o = reinterpret_cast<float*>(space);
+    a.ws_ml = reinterpret_cast<float2*>(a.ws_o + few_workers() * 2 * kRowsFew * c.head_dim);
+    space += few_bytes(c.head_dim);
+    // rows that an item of few rows can have: whole tokens
+    const int per = kRowsFew / p.group;
+    const long long tokens = p.longest < kFewItems * per ? p.longest : kFewItems * per;
+    const int rows = static_cast<int>(tokens) * p.group;
+    const int r = c.head_dim == 64 ? few_launch<64>(c, a, rows, stream) : few_launch<128>(c, a, rows, stream);
+    if (r) return r;
   }
+  if (!may_be_many(p)) return cudaSuccess;
   a.workers = device_sms();
+  a.ws_o = reinterpret_cast<float*>(space);
+  a.ws_ml = reinterpret_cast<float2*>(a.ws_o + static_cast<size_t>(device_sms()) * 2 * kRowsMany * c.head_dim);
   if (c.head_dim == 64)
     return c.page >= 64   ? many_launch<64, 1>(c, a, stream)
            : c.page == 32 ? many_launch<64, 2>(c, a, stream)

@@ -500,7 +500,8 @@ typedef struct CozyCachePlan {
   long long* slots;        /* [tokens] page number * page + row in the page, or -1 */
   int* blocks;             /* [max_blocks][4], 16-byte aligned: page (-1: none), first row, rows,
                               first token: the blocks this step's tokens go into */
-  long long* units;        /* [requests + 1] units of attention before each request, a head */
+  long long* units;        /* [2][requests + 1] units of attention before each request, a head:
+                              of requests of few rows, and of many */
   int* status;
 } CozyCachePlan;
 

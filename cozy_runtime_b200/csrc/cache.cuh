@@ -89,12 +89,16 @@ __host__ __device__ __forceinline__ bool few_rows(int group, long long added) {
   return group <= kRowsFew && added <= kFewItems * (kRowsFew / group);
 }
 
-// Tiles before item `item` of a request with `cached` tokens before its new ones: item i's last
-// token sees cached + (i + 1) · tokens_of_item keys (the last item of a request fewer).
-__host__ __device__ __forceinline__ long long tiles_before(int group, long long cached,
+// Units before item `item` of a request with `cached` tokens before its new ones: the tiles of
+// keys of each item (item i's last token sees cached + (i + 1) · tokens_of_item keys, the last
+// item of a request fewer) and kItemUnits for its start and end.
+constexpr int kItemUnits = 2;
+
+__host__ __device__ __forceinline__ long long units_before(int group, long long cached,
                                                            long long item) {
   const int per = kRowsMany / group;
-  return floor_sum_128(static_cast<uint32_t>(item), per, cached + per + kTileKeys - 1);
+  return floor_sum_128(static_cast<uint32_t>(item), per, cached + per + kTileKeys - 1) +
+         kItemUnits * item;
 }
 
 // Units of one key/value head of a request: of few rows, or of many.
@@ -107,7 +111,8 @@ __host__ __device__ __forceinline__ long long attention_units(int group, long lo
   }
   const int per = kRowsMany / group;
   const long long items = quotient(added + per - 1, per);
-  return tiles_before(group, cached, items - 1) + (cached + added + kTileKeys - 1) / kTileKeys;
+  return units_before(group, cached, items - 1) + (cached + added + kTileKeys - 1) / kTileKeys +
+         kItemUnits;
 }
 
 }  // namespace cozy

@@ -38,6 +38,7 @@ struct CacheArgs {
   __nv_bfloat16* out;
   long long o_token, o_head;
   float* lse;
+  uint32_t per_group;  // ceil(2^16 / group): r · per_group >> 16 is r / group for rows r < 256
   float scale_log2;  // softmax scale · log2(e)
   float* ws_o;       // [worker][2][rows][HD]
   float2* ws_ml;     // [worker][2][rows]
@@ -684,15 +685,22 @@ __device__ __forceinline__ float group_mul(float mul, float key_scale) {
   return fmaxf(mul * key_scale, 7.52316385e-37f);
 }
 
+// A worker's part of an item. Its units are the item's kItemUnits, then its tiles of keys.
 struct ManyAt {
-  int n, h, item, j;  // request, head, item, tile of keys
-  int items, tiles;   // items of the request's head, tiles of this item
+  int n, h, item;    // request, head, item
+  int j, steps;      // first tile of keys, tiles
+  int items, tiles;  // items of the request's head, tiles of this item
   int keys, cached, added, first_token;
+  int left, units;  // units left to the worker from this part on; units of the part
 };
 
-__device__ __forceinline__ void many_item(const CacheArgs& a, ManyAt& at) {
+// The part of the item that begins at its unit `unit`; the run ends where a part has no tile.
+__device__ __forceinline__ void many_part(const CacheArgs& a, ManyAt& at, int unit) {
   const int per = kRowsMany / a.group;
   at.tiles = (at.cached + min((at.item + 1) * per, at.added) + kTileKeys - 1) / kTileKeys;
+  at.j = max(0, unit - kItemUnits);
+  at.units = min(at.left, kItemUnits + at.tiles - unit);
+  at.steps = unit + at.units - kItemUnits - at.j;
 }
 
 __device__ __forceinline__ void many_request(const CacheArgs& a, ManyAt& at, int n) {
@@ -705,28 +713,35 @@ __device__ __forceinline__ void many_request(const CacheArgs& a, ManyAt& at, int
   at.items = a.units_many[n + 1] == a.units_many[n] ? 0 : (at.added + per - 1) / per;
 }
 
-__device__ __forceinline__ ManyAt many_at(const CacheArgs& a, long long u) {
+__device__ __forceinline__ ManyAt many_at(const CacheArgs& a, long long u, int left) {
   ManyAt at;
+  at.left = left;
   many_request(a, at, request_of(a, a.units_many, u));
   const long long units = a.units_many[at.n + 1] - a.units_many[at.n];
   const long long within = u - a.units_many[at.n] * a.heads_kv;
   at.h = static_cast<int>(quotient(within, units));
   const long long rest = within - at.h * units;
-  int low = 0, high = at.items - 1;
-  while (low < high) {
-    const int mid = (low + high + 1) >> 1;
-    if (tiles_before(a.group, at.cached, mid) <= rest) low = mid;
-    else high = mid - 1;
+  const int lane = threadIdx.x & 31;
+  int low = 0, count = at.items;  // 32 places of the search range at once
+  while (count > 1) {
+    const int step = (count + 31) / 32;
+    const bool before = lane * step < count && units_before(a.group, at.cached, low + lane * step) <= rest;
+    const int used = (31 - __clz(__ballot_sync(0xffffffffu, before))) * step;
+    low += used;
+    count = min(step, count - used);
   }
   at.item = low;
-  at.j = static_cast<int>(rest - tiles_before(a.group, at.cached, low));
-  many_item(a, at);
+  many_part(a, at, static_cast<int>(rest - units_before(a.group, at.cached, low)));
   return at;
 }
 
-// To the first tile of the next item.
+// To the worker's part of the next item.
 __device__ __forceinline__ void many_next(const CacheArgs& a, ManyAt& at) {
-  at.j = 0;
+  at.left -= at.units;
+  if (at.left <= 0) {
+    at.steps = 0;
+    return;
+  }
   if (++at.item == at.items) {
     at.item = 0;
     if (++at.h == a.heads_kv) {
@@ -735,35 +750,34 @@ __device__ __forceinline__ void many_next(const CacheArgs& a, ManyAt& at) {
       while (at.items == 0);  // only reached while units remain
     }
   }
-  many_item(a, at);
+  many_part(a, at, 0);
 }
 
 // A warp's place in shared memory: what the loop over tiles does not need stands there, not in
 // registers (128 scores and 16 weights a thread leave few).
-__device__ __forceinline__ void many_put(volatile int* to, const ManyAt& at, int left) {
+__device__ __forceinline__ void many_put(volatile int* to, const ManyAt& at) {
   __syncwarp();
-  to[0] = at.n;
-  to[1] = at.h;
-  to[2] = at.item;
-  to[3] = at.j;
-  to[4] = at.items;
-  to[5] = at.tiles;
-  to[6] = at.keys;
-  to[7] = at.cached;
-  to[8] = at.added;
-  to[9] = at.first_token;
-  to[10] = left;
+  const int v[13] = {at.n, at.h, at.item, at.j, at.steps, at.items, at.tiles, at.keys, at.cached,
+                     at.added, at.first_token, at.left, at.units};
+#pragma unroll
+  for (int i = 0; i < 13; ++i) to[i] = v[i];
   __syncwarp();
 }
 
 __device__ __forceinline__ ManyAt many_get(const volatile int* from) {
-  return {from[0], from[1], from[2], from[3], from[4], from[5], from[6], from[7], from[8], from[9]};
+  return {from[0], from[1], from[2], from[3], from[4], from[5], from[6], from[7], from[8], from[9],
+          from[10], from[11], from[12]};
 }
 
-// Halves of tiles in `steps` tiles from the place on: the last tile of an item may need only one.
-__device__ __forceinline__ int many_halves(const CacheArgs& a, const ManyAt& at, int steps) {
+// Halves of the part's tiles: the last tile of an item may need only one.
+__device__ __forceinline__ int many_halves(const CacheArgs& a, const ManyAt& at) {
   const int keys = at.cached + min((at.item + 1) * (kRowsMany / a.group), at.added);
-  return min(2 * steps, (keys - at.j * kTileKeys + 63) / 64);
+  return min(2 * at.steps, (keys - at.j * kTileKeys + 63) / 64);
+}
+
+// The token of an item's row, and its head of the group.
+__device__ __forceinline__ int row_token(const CacheArgs& a, int row) {
+  return static_cast<int>(row * a.per_group >> 16);
 }
 
 __device__ __forceinline__ int many_rows(const CacheArgs& a, const ManyAt& at) {
@@ -818,6 +832,10 @@ __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
                "r"(v.w)
                : "memory");
+}
+
+__device__ __forceinline__ void sts64(uint32_t at, uint32_t lo, uint32_t hi) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(lo), "r"(hi) : "memory");
 }
 
 // Matrix descriptors (the layout that sm100.cuh states), kept as their low words: the start
@@ -907,6 +925,7 @@ __global__ void __launch_bounds__(512, 1)
   const int workers = static_cast<int>(min(static_cast<long long>(a.workers), total));
   if (static_cast<int>(blockIdx.x) >= workers) return;
   const long long u0 = quotient(blockIdx.x * total, workers), u1 = quotient((blockIdx.x + 1) * total, workers);
+  const int units = static_cast<int>(u1 - u0);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -957,75 +976,75 @@ __global__ void __launch_bounds__(512, 1)
     uint32_t phase = 0;  // bit b: parity of half b's next scores (its last product has the other)
     bool ok = true;
     volatile int* place = reinterpret_cast<volatile int*>(smem + L::kAtOffset) + warp * 16;
-    many_put(place, many_at(a, u0), static_cast<int>(u1 - u0));
-    while (ok) {
+    many_put(place, many_at(a, u0, units));
+    while (ok && place[4] > 0) {
       int steps, halves, last, first_seen, key0;
       bool here;
       float mul = 0.f;
       {
         const ManyAt at = many_get(place);
-        steps = min(static_cast<int>(place[10]), at.tiles - at.j);
-        halves = many_halves(a, at, steps);
+        steps = at.steps;
+        halves = many_halves(a, at);
         key0 = at.j * kTileKeys;
         const int rows = many_rows(a, at);
         here = s * 128 < rows;
         const int per = kRowsMany / a.group;
         const int row = min(s * 128 + row128, rows - 1);
-        const int token = at.item * per + row / a.group;  // of the request
+        const int token = at.item * per + row_token(a, row);  // of the request
         last = at.cached + token;                         // the last key it sees
         first_seen = at.cached + at.item * per;           // the item's first token's last key
-        if (here) {  // ---- this row of Q as two e4m3 parts (rows behind the last repeat it)
-          const __nv_bfloat16* from = a.query + (at.first_token + token) * a.q_token +
-                                      (at.h * a.group + row % a.group) * a.q_head;
-          float amax = 0.f;
-#pragma unroll
-          for (int c = 0; c < HD / 8; ++c) {
-            const uint4 x = __ldg(reinterpret_cast<const uint4*>(from + c * 8));
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              amax = fmaxf(amax, fabsf(__uint_as_float(w[e] << 16)));
-              amax = fmaxf(amax, fabsf(__uint_as_float(w[e] & 0xffff0000u)));
-            }
-          }
-          // the largest value in [224, 448]: 448 = 1.75 · 2^8
-          const int e = max(-100, static_cast<int>((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8);
-          const float up = exponent_scale(-e);
-          mul = a.scale_log2 * exponent_scale(e);
+        if (here) {
+          // ---- this warp's 32 rows of Q as two e4m3 parts, HD / 8 lanes a row (rows behind the
+          // last repeat it)
+          constexpr int LANES = HD / 8, ROWS = 32 / LANES;
+          const int sub = lane / LANES, d0 = lane % LANES * 8;
           const uint32_t hi_at = smem_u32(smem + L::kQOffset + s * 2 * L::kCodeTile);
-          const uint32_t lo_at = hi_at + L::kCodeTile;
-#pragma unroll 2
-          for (int c = 0; c < HD / 16; ++c) {  // read again (from L1) rather than held
-            uint32_t hi[4], lo[4];
-            const uint4 x[2] = {__ldg(reinterpret_cast<const uint4*>(from + c * 16)),
-                                __ldg(reinterpret_cast<const uint4*>(from + c * 16 + 8))};
+          uint4 x[LANES];  // every load before the first use
+#pragma unroll
+          for (int i = 0; i < LANES; ++i) {
+            const int r = min(s * 128 + (warp & 3) * 32 + i * ROWS + sub, rows - 1);
+            const int of = row_token(a, r);
+            x[i] = *reinterpret_cast<const uint4*>(
+                a.query + (at.first_token + at.item * per + of) * a.q_token +
+                (at.h * a.group + r - of * a.group) * a.q_head + d0);
+          }
+#pragma unroll
+          for (int i = 0; i < LANES; ++i) {
+            const int r128 = (warp & 3) * 32 + i * ROWS + sub;
+            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            float amax = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              amax = max3(amax, fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u)));
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            // the largest value in [224, 448]: 448 = 1.75 · 2^8
+            const int e = max(-100, static_cast<int>((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8);
+            const float up = exponent_scale(-e);
+            const float mine = a.scale_log2 * exponent_scale(e);
+            const float given = __shfl_sync(0xffffffffu, mine, lane % ROWS * LANES);
+            if (lane / ROWS == i) mul = given;
+            uint32_t hi[2], lo[2];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint4 v = x[k >> 1];
-              const uint32_t w[2] = {(k & 1) ? v.z : v.x, (k & 1) ? v.w : v.y};
-              uint32_t parts[2][2];
-#pragma unroll
-              for (int b = 0; b < 2; ++b) {
-                float f0 = __uint_as_float(w[b] << 16) * up, f1 = __uint_as_float(w[b] & 0xffff0000u) * up;
-                // an infinity has no parts: its row is NaN, as its softmax is
-                if (!(fabsf(f0) <= 448.f)) f0 = __uint_as_float(0x7fc00000u);
-                if (!(fabsf(f1) <= 448.f)) f1 = __uint_as_float(0x7fc00000u);
-                uint16_t h, l;
-                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h) : "f"(f0), "f"(f1));
-                uint32_t back;
-                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
-                const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&back));
-                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(l) : "f"(f0 - g.x), "f"(f1 - g.y));
-                parts[0][b] = h;
-                parts[1][b] = l;
-              }
-              hi[k] = parts[0][0] | parts[0][1] << 16;
-              lo[k] = parts[1][0] | parts[1][1] << 16;
+              float f0 = __uint_as_float(w[k] << 16) * up, f1 = __uint_as_float(w[k] & 0xffff0000u) * up;
+              // an infinity has no parts: its row is NaN, as its softmax is
+              if (!(fabsf(f0) <= 448.f)) f0 = __uint_as_float(0x7fc00000u);
+              if (!(fabsf(f1) <= 448.f)) f1 = __uint_as_float(0x7fc00000u);
+              uint16_t h, l;
+              asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h) : "f"(f0), "f"(f1));
+              uint32_t back;
+              asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
+              const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&back));
+              asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(l) : "f"(f0 - g.x), "f"(f1 - g.y));
+              hi[k >> 1] = (k & 1) ? hi[k >> 1] | static_cast<uint32_t>(h) << 16 : h;
+              lo[k >> 1] = (k & 1) ? lo[k >> 1] | static_cast<uint32_t>(l) << 16 : l;
             }
-            const uint32_t off = HD == 128 ? row128 * 128 + ((c ^ (row128 & 7)) << 4)
-                                           : row128 * 64 + ((c ^ ((row128 >> 1) & 3)) << 4);
-            sts128(hi_at + off, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-            sts128(lo_at + off, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+            const int c = d0 / 16;
+            const uint32_t off = (HD == 128 ? r128 * 128 + ((c ^ (r128 & 7)) << 4)
+                                            : r128 * 64 + ((c ^ ((r128 >> 1) & 3)) << 4)) + d0 % 16;
+            sts64(hi_at + off, hi[0], hi[1]);
+            sts64(hi_at + L::kCodeTile + off, lo[0], lo[1]);
           }
           *poison = make_uint4(0, 0, 0, 0);
           fence_async_smem();
@@ -1146,12 +1165,14 @@ __global__ void __launch_bounds__(512, 1)
         // ---- the item's end, or this worker's part of it
         const ManyAt at = many_get(place);
         const int rows = many_rows(a, at), row = s * 128 + row128;
-        const int token = at.item * (kRowsMany / a.group) + row / a.group;
+        const int first_token = at.first_token + at.item * (kRowsMany / a.group);
+        const int token = first_token + row_token(a, row);
         const bool whole = steps == at.tiles;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const long long part = 2LL * blockIdx.x + (at.j == 0 ? 1 : 0);
-        const int head = at.h * a.group + row % a.group;
-        __nv_bfloat16* to = a.out + (at.first_token + token) * a.o_token + head * a.o_head;
+        const int head = at.h * a.group + row - (token - first_token) * a.group;
+        // whole rows leave through the tile's Q (free now, and of the same size), HD / 8 lanes a row
+        const uint32_t stage = smem_u32(smem + L::kQOffset + s * 2 * L::kCodeTile) + (warp & 3) * 32 * HD * 2;
         float4* ws = reinterpret_cast<float4*>(a.ws_o) + part * (HD / 4) * kRowsMany + row;
         const uint4 p = *poison;
         const bool nan = (p.x | p.y | p.z | p.w) != 0;
@@ -1167,41 +1188,53 @@ __global__ void __launch_bounds__(512, 1)
             for (int i = 0; i < 32; ++i)
               if (bits >> i & 1) o[i] = 0x7fc00000u;
           }
-          if (row < rows) {
-            if (whole) {
+          if (whole) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint32_t w[4];
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  w[k] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * k]) * inv,
-                                     __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-                *reinterpret_cast<uint4*>(to + c * 32 + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                ws[(c * 8 + i) * kRowsMany] =
-                    make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+              for (int k = 0; k < 4; ++k)
+                w[k] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * k]) * inv,
+                                   __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+              // chunk j of row r at j ^ (r mod 8): no two lanes of eight in a bank
+              sts128(stage + lane * HD * 2 + (((c * 4 + i) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
             }
+          } else if (row < rows) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              ws[(c * 8 + i) * kRowsMany] =
+                  make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                              __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
           }
         }
         tc_fence_before();
+        if (whole) {
+          constexpr int LANES = HD / 8, ROWS = 32 / LANES;
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < LANES; ++i) {
+            const int r32 = i * ROWS + lane / LANES, j = lane % LANES;
+            const int r = s * 128 + (warp & 3) * 32 + r32;
+            const uint4 v = lds128(stage + r32 * HD * 2 + ((j ^ (r32 & 7)) << 4));
+            const int of = row_token(a, r);
+            if (r < rows)
+              *reinterpret_cast<uint4*>(a.out + (first_token + of) * a.o_token +
+                                        (at.h * a.group + r - of * a.group) * a.o_head + j * 8) = v;
+          }
+          __syncwarp();
+        }
         if (row < rows) {
           if (!whole) a.ws_ml[part * kRowsMany + row] = make_float2(m, l);
           else if (a.lse != nullptr)
-            a.lse[static_cast<long long>(at.first_token + token) * a.heads_kv * a.group + head] =
+            a.lse[static_cast<long long>(token) * a.heads_kv * a.group + head] =
                 l == 0.f ? -INFINITY : 0.6931471805599453f * (m - kManyBias + __log2f(l));
         }
       } else {
         block += steps;
       }
-      const int left = place[10] - steps;
-      if (left <= 0) break;
       ManyAt at = many_get(place);
       many_next(a, at);
-      many_put(place, at, left);
+      many_put(place, at);
     }
   } else if (warp == 8) {
     // -------------------------------------------------------------- page numbers and copies
@@ -1209,9 +1242,8 @@ __global__ void __launch_bounds__(512, 1)
     const int box = min(a.page, kTileKeys), per_tile = kTileKeys / box;
     int block = 0;
     bool ok = true;
-    ManyAt at = many_at(a, u0);
-    for (long long u = u0; u < u1 && ok;) {
-      const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.tiles - at.j)));
+    for (ManyAt at = many_at(a, u0, units); at.steps > 0; many_next(a, at)) {
+      const int steps = at.steps;
       int batch = 0, id = -1;
       float key_scale = 1.f, value_e = 0.f;
       for (int step = 0; step < steps; ++step, ++block) {
@@ -1279,8 +1311,7 @@ __global__ void __launch_bounds__(512, 1)
           tma_load_2d(smem + L::kV8Offset + v_stage * L::kCodeTile + lane * box * HD, &tm_v,
                       &v8_full[v_stage], 0, y);
       }
-      u += steps;
-      if (ok && u < u1) many_next(a, at);
+      if (!ok) break;
     }
     // every copy lands before the CTA unwinds
     volatile int never = 0;
@@ -1326,10 +1357,9 @@ __global__ void __launch_bounds__(512, 1)
     int block = 0;
     uint32_t q_phase = 0, p_phase = 0;  // parities of q_ready, and of p_ready by half
     bool ok = true;
-    ManyAt at = many_at(a, u0);
-    for (long long u = u0; u < u1 && ok;) {
-      const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.tiles - at.j)));
-      const int halves = many_halves(a, at, steps);
+    for (ManyAt at = many_at(a, u0, units); at.steps > 0; many_next(a, at)) {
+      const int steps = at.steps;
+      const int halves = many_halves(a, at);
       const bool here = s * 128 < many_rows(a, at);
       if (here) {
         ok = many_warp_wait(&q_ready[s], q_phase, abort, a.status);
@@ -1368,8 +1398,7 @@ __global__ void __launch_bounds__(512, 1)
         __syncwarp();
       }
       block += steps;
-      u += steps;
-      if (ok && u < u1) many_next(a, at);
+      if (!ok) break;
     }
     // every product completes before tensor memory is given back
     if (elect_one()) mma_commit(drain);
@@ -1386,9 +1415,8 @@ __global__ void __launch_bounds__(512, 1)
     const int tid = threadIdx.x - 384;
     int block = 0;
     bool ok = true;
-    ManyAt at = many_at(a, u0);
-    for (long long u = u0; u < u1 && ok;) {
-      const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.tiles - at.j)));
+    for (ManyAt at = many_at(a, u0, units); at.steps > 0; many_next(a, at)) {
+      const int steps = at.steps;
       const int first_seen = at.cached + at.item * (kRowsMany / a.group);
       for (int step = 0; step < steps; ++step, ++block) {
         const int in = block % L::kV8Stages, slot = block % L::kV16Stages;
@@ -1443,8 +1471,7 @@ __global__ void __launch_bounds__(512, 1)
           break;
         mbar_arrive(&v16_full[slot]);
       }
-      u += steps;
-      if (ok && u < u1) many_next(a, at);
+      if (!ok) break;
     }
   }
 
@@ -1469,11 +1496,13 @@ __global__ void __launch_bounds__(256) join_many(const CacheArgs a) {
   int last = 0, rows = 0;
   if (split) {
     const long long u = quotient(w * total, workers);
-    at = many_at(a, u);
-    const long long u0 = u - at.j;
+    at = many_at(a, u, 1 << 30);
+    // cut behind its first tile, and the worker before has that one
+    const long long u0 = u - kItemUnits - at.j;
     rows = many_rows(a, at);
-    split = at.j > 0 && quotient((w - 1) * total, workers) <= u0 && static_cast<int>(blockIdx.y) * 32 < rows;
-    last = static_cast<int>(quotient((u0 + at.tiles) * workers - 1, total));
+    split = at.j > 0 && quotient((w - 1) * total, workers) <= u0 + kItemUnits &&
+            static_cast<int>(blockIdx.y) * 32 < rows;
+    last = static_cast<int>(quotient((u0 + kItemUnits + at.tiles) * workers - 1, total));
   }
   if (split || (blockIdx.x == 0 && blockIdx.y == 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!split) return;
@@ -1668,6 +1697,7 @@ int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyC
   a.pages = p.pages;
   a.page = p.page;
   a.group = p.group;
+  a.per_group = (65536u + p.group - 1) / p.group;
   a.heads_kv = c.heads_kv;
   a.key_exponent = static_cast<const int8_t*>(c.key_exponent);
   a.value_exponent = static_cast<const int8_t*>(c.value_exponent);

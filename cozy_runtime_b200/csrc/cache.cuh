@@ -92,7 +92,7 @@ __host__ __device__ __forceinline__ bool few_rows(int group, long long added) {
 // Units before item `item` of a request with `cached` tokens before its new ones: the tiles of
 // keys of each item (item i's last token sees cached + (i + 1) · tokens_of_item keys, the last
 // item of a request fewer) and kItemUnits for its start and end.
-constexpr int kItemUnits = 2;
+constexpr int kItemUnits = 3;
 
 __host__ __device__ __forceinline__ long long units_before(int group, long long cached,
                                                            long long item) {

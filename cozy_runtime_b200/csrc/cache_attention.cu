@@ -999,52 +999,70 @@ __global__ void __launch_bounds__(512, 1)
           constexpr int LANES = HD / 8, ROWS = 32 / LANES;
           const int sub = lane / LANES, d0 = lane % LANES * 8;
           const uint32_t hi_at = smem_u32(smem + L::kQOffset + s * 2 * L::kCodeTile);
-          uint4 x[LANES];  // every load before the first use
+          // Four rows' loads and exchanges side by side, the next four's loads ahead. A loop, not
+          // straight code: run once an item, that would come from memory instruction by instruction.
+          auto load = [&](int g, uint4 (&v)[4]) {
 #pragma unroll
-          for (int i = 0; i < LANES; ++i) {
-            const int r = min(s * 128 + (warp & 3) * 32 + i * ROWS + sub, rows - 1);
-            const int of = row_token(a, r);
-            x[i] = *reinterpret_cast<const uint4*>(
-                a.query + (at.first_token + at.item * per + of) * a.q_token +
-                (at.h * a.group + r - of * a.group) * a.q_head + d0);
-          }
-#pragma unroll
-          for (int i = 0; i < LANES; ++i) {
-            const int r128 = (warp & 3) * 32 + i * ROWS + sub;
-            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            float amax = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              amax = max3(amax, fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u)));
-#pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            // the largest value in [224, 448]: 448 = 1.75 · 2^8
-            const int e = max(-100, static_cast<int>((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8);
-            const float up = exponent_scale(-e);
-            const float mine = a.scale_log2 * exponent_scale(e);
-            const float given = __shfl_sync(0xffffffffu, mine, lane % ROWS * LANES);
-            if (lane / ROWS == i) mul = given;
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              float f0 = __uint_as_float(w[k] << 16) * up, f1 = __uint_as_float(w[k] & 0xffff0000u) * up;
-              // an infinity has no parts: its row is NaN, as its softmax is
-              if (!(fabsf(f0) <= 448.f)) f0 = __uint_as_float(0x7fc00000u);
-              if (!(fabsf(f1) <= 448.f)) f1 = __uint_as_float(0x7fc00000u);
-              uint16_t h, l;
-              asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h) : "f"(f0), "f"(f1));
-              uint32_t back;
-              asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
-              const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&back));
-              asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(l) : "f"(f0 - g.x), "f"(f1 - g.y));
-              hi[k >> 1] = (k & 1) ? hi[k >> 1] | static_cast<uint32_t>(h) << 16 : h;
-              lo[k >> 1] = (k & 1) ? lo[k >> 1] | static_cast<uint32_t>(l) << 16 : l;
+            for (int i = 0; i < 4; ++i) {
+              const int r = min(s * 128 + (warp & 3) * 32 + (g * 4 + i) * ROWS + sub, rows - 1);
+              const int of = row_token(a, r);
+              v[i] = *reinterpret_cast<const uint4*>(
+                  a.query + (at.first_token + at.item * per + of) * a.q_token +
+                  (at.h * a.group + r - of * a.group) * a.q_head + d0);
             }
-            const int c = d0 / 16;
-            const uint32_t off = (HD == 128 ? r128 * 128 + ((c ^ (r128 & 7)) << 4)
-                                            : r128 * 64 + ((c ^ ((r128 >> 1) & 3)) << 4)) + d0 % 16;
-            sts64(hi_at + off, hi[0], hi[1]);
-            sts64(hi_at + L::kCodeTile + off, lo[0], lo[1]);
+          };
+          uint4 x[4];
+          load(0, x);
+#pragma unroll 1
+          for (int g = 0; g < LANES / 4; ++g) {
+            uint4 y[4];
+            load(min(g + 1, LANES / 4 - 1), y);
+            float amax[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+              amax[i] = 0.f;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                amax[i] = max3(amax[i], fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u)));
+            }
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r128 = (warp & 3) * 32 + (g * 4 + i) * ROWS + sub;
+              const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+              // the largest value in [224, 448]: 448 = 1.75 · 2^8
+              const int e = max(-100, static_cast<int>((__float_as_uint(amax[i]) + 0x1fffffu) >> 23) - 127 - 8);
+              const float up = exponent_scale(-e);
+              const float mine = a.scale_log2 * exponent_scale(e);
+              const float given = __shfl_sync(0xffffffffu, mine, lane % ROWS * LANES);
+              if (lane / ROWS == g * 4 + i) mul = given;
+              uint32_t hi[2], lo[2];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                float f0 = __uint_as_float(w[k] << 16) * up, f1 = __uint_as_float(w[k] & 0xffff0000u) * up;
+                // an infinity has no parts: its row is NaN, as its softmax is
+                if (!(fabsf(f0) <= 448.f)) f0 = __uint_as_float(0x7fc00000u);
+                if (!(fabsf(f1) <= 448.f)) f1 = __uint_as_float(0x7fc00000u);
+                uint16_t h, l;
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(h) : "f"(f0), "f"(f1));
+                uint32_t back;
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
+                const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&back));
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(l) : "f"(f0 - g.x), "f"(f1 - g.y));
+                hi[k >> 1] = (k & 1) ? hi[k >> 1] | static_cast<uint32_t>(h) << 16 : h;
+                lo[k >> 1] = (k & 1) ? lo[k >> 1] | static_cast<uint32_t>(l) << 16 : l;
+              }
+              const int c = d0 / 16;
+              const uint32_t off = (HD == 128 ? r128 * 128 + ((c ^ (r128 & 7)) << 4)
+                                              : r128 * 64 + ((c ^ ((r128 >> 1) & 3)) << 4)) + d0 % 16;
+              sts64(hi_at + off, hi[0], hi[1]);
+              sts64(hi_at + L::kCodeTile + off, lo[0], lo[1]);
+              x[i] = y[i];
+            }
           }
           *poison = make_uint4(0, 0, 0, 0);
           fence_async_smem();

@@ -13,6 +13,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "../../include/cozy_ulysses.h"
 #include "cache.cuh"
 #include "sm100.cuh"
@@ -30,7 +32,7 @@ struct CacheArgs {
   const long long* units_few;   // [requests + 1] units of one head before each request
   const long long* units_many;  // (a request has units of one kind only)
   int* status;
-  int requests, pages, page, group, heads_kv;
+  int requests, pages, page, page_shift, group, heads_kv;
   const int8_t* key_exponent;
   const int8_t* value_exponent;
   const __nv_bfloat16* query;
@@ -222,59 +224,73 @@ __global__ void __launch_bounds__(256, 1)
   __syncwarp();
 
   // ---- the loads: fill f is the keys (even) or values (odd) of unit u0 + f / 2
-  const int box = min(a.page, kChunkKeys), per_chunk = kChunkKeys / box;
-  const long long fills = 2 * (u1 - u0);
+  const int box_shift = min(a.page_shift, 6), box = 1 << box_shift, per_chunk = kChunkKeys >> box_shift;
+  const unsigned units = static_cast<unsigned>(u1 - u0), fills = 2 * units;
   FewAt to = few_at(a, u0);  // the chunk to load next
   FewAt at = to;             // the chunk to compute
-  int batch = 0, id = -1, ids = 0;      // a lane's page number among 32 of the item's
-  float key_scale = 1.f, value_e = 0.f;
-  bool fresh = true;
-  auto load = [&](long long f) {
+  int batch = 0, id = -1, ids = 0;  // a lane's page number among 32 of the item's, of the chunk's
+  int key_e = 0, value_e = 0;       // its page's exponents
+  bool fresh_pages = true, fresh_scales = true;
+  auto load = [&](unsigned f) {
     if (f >= fills) return;
-    const int slot = static_cast<int>(f % L::kSlots);
-    const int first = a.page > kChunkKeys ? to.j * kChunkKeys / a.page : to.j * per_chunk;
-    const int offset = a.page > kChunkKeys ? to.j * kChunkKeys % a.page : 0;
-    const int count = min(per_chunk, (to.keys - to.j * kChunkKeys + box - 1) / box);
-    if ((f & 1) == 0) {
-      if (fresh || first + per_chunk > batch + 32) {
-        fresh = false;
+    const unsigned slot = f % L::kSlots;
+    const int first = to.j * kChunkKeys >> a.page_shift;
+    const int offset = to.j * kChunkKeys & (a.page - 1);
+    const int count = min(per_chunk, (to.keys - to.j * kChunkKeys + box - 1) >> box_shift);
+    const bool keys = (f & 1) == 0;
+    if (keys) {
+      const bool other = first < batch || first + per_chunk > batch + 32;
+      if (fresh_pages || other) {
         batch = first;
         id = -1;
-        key_scale = 1.f;
-        value_e = 0.f;
         const int index = first + lane;
         if (index * static_cast<long long>(a.page) < to.keys) {
           id = a.table[to.n * a.table_stride + index];
           if (id < 0 || id >= a.pages) {
             id = -1;
             atomicOr(a.status, kPlanBadPage);
-          } else {
-            const long long block = static_cast<long long>(id) * a.heads_kv + to.h;
-            key_scale = exponent_scale(a.key_exponent[block]);
-            value_e = static_cast<float>(a.value_exponent[block]);
           }
         }
       }
-      // the chunk's scales; a page that is not there has a scale of zero
-      const int from = first - batch + (lane & 3);
-      const float ks = __shfl_sync(0xffffffffu, key_scale, from & 31);
-      const float ve = __shfl_sync(0xffffffffu, value_e, from & 31);
-      ids = __shfl_sync(0xffffffffu, id, from & 31);
+      ids = __shfl_sync(0xffffffffu, id, (first - batch + (lane & 3)) & 31);
       if (lane >= count) ids = -1;
-      if (lane < per_chunk)
-        meta[(f >> 1) % L::kMeta * 4 + lane] = make_float2(ids < 0 ? 0.f : ks, ve);
+      fresh_scales |= fresh_pages || other;
+      fresh_pages = false;
     }
     const unsigned there = __ballot_sync(0xffffffffu, lane < per_chunk && ids >= 0);
     if (lane == 0) mbar_expect_tx(&full[slot], __popc(there) * box * HD);
     __syncwarp();
     if (lane < per_chunk && ids >= 0)
-      tma_load_2d(ring + slot * L::kSlotBytes + lane * box * HD, (f & 1) ? &tm_v : &tm_k,
-                  &full[slot], 0, (ids * a.heads_kv + to.h) * a.page + offset);
-    if (f & 1) {
-      if (f + 1 < fills) fresh |= few_next(a, to);
+      tma_load_2d(ring + slot * L::kSlotBytes + lane * box * HD, keys ? &tm_k : &tm_v, &full[slot],
+                  0, (ids * a.heads_kv + to.h) * a.page + offset);
+    if (keys) {
+      if (fresh_scales) {  // asked for here, looked at when the chunk's values are loaded
+        fresh_scales = false;
+        key_e = value_e = 0;
+        if (id >= 0) {
+          const long long block = static_cast<long long>(id) * a.heads_kv + to.h;
+          key_e = a.key_exponent[block];
+          value_e = a.value_exponent[block];
+        }
+      }
+    } else {
+      // the chunk's scales; a page that is not there has a scale of zero
+      const int from = (first - batch + (lane & 3)) & 31;
+      const int ke = __shfl_sync(0xffffffffu, key_e, from), ve = __shfl_sync(0xffffffffu, value_e, from);
+      if (lane < per_chunk)
+        meta[(f >> 1) % L::kMeta * 4 + lane] =
+            make_float2(ids < 0 ? 0.f : exponent_scale(ke), static_cast<float>(ve));
+      __syncwarp();
+      if (f + 1 < fills) {
+        const int was = to.n;
+        if (few_next(a, to)) {
+          fresh_scales = true;
+          fresh_pages = to.n != was;  // a request's heads share its pages
+        }
+      }
     }
   };
-  for (int f = 0; f < L::kSlots; ++f) load(f);
+  for (unsigned f = 0; f < L::kSlots; ++f) load(f);
 
   const int order = (g & 1) ? ((g + 4) & 7) : g;  // row of this lane's column of K
   const uint32_t base = smem_u32(ring);
@@ -293,8 +309,8 @@ __global__ void __launch_bounds__(256, 1)
   }
 
   bool ok = true;
-  long long u = u0;
-  while (u < u1 && ok) {
+  unsigned u = 0;
+  while (u < units && ok) {
     // ---- an item, or the part of it that this worker has
     const int per = kRowsFew / a.group;
     const int first_token = a.starts[at.n] + at.item * per;
@@ -302,7 +318,7 @@ __global__ void __launch_bounds__(256, 1)
     const int rows = min(left, per) * a.group;
     const int seen0 = at.keys - left;  // keys before the item's own
     const int j0 = at.j;
-    const int steps = static_cast<int>(min(u1 - u, static_cast<long long>(at.chunks - at.j)));
+    const int steps = static_cast<int>(min(units - u, static_cast<unsigned>(at.chunks - at.j)));
     // rows g and g + 8: query times a power of two that puts its largest value in [2^14, 2^15)
     uint32_t q[KSTEPS][4];
     float mul[2];
@@ -356,8 +372,8 @@ __global__ void __launch_bounds__(256, 1)
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     for (int step = 0; step < steps; ++step, ++u) {
-      const long long f = 2 * (u - u0);
-      int slot = static_cast<int>(f % L::kSlots);
+      const unsigned f = 2 * u;
+      unsigned slot = f % L::kSlots;
       if (!(ok = __all_sync(0xffffffffu, cache_wait(&full[slot], (f / L::kSlots) & 1, a.status)))) break;
       const float2* scales = meta + (f >> 1) % L::kMeta * 4;
       const int key0 = (j0 + step) * kChunkKeys;
@@ -445,7 +461,7 @@ __global__ void __launch_bounds__(256, 1)
         p[nt / 2][(nt & 1) * 2 + 1] = f16_pair(p2, p3);
       }
       // ---- values
-      slot = static_cast<int>((f + 1) % L::kSlots);
+      slot = (f + 1) % L::kSlots;
       if (!(ok = __all_sync(0xffffffffu, cache_wait(&full[slot], ((f + 1) / L::kSlots) & 1, a.status)))) break;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
@@ -552,70 +568,105 @@ __global__ void __launch_bounds__(256, 1)
       }
     }
     at.j += steps - 1;
-    if (u < u1) few_next(a, at);
+    if (u < units) few_next(a, at);
   }
   if (!ok) {  // copies in flight land before the warp leaves
-    const long long f = 2 * (u - u0);
-    for (long long i = f; i < f + 2 * L::kSlots && i < fills; ++i)
+    const unsigned f = 2 * u;
+    for (unsigned i = f; i < f + 2 * L::kSlots && i < fills; ++i)
       cache_wait_slow(&full[i % L::kSlots], (i / L::kSlots) & 1, a.status);
   }
 }
 
-// Joins the parts of an item that several workers had: block (item, row), 8 warps over the
-// parts, in a fixed order.
+// Joins the parts of an item that several workers had: block (item, row). The parts' references
+// and sums are read at once, a thread a part; then 8 warps add the parts up, in a fixed order.
+constexpr int kMostParts = 2048;  // workers: 8 warps an SM
+
 template <int HD>
 __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
   constexpr int PER = HD / 32;  // channels a lane
+  __shared__ float weight[kMostParts];
   __shared__ float sum_o[8][HD];
-  __shared__ float2 sum_ml[8];
+  __shared__ float warp_top[8], warp_sum[8];
   const int n = blockIdx.x / a.heads_kv, h = blockIdx.x % a.heads_kv;
   const int per = kRowsFew / a.group, item = blockIdx.y / (per * a.group), row = blockIdx.y % (per * a.group);
-  const int first_token = a.starts[n] + item * per;
-  const int rows = a.units_few[n + 1] == a.units_few[n] ? 0 : (a.starts[n + 1] - first_token) * a.group;
-  const int items = (a.starts[n + 1] - a.starts[n] + per - 1) / per;
-  const long long chunks = (a.lengths[n] + kChunkKeys - 1) / kChunkKeys;
-  const long long total = a.units_few[a.requests] * a.heads_kv;
+  const int start = a.starts[n], next = a.starts[n + 1], length = a.lengths[n];
+  const long long before = a.units_few[n], behind = a.units_few[n + 1], all = a.units_few[a.requests];
+  const int first_token = start + item * per;
+  const int rows = behind == before ? 0 : (next - first_token) * a.group;
+  const int items = (next - start + per - 1) / per;
+  const long long chunks = (length + kChunkKeys - 1) / kChunkKeys;
+  const long long total = all * a.heads_kv;
   const long long workers = min(static_cast<long long>(a.workers), total);
-  const long long u0 = a.units_few[n] * a.heads_kv + (static_cast<long long>(h) * items + item) * chunks;
+  const long long u0 = before * a.heads_kv + (static_cast<long long>(h) * items + item) * chunks;
   const int first = total == 0 ? 0 : static_cast<int>(quotient((u0 + 1) * workers - 1, total));
   const int last = total == 0 ? 0 : static_cast<int>(quotient((u0 + chunks) * workers - 1, total));
   const bool split = row < rows && first != last;
   // one block at least waits, so that this grid does not end before the one it follows
   if (split || (blockIdx.x == 0 && blockIdx.y == 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!split) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float o[PER], m = -INFINITY, l = 0.f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = last - first + 1;
+  auto place = [&](int p) { return (2LL * (first + p) + (p == 0 ? 1 : 0)) * kRowsFew + row; };
+  // the loads of the parts' rows do not wait for their weights
+  constexpr int AHEAD = 4;
+  float x[AHEAD][PER] = {};
 #pragma unroll
-  for (int i = 0; i < PER; ++i) o[i] = 0.f;
-#pragma unroll 4
-  for (int w = first + warp; w <= last; w += 8) {
-    const long long part = (2LL * w + (w == first ? 1 : 0)) * kRowsFew + row;
-    const float2 ml = __ldcg(&a.ws_ml[part]);
-    float x[PER];
+  for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = __ldcg(&a.ws_o[part * HD + i * 32 + lane]);
-    const float top = fmaxf(m, ml.x);
-    const float mine = m == -INFINITY ? 0.f : ex2_approx(m - top);
-    const float other = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
-    m = top;
+    for (int c = 0; c < PER; ++c)
+      if (warp + 8 * i < parts) x[i][c] = __ldcg(&a.ws_o[place(warp + 8 * i) * HD + c * 32 + lane]);
+  float top = -INFINITY;
+  for (int p = threadIdx.x; p < parts; p += 256) top = fmaxf(top, __ldcg(&a.ws_ml[place(p)]).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) warp_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, warp_top[i]);
+  float sum = 0.f;
+  for (int p = threadIdx.x; p < parts; p += 256) {
+    const float2 ml = __ldcg(&a.ws_ml[place(p)]);
     // a part without a key has zeros; one whose scores are NaN has a sum of NaN
-    l = l * mine + ml.y * (ml.x == -INFINITY ? 1.f : other);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = o[i] * mine + x[i] * (ml.x == -INFINITY ? 1.f : other);
+    const float w = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - top);
+    weight[p] = w;
+    sum += ml.y * w;
   }
-  if (lane == 0) sum_ml[warp] = make_float2(m, l);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) sum_o[warp][i * 32 + lane] = o[i];
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) warp_sum[warp] = sum;
+  __syncthreads();
+  float o[PER];
+#pragma unroll
+  for (int c = 0; c < PER; ++c) o[c] = 0.f;
+  for (int p = warp; p < parts; p += 8 * AHEAD) {
+    float y[AHEAD][PER] = {};  // the next ones, meanwhile
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+      for (int c = 0; c < PER; ++c)
+        if (p + 8 * (AHEAD + i) < parts)
+          y[i][c] = __ldcg(&a.ws_o[place(p + 8 * (AHEAD + i)) * HD + c * 32 + lane]);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (p + 8 * i < parts) {
+        const float w = weight[p + 8 * i];
+#pragma unroll
+        for (int c = 0; c < PER; ++c) o[c] = fmaf(x[i][c], w, o[c]);
+      }
+#pragma unroll
+      for (int c = 0; c < PER; ++c) x[i][c] = y[i][c];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < PER; ++c) sum_o[warp][c * 32 + lane] = o[c];
   __syncthreads();
   const int d = threadIdx.x;
   if (d >= HD) return;
-  float top = -INFINITY;
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, sum_ml[w].x);
-  float value = 0.f, sum = 0.f;
+  float value = 0.f;
+  sum = 0.f;
+#pragma unroll
   for (int w = 0; w < 8; ++w) {
-    const float mine = sum_ml[w].x == -INFINITY ? 1.f : ex2_approx(sum_ml[w].x - top);
-    value += sum_o[w][d] * mine;
-    sum += sum_ml[w].y * mine;
+    value += sum_o[w][d];
+    sum += warp_sum[w];
   }
   const int token = first_token + row / a.group, head = h * a.group + row % a.group;
   a.out[token * a.o_token + head * a.o_head + d] = __float2bfloat16(sum == 0.f ? 0.f : value / sum);
@@ -1257,7 +1308,7 @@ __global__ void __launch_bounds__(512, 1)
   } else if (warp == 8) {
     // -------------------------------------------------------------- page numbers and copies
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyOtherRegs));
-    const int box = min(a.page, kTileKeys), per_tile = kTileKeys / box;
+    const int box = a.page, per_tile = kTileKeys >> a.page_shift;
     int block = 0;
     bool ok = true;
     for (ManyAt at = many_at(a, u0, units); at.steps > 0; many_next(a, at)) {
@@ -1266,7 +1317,7 @@ __global__ void __launch_bounds__(512, 1)
       float key_scale = 1.f, value_e = 0.f;
       for (int step = 0; step < steps; ++step, ++block) {
         const int key0 = (at.j + step) * kTileKeys;
-        const int first = key0 / a.page;
+        const int first = key0 >> a.page_shift;
         if (step == 0 || first + per_tile > batch + 32) {  // 32 pages' numbers and scales at once
           batch = first;
           id = -1;
@@ -1286,7 +1337,7 @@ __global__ void __launch_bounds__(512, 1)
           }
         }
         // groups of 16 keys: lane's group is in page (key0 + 16 · lane) / page
-        const int from = ((key0 + (lane & 7) * 16) / a.page - batch) & 31;
+        const int from = ((key0 + (lane & 7) * 16 >> a.page_shift) - batch) & 31;
         const float ks = __shfl_sync(0xffffffffu, key_scale, from);
         const float ve = __shfl_sync(0xffffffffu, value_e, from);
         const int group_id = __shfl_sync(0xffffffffu, id, from);
@@ -1313,7 +1364,7 @@ __global__ void __launch_bounds__(512, 1)
           mbar_expect_tx(&k_full[ks_stage], bytes);
         }
         __syncwarp();
-        const int y = (page_id * a.heads_kv + at.h) * a.page + key0 % a.page;
+        const int y = (page_id * a.heads_kv + at.h) * a.page;
         if (load)
           tma_load_2d(smem + L::kKOffset + ks_stage * L::kCodeTile + lane * box * HD, &tm_k,
                       &k_full[ks_stage], 0, y);
@@ -1611,7 +1662,7 @@ static int device_sms() {
   return counts[device];
 }
 
-static long long few_workers() { return static_cast<long long>(device_sms()) * 8; }
+static long long few_workers() { return std::min(device_sms() * 8, kMostParts); }
 
 // Bytes of partial results that the kernels of a call may leave: two parts a worker.
 static size_t few_bytes(int head_dim) {
@@ -1714,6 +1765,7 @@ int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyC
   a.requests = p.requests;
   a.pages = p.pages;
   a.page = p.page;
+  a.page_shift = p.page == 16 ? 4 : p.page == 32 ? 5 : p.page == 64 ? 6 : 7;
   a.group = p.group;
   a.per_group = (65536u + p.group - 1) / p.group;
   a.heads_kv = c.heads_kv;

@@ -289,11 +289,10 @@ int cache_plan(const CozyCachePlan& p, cudaStream_t stream) {
 // and their codes are written. WARPS warps share a unit. Queries take CTAs of the same launch.
 // HBM bounds the long form: a token reads (Hq + 2 Hkv) · D bf16 and writes Hq · D bf16 and
 // 2 · Hkv · D codes.
-struct AppendTensor {  // the fields norm_rope_row reads
+struct AppendTensor {
   int normalize;
   const float* norm_weight;
   float norm_offset, norm_eps;
-  int rotate;
 };
 
 struct AppendArgs {
@@ -309,8 +308,83 @@ struct AppendArgs {
   int8_t* exponents[2];
   AppendTensor t[3];
   CozyRope rope;
+  int rotate, wide;  // wide: the tables' rows can be read 16 bytes at a time
   unsigned query_ctas;
 };
+
+// A thread's part of the rotation by one position: cos and sin of its 8 channels (split halves),
+// or of its 4 pairs (interleaved, the first 4). Read once for all heads of a token.
+struct Turn {
+  float c[8], s[8];
+};
+
+template <int HD>
+__device__ __forceinline__ Turn turn_at(const AppendArgs& a, long long position, int d0) {
+  Turn t;
+  const CozyRope& r = a.rope;
+  const float* cs = r.cos + position * r.stride_token;
+  const float* sn = r.sin + position * r.stride_token;
+  const int first = r.interleaved ? d0 / 2 : d0, count = r.interleaved ? 4 : 8;
+  const int columns = r.interleaved ? r.rotary / 2 : r.rotary;
+  if (a.wide && first + count <= columns) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      if (i >= count) break;
+      const float4 c = __ldg(reinterpret_cast<const float4*>(cs + first + i));
+      const float4 s = __ldg(reinterpret_cast<const float4*>(sn + first + i));
+      t.c[i] = c.x; t.c[i + 1] = c.y; t.c[i + 2] = c.z; t.c[i + 3] = c.w;
+      t.s[i] = s.x; t.s[i + 1] = s.y; t.s[i + 2] = s.z; t.s[i + 3] = s.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool in = i < count && first + i < columns;
+      t.c[i] = in ? __ldg(cs + (first + i) * r.stride_channel) : 1.f;
+      t.s[i] = in ? __ldg(sn + (first + i) * r.stride_channel) : 0.f;
+    }
+  }
+  return t;
+}
+
+// Per-head RMSNorm, then the rotation, of a row held 8 channels a thread (the laws of
+// norm_rope.cuh, with the tables' values given): fp32, rounded by the caller.
+template <int HD>
+__device__ __forceinline__ void ready_row(float (&x)[8], int d0, unsigned mask, const AppendTensor& t,
+                                          const AppendArgs& a, const Turn& turn) {
+  constexpr int CHUNKS = HD / 8;
+  if (t.normalize) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+    for (int o = CHUNKS / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+    const float inv = rsqrtf(ss / HD + t.norm_eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] = t.norm_weight ? x[i] * inv * (__ldg(t.norm_weight + d0 + i) + t.norm_offset) : x[i] * inv;
+  }
+  if (!a.rotate || a.rope.rotary == 0) return;
+  if (a.rope.interleaved) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // pairs behind the rotated ones have cos 1, sin 0
+      const float lo = x[2 * i], hi = x[2 * i + 1];
+      x[2 * i] = lo * turn.c[i] - hi * turn.s[i];
+      x[2 * i + 1] = hi * turn.c[i] + lo * turn.s[i];
+    }
+  } else {
+    // channel j pairs with j ± rotary / 2: whole threads, rotary / 16 of them apart
+    const int half = a.rope.rotary / 16, chunk = d0 / 8, lane = threadIdx.x & 31;
+    const int other = chunk < half ? chunk + half : chunk < 2 * half ? chunk - half : chunk;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(mask, x[i], lane - chunk + other);
+    if (chunk < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = chunk < half ? x[i] * turn.c[i] - y[i] * turn.s[i] : x[i] * turn.c[i] + y[i] * turn.s[i];
+    }
+  }
+}
 
 __device__ __forceinline__ void widen8(uint4 v, float (&x)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -361,27 +435,41 @@ __device__ __forceinline__ int exponent_of(float amax) {
   return max(e, kExponentFloor);
 }
 
-template <int HD, int WARPS>
-__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+// Heads of a token that a thread group readies: the tables' values are read once for them.
+constexpr int kHeadsAThread = 4;
+
+template <int HD, int WARPS, int PASSES>
+__global__ void __launch_bounds__(256, 3) cache_append_kernel(const AppendArgs a) {
   constexpr int CHUNKS = HD / 8;         // threads a row
   constexpr int ROWS = 32 / CHUNKS;      // rows a warp and pass
-  constexpr int PASSES = 8;              // rows a unit holds: WARPS · ROWS · PASSES
   constexpr int UNITS = 8 / WARPS;       // units a CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int chunk = lane % CHUNKS, sub = lane / CHUNKS, d0 = chunk * 8;
   const unsigned mask = row_group_mask<CHUNKS>();
 
-  if (blockIdx.x < a.query_ctas) {  // queries: a row a group of threads
-    const long long row = (static_cast<long long>(blockIdx.x) * 8 + warp) * ROWS + sub;
-    if (row >= static_cast<long long>(a.tokens) * a.heads_q) return;
-    const int token = static_cast<int>(row / a.heads_q), head = static_cast<int>(row % a.heads_q);
+  if (blockIdx.x < a.query_ctas) {  // queries: some heads of a token a group of threads
+    const int sets = (a.heads_q + kHeadsAThread - 1) / kHeadsAThread;
+    const unsigned at = (blockIdx.x * 8 + warp) * ROWS + sub;
+    const int token = at / sets, head0 = at % sets * kHeadsAThread;
+    if (token >= a.tokens) return;
     const int position = a.positions[token];
+    uint4 v[kHeadsAThread];
+#pragma unroll
+    for (int i = 0; i < kHeadsAThread; ++i)
+      if (head0 + i < a.heads_q)
+        v[i] = *reinterpret_cast<const uint4*>(a.src[0] + token * a.src_token[0] +
+                                               (head0 + i) * a.src_head[0] + d0);
     if (position < 0) return;
-    float x[8];
-    widen8(*reinterpret_cast<const uint4*>(a.src[0] + token * a.src_token[0] +
-                                           head * a.src_head[0] + d0), x);
-    norm_rope_row<HD>(x, d0, chunk, mask, position, a.t[0], a.rope);
-    *reinterpret_cast<uint4*>(a.out + token * a.out_token + head * a.out_head + d0) = narrow8(x);
+    Turn turn = {};
+    if (a.rotate) turn = turn_at<HD>(a, position, d0);
+#pragma unroll
+    for (int i = 0; i < kHeadsAThread; ++i) {
+      if (head0 + i >= a.heads_q) break;
+      float x[8];
+      widen8(v[i], x);
+      ready_row<HD>(x, d0, mask, a.t[0], a, turn);
+      *reinterpret_cast<uint4*>(a.out + token * a.out_token + (head0 + i) * a.out_head + d0) = narrow8(x);
+    }
     return;
   }
 
@@ -391,11 +479,14 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
   const int head = static_cast<int>((unit >> 1) % a.heads_kv);
   const long long at = (unit >> 1) / a.heads_kv;
   const int4 entry = at < a.max_blocks ? a.blocks[at] : make_int4(-1, 0, 0, 0);
-  if (entry.x < 0) return;  // all warps of the unit alike (WARPS = 8: the whole CTA)
+  if (entry.x < 0) return;  // all warps of the unit alike
   const int slot = (warp % WARPS) * ROWS + sub;
   const AppendTensor& t = a.t[1 + which];
   const __nv_bfloat16* src = a.src[1 + which] + entry.w * a.src_token[1 + which] +
                              head * a.src_head[1 + which] + d0;
+  const long long block = static_cast<long long>(entry.x) * a.heads_kv + head;
+  int8_t* exponent = a.exponents[which] + block;
+  const int before = entry.y > 0 ? *exponent : kExponentFloor;
   uint4 held[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
@@ -410,8 +501,10 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
     if (r < entry.z) {
       float x[8];
       widen8(held[i], x);
-      if (t.normalize || t.rotate) {
-        norm_rope_row<HD>(x, d0, chunk, mask, position + r, t, a.rope);
+      if (which == 0 && (t.normalize || a.rotate)) {
+        Turn turn = {};
+        if (a.rotate) turn = turn_at<HD>(a, position + r, d0);
+        ready_row<HD>(x, d0, mask, t, a, turn);
         held[i] = narrow8(x);
         widen8(held[i], x);
       }
@@ -424,14 +517,12 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const long long block = static_cast<long long>(entry.x) * a.heads_kv + head;
-  int8_t* exponent = a.exponents[which] + block;
-  const int before = entry.y > 0 ? *exponent : kExponentFloor;
   if constexpr (WARPS > 1) {
     if (lane == 0) largest[warp] = amax;
-    __syncthreads();
+    // the unit's own barrier: other units of the CTA may have left
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / WARPS), "n"(WARPS * 32) : "memory");
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) amax = fmaxf(amax, largest[w]);
+    for (int w = 0; w < WARPS; ++w) amax = fmaxf(amax, largest[warp / WARPS * WARPS + w]);
   } else {
     __syncwarp();
   }
@@ -467,20 +558,24 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
 template <int HD>
 static int append_launch(AppendArgs& a, int longest, cudaStream_t stream) {
   constexpr int kRows = 32 / (HD / 8);
-  const long long rows = a.out != nullptr ? static_cast<long long>(a.tokens) * a.heads_q : 0;
+  const long long sets = (a.heads_q + kHeadsAThread - 1) / kHeadsAThread;
+  const long long rows = a.out != nullptr ? a.tokens * sets : 0;
+  if (rows > 0x7fffffffLL) return cudaErrorInvalidValue;
   const long long query_ctas = (rows + 8 * kRows - 1) / (8 * kRows);
   const long long units = 2LL * a.heads_kv * a.max_blocks;
-  // A warp holds 8 passes of rows. Where no block gets more than that, a warp a unit (a decode
-  // step: one row a unit); else the 8 warps of a CTA share one (up to 128 rows).
+  // Four passes of rows a warp, and as many warps a unit as its rows then take (a decode step has
+  // one row a unit; a page of 128 rows of 128 channels takes eight passes of 8 warps).
   const int most = longest < a.page ? longest : a.page;
-  const bool narrow = most <= 8 * kRows;
-  const long long ctas = query_ctas + (narrow ? (units + 7) / 8 : units);
+  const int warps = most <= 4 * kRows ? 1 : most <= 8 * kRows ? 2 : most <= 16 * kRows ? 4 : 8;
+  const long long ctas = query_ctas + (units * warps + 7) / 8;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
   a.query_ctas = static_cast<unsigned>(query_ctas);
-  if (narrow)
-    cache_append_kernel<HD, 1><<<static_cast<unsigned>(ctas), 256, 0, stream>>>(a);
-  else
-    cache_append_kernel<HD, 8><<<static_cast<unsigned>(ctas), 256, 0, stream>>>(a);
+  const unsigned grid = static_cast<unsigned>(ctas);
+  if (warps == 1) cache_append_kernel<HD, 1, 4><<<grid, 256, 0, stream>>>(a);
+  else if (warps == 2) cache_append_kernel<HD, 2, 4><<<grid, 256, 0, stream>>>(a);
+  else if (warps == 4) cache_append_kernel<HD, 4, 4><<<grid, 256, 0, stream>>>(a);
+  else if (most <= 32 * kRows) cache_append_kernel<HD, 8, 4><<<grid, 256, 0, stream>>>(a);
+  else cache_append_kernel<HD, 8, 128 / 8 / kRows><<<grid, 256, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -538,7 +633,6 @@ int cache_append(const CozyCachePlan& p, const CozyCacheStore& c, const CozyCach
     a.t[i].norm_weight = x.norm_weight[i];
     a.t[i].norm_offset = x.norm_offset[i];
     a.t[i].norm_eps = x.norm_eps[i];
-    a.t[i].rotate = x.rope != nullptr;
   }
   if (x.rope != nullptr) {
     a.rope = *x.rope;
@@ -546,6 +640,10 @@ int cache_append(const CozyCachePlan& p, const CozyCacheStore& c, const CozyCach
         a.rope.rotary % 2)
       return cudaErrorInvalidValue;
     if (!a.rope.interleaved && a.rope.rotary % 16) return cudaErrorNotSupported;
+    a.rotate = 1;
+    a.wide = a.rope.stride_channel == 1 && a.rope.stride_token % 4 == 0 &&
+             reinterpret_cast<uintptr_t>(a.rope.cos) % 16 == 0 &&
+             reinterpret_cast<uintptr_t>(a.rope.sin) % 16 == 0;
   }
   return c.head_dim == 64 ? append_launch<64>(a, p.longest, stream)
                           : append_launch<128>(a, p.longest, stream);

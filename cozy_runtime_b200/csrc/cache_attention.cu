@@ -145,9 +145,11 @@ __device__ __forceinline__ int request_of(const CacheArgs& a, const long long* u
 // free of bank conflicts); and V's pairs of keys are joined by byte permutes before widening.
 template <int HD>
 struct Few {
-  static constexpr int kWarps = 8;
+  // Warps by registers: heads of 128 need 255 a thread (at 168 they spill: 198 -> 273 us for 64
+  // requests of 10000 keys on a B200), heads of 64 run with 168 (64 requests of 4000 keys: 80 -> 69 us).
+  static constexpr int kWarps = HD == 128 ? 8 : 12;
   static constexpr int kSlotBytes = kChunkKeys * HD;
-  static constexpr int kSlots = 24576 / kSlotBytes;  // a warp's ring: 24 KB
+  static constexpr int kSlots = 196608 / kWarps / kSlotBytes;  // rings of 192 KB an SM
   static constexpr int kMeta = 8;                    // chunks whose scales are kept
   static constexpr int kBarOffset = kWarps * kSlots * kSlotBytes;
   static constexpr int kMetaOffset = kBarOffset + kWarps * kSlots * 8;
@@ -195,7 +197,7 @@ __device__ __forceinline__ bool few_next(const CacheArgs& a, FewAt& at) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(Few<HD>::kWarps * 32, 1)
     attend_few(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const CacheArgs a) {
   using L = Few<HD>;
@@ -579,7 +581,7 @@ __global__ void __launch_bounds__(256, 1)
 
 // Joins the parts of an item that several workers had: block (item, row). The parts' references
 // and sums are read at once, a thread a part; then 8 warps add the parts up, in a fixed order.
-constexpr int kMostParts = 2048;  // workers: 8 warps an SM
+constexpr int kMostParts = 2048;  // workers: 8 or 12 warps an SM
 
 template <int HD>
 __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
@@ -1662,11 +1664,13 @@ static int device_sms() {
   return counts[device];
 }
 
-static long long few_workers() { return std::min(device_sms() * 8, kMostParts); }
+static long long few_workers(int head_dim) {
+  return std::min(device_sms() * (head_dim == 128 ? Few<128>::kWarps : Few<64>::kWarps), kMostParts);
+}
 
 // Bytes of partial results that the kernels of a call may leave: two parts a worker.
 static size_t few_bytes(int head_dim) {
-  return few_workers() * 2 * kRowsFew * (head_dim * sizeof(float) + sizeof(float2));
+  return few_workers(head_dim) * 2 * kRowsFew * (head_dim * sizeof(float) + sizeof(float2));
 }
 
 static size_t many_bytes(int head_dim) {
@@ -1711,7 +1715,7 @@ static int few_launch(const CozyCacheStore& c, CacheArgs& a, int rows, cudaStrea
   const int box = c.page < kChunkKeys ? c.page : kChunkKeys;
   int e = code_map(&mk, c.key, c, box, true);
   if (e || (e = code_map(&mv, c.value, c, box, true))) return e;
-  attend_few<HD><<<device_sms(), 256, L::kAlloc, stream>>>(mk, mv, a);
+  attend_few<HD><<<device_sms(), L::kWarps * 32, L::kAlloc, stream>>>(mk, mv, a);
   if ((e = cudaGetLastError())) return e;
   return join_launch(join_few<HD>, dim3(a.requests * a.heads_kv, rows), a, stream);
 }
@@ -1782,9 +1786,9 @@ int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyC
   uint8_t* space = static_cast<uint8_t*>(x.workspace);
   if (may_be_few(p)) {
     if (static_cast<long long>(p.requests) * c.heads_kv > 0x7fffffffLL) return cudaErrorInvalidValue;
-    a.workers = static_cast<int>(few_workers());
+    a.workers = static_cast<int>(few_workers(c.head_dim));
     a.ws_o = reinterpret_cast<float*>(space);
-    a.ws_ml = reinterpret_cast<float2*>(a.ws_o + few_workers() * 2 * kRowsFew * c.head_dim);
+    a.ws_ml = reinterpret_cast<float2*>(a.ws_o + few_workers(c.head_dim) * 2 * kRowsFew * c.head_dim);
     space += few_bytes(c.head_dim);
     // rows that an item of few rows can have: whole tokens
     const int per = kRowsFew / p.group;

@@ -74,34 +74,32 @@ class Layout:
         return self.heads_q // self.heads_kv
 
 
-def _need(t: Tensor, name: str, dtype: torch.dtype, shape: tuple[int | None, ...]) -> None:
+def _need(t: Tensor, name: str, dtype: torch.dtype, shape: tuple[int, ...]) -> None:
     if t.dtype != dtype:
         raise ValueError(f"{name} is {t.dtype}, not {dtype}")
-    got = t.shape
-    if got != shape and (
-        len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape))
-    ):
-        raise ValueError(f"{name} has shape {tuple(got)}, not {shape}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
 
 
-def _one_device(device: torch.device, *tensors: Tensor | None) -> None:
+def _one_device(device: torch.device, index: int, *tensors: Tensor) -> None:
+    """All on the CUDA device `index` (-1: not a CUDA device), which is `device`."""
     for t in tensors:
-        if t is not None and t.device != device:
+        if t.get_device() != index:
             raise ValueError(f"operands are on {t.device} and on {device}")
-    if device.type != "cuda":
+    if index < 0:
         raise ValueError("operands are not on a CUDA device")
 
 
 _HERE = contextlib.nullcontext()
 
 
-def _on(device: torch.device):
+def _on(index: int):
     """The device's context, entered only where another one is current."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device.index).cuda_stream
+def _stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 class Cache:
@@ -110,8 +108,10 @@ class Cache:
     heads_kv] int8; a stored value is code · 2^exponent."""
 
     def __init__(self, key: Tensor, value: Tensor, key_exponent: Tensor, value_exponent: Tensor):
-        _need(key, "key", torch.float8_e4m3fn, (None, None, None, None))
+        if key.dim() != 4:
+            raise ValueError("key has shape [pages, heads_kv, page, head_dim]")
         pages, heads, page, dim = key.shape
+        _need(key, "key", torch.float8_e4m3fn, (pages, heads, page, dim))
         _need(value, "value", torch.float8_e4m3fn, (pages, heads, page, dim))
         _need(key_exponent, "key_exponent", torch.int8, (pages, heads))
         _need(value_exponent, "value_exponent", torch.int8, (pages, heads))
@@ -119,13 +119,15 @@ class Cache:
                         ("value_exponent", value_exponent)):
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
-        _one_device(key.device, value, key_exponent, value_exponent)
+        self._index = key.get_device()
+        _one_device(key.device, self._index, value, key_exponent, value_exponent)
         for name, t in (("key", key), ("value", value)):
             if t.data_ptr() % 128:
                 raise ValueError(f"{name} must start on a 128-byte boundary")
         if pages * heads * page > 2**31 - 1:
             raise ValueError("a pool holds at most 2^31 - 1 rows")
         self.key, self.value = key, value
+        self._blocks = pages, heads, page, dim
         self.key_exponent, self.value_exponent = key_exponent, value_exponent
         self._c = _lib.CacheStore(
             key.data_ptr(), value.data_ptr(), key_exponent.data_ptr(), value_exponent.data_ptr(),
@@ -166,6 +168,7 @@ class Plan:
         self._buffers = whole, wide
         self.layout, self.table, self.tokens, self.longest = layout, table, tokens, longest
         self.requests, self.pages = n, free.shape[0]
+        self._blocks = self.pages, layout.heads_kv, page, layout.head_dim
         # what the calls of this step read must outlive them
         self._inputs = (lengths, new, free, cursor)
         at, at8 = whole.data_ptr(), wide.data_ptr()
@@ -274,38 +277,37 @@ def plan(
         raise ValueError("a request holds at most 2^31 - 1 tokens")
     if not 0 <= tokens < 2**31 or not 0 <= longest < 2**31:
         raise ValueError("tokens and longest must be counts below 2^31")
-    device = table.device
-    _one_device(device, lengths, new, free, cursor)
+    index = table.get_device()
+    _one_device(table.device, index, lengths, new, free, cursor)
     made = Plan(layout, table, lengths, new, free, cursor, tokens, longest)
-    with _on(device):
-        code = _lib.load().cozy_cache_plan(ctypes.byref(made._c), _stream(device))
+    with _on(index):
+        code = _lib.load().cozy_cache_plan(ctypes.byref(made._c), _stream(index))
     _lib.check("cozy_cache_plan", code)
     return made
 
 
-def _rows(t: Tensor, name: str, step: Plan, heads: int) -> tuple[int, int]:
+def _rows(t: Tensor, name: str, tokens: int, heads: int, dim: int) -> tuple[int, int]:
     """Element strides {token, head} of a step's [tokens, heads, head_dim] rows."""
-    dim = step.layout.head_dim
-    _need(t, name, torch.bfloat16, (step.tokens, heads, dim))
+    if t.dtype != torch.bfloat16 or t.shape != (tokens, heads, dim):
+        _need(t, name, torch.bfloat16, (tokens, heads, dim))
     token, head, last = t.stride()
-    if step.tokens <= 1:
+    if tokens <= 1:
         token = dim
     if heads == 1:
         head = dim
-    if (last != 1 and step.tokens > 0) or token % 8 or head % 8 or t.data_ptr() % 16:
+    if (last != 1 and tokens > 0) or (token | head) % 8 or t.data_ptr() % 16:
         raise ValueError(f"{name}: the head dimension must be contiguous and rows 16-byte aligned")
     return token, head
 
 
-def _out(given: Tensor | None, like: Tensor, step: Plan) -> tuple[Tensor, tuple[int, int]]:
+def _out(given: Tensor | None, like: Tensor) -> tuple[Tensor, tuple[int, int]]:
+    tokens, heads, dim = like.shape
     if given is None:
-        given = torch.empty(like.shape, dtype=like.dtype, device=like.device)
-        return given, (like.shape[1] * like.shape[2], like.shape[2])
-    token, head = _rows(given, "out", step, like.shape[1])
-    rows, heads, dim = given.shape
+        return like.new_empty(like.shape), (heads * dim, dim)
+    token, head = _rows(given, "out", tokens, heads, dim)
     apart = head >= dim and token >= (heads - 1) * head + dim
-    apart = apart or (token >= dim and head >= (rows - 1) * token + dim)
-    if rows * heads > 1 and not apart:
+    apart = apart or (token >= dim and head >= (tokens - 1) * token + dim)
+    if tokens * heads > 1 and not apart:
         raise ValueError("rows of out overlap")
     return given, (token, head)
 
@@ -316,11 +318,9 @@ def _range(t: Tensor) -> tuple[int, int]:
 
 
 def _fits(store: Cache, step: Plan) -> None:
-    c, layout = store._c, step.layout
-    if (c.heads_kv, c.page, c.head_dim) != (layout.heads_kv, layout.page, layout.head_dim):
-        raise ValueError("the cache's heads or pages are not the plan's layout")
-    if c.pages != step.pages:
-        raise ValueError(f"a cache of {c.pages} pages and a plan over {step.pages}")
+    if store._blocks != step._blocks:
+        raise ValueError(f"a cache of {store._blocks} [pages, heads, page, head_dim] "
+                         f"and a plan over {step._blocks}")
 
 
 def append(
@@ -349,20 +349,26 @@ def append(
     NaN and leave the exponent alone. The same step can be appended again: it stores the same.
     A page that requests share must be full: two writers of one block are not ordered."""
     _fits(store, step)
-    layout = step.layout
-    device = store.key.device
-    _one_device(device, step.table, key, value, query, out)
+    layout, index, tokens = step.layout, store._index, step.tokens
+    device, dim = store.key.device, layout.head_dim
+    _one_device(device, index, step.table, key, value)
     a = _lib.CacheAppend()
     a.key, a.value = key.data_ptr(), value.data_ptr()
-    a.key_strides[:] = _rows(key, "key", step, layout.heads_kv)
-    a.value_strides[:] = _rows(value, "value", step, layout.heads_kv)
+    a.key_strides[:] = _rows(key, "key", tokens, layout.heads_kv, dim)
+    a.value_strides[:] = _rows(value, "value", tokens, layout.heads_kv, dim)
     if query is not None:
-        a.query_strides[:] = _rows(query, "query", step, layout.heads_q)
+        _one_device(device, index, query)
+        a.query_strides[:] = _rows(query, "query", tokens, layout.heads_q, dim)
+        given, (out, strides) = out, _out(out, query)
+        if given is not None:
+            _one_device(device, index, out)
+        a.query, a.out = query.data_ptr(), out.data_ptr()
+        a.out_strides[:] = strides
     elif norm_q is not None or out is not None:
         raise ValueError("norm_q and out are the query's")
     tables = None
     if rope is not None:
-        _one_device(device, rope.cos, rope.sin)
+        _one_device(device, index, rope.cos, rope.sin)
         last = step._c.width * layout.page - 1
         columns = rope.rotary // 2 if rope.interleaved else rope.rotary
         if rope.rotary < 0 or rope.rotary > layout.head_dim or rope.rotary % 2:
@@ -389,13 +395,9 @@ def append(
             w = norm.weight.to(device=device, dtype=torch.float32).contiguous()
             weights.append(w)
             a.norm_weight[i] = w.data_ptr()
-    if query is not None:
-        out, strides = _out(out, query, step)
-        a.query, a.out = query.data_ptr(), out.data_ptr()
-        a.out_strides[:] = strides
-    with _on(device):
+    with _on(index):
         code = _lib.load().cozy_cache_append(
-            ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a), _stream(device)
+            ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a), _stream(index)
         )
     _lib.check("cozy_cache_append", code)
     return out
@@ -419,32 +421,31 @@ def attention(
     What stands in blocks behind a row's last key, NaN among it, does not reach the row. Keys in a
     page whose number is outside the pool are left out, and the plan's status says so."""
     _fits(store, step)
-    device = store.key.device
-    _one_device(device, step.table, query, out)
-    scale = 1.0 / math.sqrt(step.layout.head_dim) if scale is None else float(scale)
+    layout, index = step.layout, store._index
+    _one_device(store.key.device, index, step.table, query)
+    scale = 1.0 / math.sqrt(layout.head_dim) if scale is None else float(scale)
     if not (0.0 < scale < 3e38):
         raise ValueError("attention scale must be positive and finite")
     a = _lib.CacheAttend()
     a.query, a.scale = query.data_ptr(), scale
-    a.query_strides[:] = _rows(query, "query", step, step.layout.heads_q)
-    given, (out, strides) = out, _out(out, query, step)
-    if given is not None and query.numel() > 0:
+    a.query_strides[:] = _rows(query, "query", step.tokens, layout.heads_q, layout.head_dim)
+    given, (out, strides) = out, _out(out, query)
+    if given is not None:
+        _one_device(store.key.device, index, out)
         (q0, q1), (o0, o1) = _range(query), _range(out)
-        if q0 < o1 and o0 < q1:
+        if q0 < o1 and o0 < q1 and query.numel() > 0:
             raise ValueError("out overlaps the query")
     a.out = out.data_ptr()
     a.out_strides[:] = strides
     lse = None
     if return_lse:
-        lse = torch.empty(query.shape[:2], dtype=torch.float32, device=device)
+        lse = query.new_empty(query.shape[:2], dtype=torch.float32)
         a.lse = lse.data_ptr()
-    lib = _lib.load()
-    with _on(device):
-        size = lib.cozy_cache_workspace(ctypes.byref(step._c), ctypes.byref(store._c))
-        space = torch.empty(size, dtype=torch.uint8, device=device)
+    lib, plan_c, store_c = _lib.load(), ctypes.byref(step._c), ctypes.byref(store._c)
+    with _on(index):
+        size = lib.cozy_cache_workspace(plan_c, store_c)
+        space = query.new_empty(size, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = space.data_ptr(), size
-        code = lib.cozy_cache_attention(
-            ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a), _stream(device)
-        )
+        code = lib.cozy_cache_attention(plan_c, store_c, ctypes.byref(a), _stream(index))
     _lib.check("cozy_cache_attention", code)
     return out if lse is None else (out, lse)

@@ -1134,11 +1134,12 @@ __global__ void __launch_bounds__(512, 1)
             ok = false;
             break;
           }
-          float mul_of[GROUPS], add_of[GROUPS];
+          float mul_of[GROUPS], add_of[GROUPS], back_of[GROUPS];
 #pragma unroll
           for (int c = 0; c < GROUPS; ++c) {
             mul_of[c] = group_mul(mul, scales[c * (4 / GROUPS)]);
             add_of[c] = scales[8 + c * (4 / GROUPS)];
+            back_of[c] = scales[16 + c * (4 / GROUPS)];
           }
           const int gone = reinterpret_cast<const int*>(scales)[24 - b * 4];
           if (!many_wait(&s_full[2 * s + b], phase >> b & 1, abort, a.status)) {
@@ -1194,19 +1195,16 @@ __global__ void __launch_bounds__(512, 1)
           }
           if (m == -INFINITY) m = m_new;
           const float ref = (m == -INFINITY ? 0.f : m) - kManyBias;
+          uint32_t pk[32];
           float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int of = c * 2 + e, group = of * GROUPS / 4;
-              if (of % (4 / GROUPS) == 0) acc = make_float2(0.f, 0.f);
-              weigh16(&r[c][e * 16], mul_of[group], add_of[group] - ref, acc, pk + 8 * e);
-              if ((of + 1) % (4 / GROUPS) == 0) l = fmaf(acc.x + acc.y, scales[16 + of], l);
-            }
-            tmem_st16(tS + b * 64 + c * 16, pk);
+          for (int of = 0; of < 4; ++of) {
+            const int group = of * GROUPS / 4;
+            if (of % (4 / GROUPS) == 0) acc = make_float2(0.f, 0.f);
+            weigh16(&r[of / 2][of % 2 * 16], mul_of[group], add_of[group] - ref, acc, pk + 8 * of);
+            if ((of + 1) % (4 / GROUPS) == 0) l = fmaf(acc.x + acc.y, back_of[group], l);
           }
+          tmem_st32(tS + b * 64, pk);
           if (partial) {
             // values that are NaN in a tile that some row does not see whole: the rows that see
             // the key take the NaN, in its channels, at the end

@@ -317,3 +317,329 @@ def test_attention_matches_the_law(lengths, new, page, hq, hkv, dim, amp):
     again = cache.attention(store, step, q.cuda())
     assert torch.equal(again[:used], out[:used])
     step.check()
+
+
+@pytest.mark.parametrize("lengths,new,page,hq,hkv,dim", [
+    ([20000], [1], 64, 8, 2, 128),  # one row's keys over every worker
+    ([9000, 40], [3, 1], 128, 4, 2, 64),
+    ([3000, 0], [200, 1], 32, 6, 2, 128),  # an item's tiles over several workers
+    ([2500], [90], 64, 2, 1, 64),
+])
+def test_attention_over_long_contexts(lengths, new, page, hq, hkv, dim):
+    from cozy_runtime_b200 import cache
+
+    g = torch.Generator().manual_seed(sum(lengths))
+    m = make(lengths, new, page, g)
+    step, t = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    k, ke = fill(step.pages, hkv, page, dim, g)
+    v, ve = fill(step.pages, hkv, page, dim, g)
+    q = torch.randn(m["tokens"], hq, dim, generator=g).to(torch.bfloat16)
+    out, lse = cache.attention(store_on_gpu(k, ke, v, ve), step, q.cuda(), scale=0.2, return_lse=True)
+    want = law.attend_step(values(k, ke), values(v, ve), t["table"].tolist(), lengths, new, q, page, 0.2)
+    check_attention(out, lse, want, m["tokens"], floor_of(max(lengths) + max(new), ve))
+
+
+@pytest.mark.parametrize("lengths,new,hq,hkv,dim", [
+    ([100, 30], [1, 1], 4, 2, 128), ([100, 30], [5, 3], 2, 1, 64), ([100, 30], [150, 90], 4, 2, 128),
+    ([100, 30], [150, 90], 3, 1, 64),
+])
+def test_attention_nan_reaches_the_rows_that_see_it(lengths, new, hq, hkv, dim):
+    """A NaN value reaches its own channels, a NaN key whole rows, of those rows only that see it."""
+    from cozy_runtime_b200 import cache
+
+    page = 32
+    g = torch.Generator().manual_seed(3)
+    m = make(lengths, new, page, g)
+    step, t = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    k, ke = fill(step.pages, hkv, page, dim, g)
+    v, ve = fill(step.pages, hkv, page, dim, g)
+    q = torch.randn(m["tokens"], hq, dim, generator=g).to(torch.bfloat16).cuda()
+    plain, plain_lse = cache.attention(store_on_gpu(k, ke, v, ve), step, q, return_lse=True)
+    table, group = t["table"].tolist(), hq // hkv
+    kf, vf = k.float(), v.float()
+    spots = [(0, lengths[0] + new[0] - 1, "v"), (0, 7, "v"), (1, lengths[1] + new[1] // 2, "k")]
+    for n, x, which in spots:
+        to = (kf if which == "k" else vf)[table[n][x // page], hkv - 1, x % page]
+        to[dim - 3] = math.nan
+    got, lse = cache.attention(
+        store_on_gpu(kf.to(torch.float8_e4m3fn), ke, vf.to(torch.float8_e4m3fn), ve), step, q, return_lse=True)
+    hit = torch.zeros(got.shape, dtype=torch.bool)
+    t0 = 0
+    for n, (length, a) in enumerate(zip(lengths, new)):
+        for i in range(a):
+            for which_n, x, which in spots:
+                if which_n == n and x <= length + i:
+                    channels = slice(None) if which == "k" else slice(dim - 3, dim - 2)
+                    hit[t0 + i, (hkv - 1) * group:, channels] = True
+        t0 += a
+    assert torch.equal(got.isnan().cpu(), hit)
+    assert torch.equal(got.cpu()[~hit], plain.cpu()[~hit])
+    rows = hit.all(-1)
+    assert torch.equal(lse.cpu()[~rows], plain_lse.cpu()[~rows]) and lse.cpu()[rows].isnan().all()
+
+
+@pytest.mark.parametrize("new,dim", [([1, 1, 1], 128), ([4, 1, 2], 64), ([200, 1, 60], 128), ([70, 70, 1], 64)])
+def test_attention_leaves_out_bad_pages(new, dim):
+    """Page numbers outside the pool (written into the table behind the plan): their keys are left
+    out and the status says so; a row without any key is zero, its lse -inf."""
+    from cozy_runtime_b200 import cache
+
+    lengths, page, hq, hkv = [130, 75, 20], 16, 4, 2
+    g = torch.Generator().manual_seed(8)
+    m = make(lengths, new, page, g)
+    step, t = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    k, ke = fill(step.pages, hkv, page, dim, g)
+    v, ve = fill(step.pages, hkv, page, dim, g)
+    table = t["table"].tolist()
+    table[0][2], table[0][5], table[0][8], table[2] = step.pages, -1, 2**31 - 1, [-5] * len(table[2])
+    t["table"].copy_(torch.tensor(table, dtype=torch.int32))
+    q = torch.randn(m["tokens"], hq, dim, generator=g).to(torch.bfloat16)
+    out, lse = cache.attention(store_on_gpu(k, ke, v, ve), step, q.cuda(), return_lse=True)
+    want = law.attend_step(values(k, ke), values(v, ve), table, lengths, new, q, page, dim**-0.5)
+    check_attention(out, lse, want, m["tokens"], floor_of(500, ve))
+    assert (out[-new[2]:] == 0).all()
+    assert int(step.status) == 16
+
+
+@pytest.mark.parametrize("new", [[1, 2], [70, 90]])
+def test_attention_over_the_whole_range_of_scales(new):
+    """Value exponents from the floor to the ceiling in one row, keys of tiny blocks, zero queries."""
+    from cozy_runtime_b200 import cache
+
+    lengths, page, hq, hkv, dim = [200, 90], 16, 2, 1, 64
+    g = torch.Generator().manual_seed(5)
+    m = make(lengths, new, page, g)
+    step, t = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    k, ke = fill(step.pages, hkv, page, dim, g)
+    v, _ = fill(step.pages, hkv, page, dim, g)
+    ve = torch.randint(-60, 41, (step.pages, hkv), generator=g).to(torch.int8)
+    ke[::3] = -60
+    k[1::5] = 0
+    q = torch.randn(m["tokens"], hq, dim, generator=g)
+    q[::4] = 0
+    q[1::4] *= 1e-20
+    q = q.to(torch.bfloat16)
+    out, lse = cache.attention(store_on_gpu(k, ke, v, ve), step, q.cuda(), return_lse=True)
+    want = law.attend_step(values(k, ke), values(v, ve), t["table"].tolist(), lengths, new, q, page, dim**-0.5)
+    check_attention(out, lse, want, m["tokens"], floor_of(300, ve))
+
+
+def test_attention_far_into_a_large_pool():
+    """Blocks behind the first 4 GB of a pool, rows of a packed projection, a strided output."""
+    from cozy_runtime_b200 import cache
+
+    page, hkv, hq, dim, pages = 128, 8, 16, 128, 40000
+    g = torch.Generator().manual_seed(6)
+    for lengths, new in (([300, 77], [1, 1]), ([300, 77], [60, 40])):  # 3 pages and 1
+        layout = cache.Layout(hq, hkv, dim, page)
+        large = cache.Cache.empty(layout, pages)
+        table = torch.tensor([[pages - 1, 5, pages - 2, pages - 7], [pages - 4, pages - 3, 0, 1]], dtype=torch.int32)
+        small_table = torch.tensor([[0, 1, 2, 3], [4, 5, 6, 7]], dtype=torch.int32)
+        k, ke = fill(8, hkv, page, dim, g)
+        v, ve = fill(8, hkv, page, dim, g)
+        small = store_on_gpu(k, ke, v, ve)
+        at = table.reshape(-1).long().cuda()
+        for to, of in ((large.key, small.key), (large.value, small.value)):
+            to.view(torch.uint8)[at] = of.view(torch.uint8)
+        for to, of in ((large.key_exponent, small.key_exponent), (large.value_exponent, small.value_exponent)):
+            to[at] = of
+        T = sum(new)
+        qkv = torch.randn(T, hq + 2 * hkv, dim, generator=g).to(torch.bfloat16).cuda()
+        q = qkv[:, :hq]
+        outs = []
+        for store, tab, n_pages in ((large, table, pages), (small, small_table, 8)):
+            # no request needs a page that its row does not name already
+            step = cache.plan(layout, tab.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(),
+                              torch.tensor(new, dtype=torch.int32).cuda(),
+                              torch.zeros(n_pages, dtype=torch.int32).cuda(),
+                              torch.zeros(2, dtype=torch.int64).cuda(), tokens=T, longest=max(new))
+            outs.append((store, step))
+        results = []
+        for store, step in outs:
+            step.check()
+            cache.append(store, step, qkv[:, hq:hq + hkv], qkv[:, hq + hkv:])
+            out = torch.zeros(T, 2 * hq, dim, dtype=torch.bfloat16, device="cuda")
+            cache.attention(store, step, q, out=out[:, ::2])
+            assert (out[:, 1::2] == 0).all()
+            results.append(out)
+        assert torch.equal(results[0], results[1])
+        assert torch.equal(large.key.view(torch.uint8)[at], small.key.view(torch.uint8))
+
+
+# --------------------------------------------------------------------------------------- together
+def test_requests_come_grow_and_go():
+    """Steps as a server makes them: prompts in chunks, single tokens, drafts, finished requests
+    whose pages go to others, two layers. Lengths and cursor go from step to step."""
+    from cozy_runtime_b200 import cache, rope, ulysses
+
+    g = torch.Generator().manual_seed(12)
+    layout = cache.Layout(6, 2, 64, 16)
+    pages, width = 40, 20
+    table = torch.zeros(3, width, dtype=torch.int32, device="cuda")
+    free = torch.randperm(pages, generator=g).to(torch.int32).cuda()
+    lengths = torch.zeros(3, dtype=torch.int32, device="cuda")
+    cursor = torch.tensor([0, pages], device="cuda")
+    stores = [cache.Cache.empty(layout, pages) for _ in "ab"]
+    spec = rope.llama(width * 16, 64).to("cuda")
+    norm = ulysses.Norm(torch.rand(64, generator=g) + 0.5)
+    steps = [[70, 5, 0], [33, 1, 90], [1, 1, 1], [4, -1, 1], [1, 200, 3], [-1, 1, 1], [120, -1, -1], [1, 0, 40]]
+    held = [0, 0, 0]
+    for new in steps:
+        t = sum(max(a, 0) for a in new)
+        step = cache.plan(layout, table, lengths, torch.tensor(new, dtype=torch.int32).cuda(), free, cursor,
+                          tokens=t + 3, longest=max(new))
+        step.check()
+        lengths, cursor = step.lengths, step.cursor
+        for store in stores:
+            qkv = torch.randn(t + 3, 10, 64, generator=g).to(torch.bfloat16).cuda()
+            q, k, v = qkv.split([6, 2, 2], dim=1)
+            q = cache.append(store, step, k, v, query=q, rope=spec, norm_q=norm, norm_k=norm)
+            out, lse = cache.attention(store, step, q, return_lse=True)
+            step.check()
+            kv, vv = (x.double().cpu() for x in store.read(torch.arange(pages, device="cuda")))
+            want = law.attend_step(kv, vv, table.tolist(), held, new, q.cpu(), 16, 0.125)
+            check_attention(out, lse, want, t, floor_of(400, store.value_exponent))
+        held = [0 if a < 0 else x + a for x, a in zip(held, new)]
+        assert lengths.tolist() == held
+        free_now = sum(-(-x // 16) for x in held)
+        assert int(cursor[1] - cursor[0]) == pages - free_now
+
+
+def test_a_captured_step_plans_anew_at_each_replay():
+    from cozy_runtime_b200 import cache, rope
+
+    g = torch.Generator().manual_seed(13)
+    layout = cache.Layout(8, 2, 128, 32)
+    spec = rope.llama(40 * 32, 128).to("cuda")
+    for longest, news in ((1, ([1, 1, 0], [1, 1, 1], [0, 1, 1])), (100, ([100, 3, 1], [1, 0, 60], [7, 80, 0]))):
+        T = 200
+        m = make([40, 1000, 333], [longest] * 3, 32, g, spare=40)
+        state = {k: torch.tensor(m[k], dtype=torch.int64 if k == "cursor" else torch.int32, device="cuda")
+                 for k in ("table", "lengths", "new", "free", "cursor")}
+        state["table"] = torch.cat([state["table"], state["table"].new_full((3, 4), -1)], dim=1)
+        pages = len(m["free"])
+        k, ke = fill(pages, 2, 32, 128, g)
+        stores = [store_on_gpu(k, ke, k, ke) for _ in "ab"]
+        qkv = torch.empty(T, 12, 128, dtype=torch.bfloat16, device="cuda")
+
+        def step(store, s):
+            p = cache.plan(layout, s["table"], s["lengths"], s["new"], s["free"], s["cursor"], tokens=T, longest=longest)
+            q = cache.append(store, p, qkv[:, 8:10], qkv[:, 10:], query=qkv[:, :8], rope=spec)
+            out = torch.zeros(T, 8, 128, dtype=torch.bfloat16, device="cuda")
+            cache.attention(store, p, q, out=out)
+            s["lengths"].copy_(p.lengths)
+            s["cursor"].copy_(p.cursor)
+            return out, p
+
+        captured, eager = ({k: v.clone() for k, v in state.items()} for _ in "ab")
+        warm = {k: v.clone() for k, v in state.items()}
+        warm["new"].zero_()
+        step(cache.Cache.empty(layout, pages), warm)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured_out, captured_plan = step(stores[0], captured)
+        for new in news:
+            qkv.copy_(torch.randn(T, 12, 128, generator=g))
+            for s in (captured, eager):
+                s["new"].copy_(torch.tensor(new, dtype=torch.int32))
+            graph.replay()
+            out, p = step(stores[1], eager)
+            p.check()
+            captured_plan.check()
+            assert torch.equal(captured["lengths"], eager["lengths"]) and torch.equal(captured["table"], eager["table"])
+            assert torch.equal(captured_out, out)
+            for a, b in ((stores[0].key, stores[1].key), (stores[0].value, stores[1].value)):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+            assert (out[sum(new):] == 0).all()
+
+
+@pytest.mark.parametrize("new", [[1] * 20, [60, 1, 9] + [1] * 17])
+def test_calls_side_by_side_on_two_streams(new):
+    """Two layers of one step on two streams: the same plan, caches of their own."""
+    from cozy_runtime_b200 import cache
+
+    g = torch.Generator().manual_seed(14)
+    lengths = [137 * i % 900 for i in range(20)]
+    m = make(lengths, new, 64, g)
+    step, _ = on_gpu(m, cache.Layout(8, 2, 128, 64))
+    made = []
+    for _ in "ab":
+        k, ke = fill(step.pages, 2, 64, 128, g)
+        v, ve = fill(step.pages, 2, 64, 128, g)
+        q = torch.randn(m["tokens"], 8, 128, generator=g).to(torch.bfloat16).cuda()
+        made.append((store_on_gpu(k, ke, v, ve), q))
+    alone = [cache.attention(s, step, q) for s, q in made]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in made]
+    outs = [[], []]
+    for _ in range(10):
+        for i, (stream, (s, q)) in enumerate(zip(streams, made)):
+            with torch.cuda.stream(stream):
+                outs[i].append(cache.attention(s, step, q))
+    torch.cuda.synchronize()
+    for want, got in zip(alone, outs):
+        assert all(torch.equal(want, x) for x in got)
+
+
+def test_an_empty_step():
+    from cozy_runtime_b200 import cache
+
+    layout = cache.Layout(4, 2, 64, 16)
+    m = make([5, 0], [0, 0], 16, torch.Generator().manual_seed(1))
+    step, _ = on_gpu(m, layout)
+    store = cache.Cache.empty(layout, step.pages)
+    q, k = (torch.empty(0, h, 64, dtype=torch.bfloat16, device="cuda") for h in (4, 2))
+    assert cache.append(store, step, k, k, query=q).shape == (0, 4, 64)
+    out, lse = cache.attention(store, step, q, return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    step.check()
+
+
+def test_refusals():
+    from cozy_runtime_b200 import _lib, cache, rope, ulysses
+    import ctypes
+
+    layout = cache.Layout(4, 2, 64, 16)
+    m = make([20, 0], [1, 2], 16, torch.Generator().manual_seed(1))
+    step, t = on_gpu(m, layout)
+    store = cache.Cache.empty(layout, step.pages)
+    q, k = (torch.zeros(3, h, 64, dtype=torch.bfloat16, device="cuda") for h in (4, 2))
+    bad = [
+        lambda: cache.attention(store, step, q.float()),
+        lambda: cache.attention(store, step, q[:2]),
+        lambda: cache.attention(store, step, q.cpu()),
+        lambda: cache.attention(store, step, q.transpose(1, 2).contiguous().transpose(1, 2)),
+        lambda: cache.attention(store, step, q, scale=0.0),
+        lambda: cache.attention(store, step, q, scale=-1.0),
+        lambda: cache.attention(store, step, q, scale=math.inf),
+        lambda: cache.attention(store, step, q, out=q),
+        lambda: cache.attention(store, step, q, out=q[:1].expand(3, 4, 64)),
+        lambda: cache.attention(cache.Cache.empty(layout, step.pages + 1), step, q),
+        lambda: cache.attention(cache.Cache.empty(cache.Layout(4, 2, 64, 32), step.pages), step, q),
+        lambda: cache.append(store, step, k, q),
+        lambda: cache.append(store, step, k, k, out=q),
+        lambda: cache.append(store, step, k, k, norm_q=ulysses.Norm()),
+        lambda: cache.append(store, step, k, k, query=q, norm_q=ulysses.Norm(torch.ones(32))),
+        lambda: cache.append(store, step, k, k, query=q, rope=rope.llama(16, 64).to("cuda")),
+        lambda: cache.append(store, step, k, k, query=q, rope=rope.llama(2000, 64)),
+        lambda: cache.append(store, step, k, k, query=q, rope=rope.llama(2000, 128).to("cuda")),
+        lambda: cache.Cache(store.key, store.value, store.key_exponent[:1], store.value_exponent),
+        lambda: cache.Cache(store.key, store.value.bfloat16(), store.key_exponent, store.value_exponent),
+        lambda: cache.Cache(store.key, store.value.cpu(), store.key_exponent, store.value_exponent),
+        lambda: cache.plan(layout, t["table"], t["lengths"], t["new"], t["free"], t["cursor"].cpu(), tokens=3, longest=2),
+        lambda: cache.plan(layout, t["table"].T, t["lengths"], t["new"], t["free"], t["cursor"], tokens=3, longest=2),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    # the C entries' own checks: a workspace too small, a pointer off its boundary
+    lib = _lib.load()
+    a = _lib.CacheAttend()
+    a.query = a.out = q.data_ptr()
+    a.query_strides[:] = a.out_strides[:] = (256, 64)
+    a.scale, a.workspace, a.workspace_bytes = 1.0, q.data_ptr(), 0
+    call = lambda: lib.cozy_cache_attention(ctypes.byref(step._c), ctypes.byref(store._c), ctypes.byref(a), 0)  # noqa: E731
+    assert call() == _lib.INVALID_VALUE
+    a.query = q.data_ptr() + 2
+    assert call() == _lib.INVALID_VALUE
+    torch.cuda.synchronize()

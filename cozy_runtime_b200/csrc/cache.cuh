@@ -74,19 +74,20 @@ __host__ __device__ inline long long floor_sum_128(uint32_t n, uint32_t a, long 
 
 // ------------------------------------------------------------------------ the attention's work
 // A request's new tokens × the group's query heads are the rows that read one key/value head. Each
-// request goes by its own rows: up to kFewItems items of kRowsFew rows (whole tokens) walk the
-// keys in chunks of kChunkKeys; more rows are cut into items of kRowsMany whose keys are walked in
+// request goes by its own rows: up to kFewItems items of kRowsFew rows walk the keys in chunks of
+// kChunkKeys; more rows are cut into items of kRowsMany (whole tokens) whose keys are walked in
 // tiles of kTileKeys. A unit is one chunk or tile; a plan counts the units of one key/value head
-// before each request, of either kind. (An item of few rows reads its keys again, from L2: on a
-// B200 20 rows took X us as two such items and Y as one item of many, Z against W at 60.)
-constexpr int kRowsFew = 16;
+// before each request, of either kind. An item of few rows reads its keys again, mostly from L2:
+// on a B200 16 requests of 8000 keys and 8 heads took 110 us with 20 rows as three such items,
+// 244 with 48 rows as six, and 127 as one item of many whatever its rows.
+constexpr int kRowsFew = 8;
 constexpr int kFewItems = 3;
 constexpr int kChunkKeys = 64;
 constexpr int kRowsMany = 256;
 constexpr int kTileKeys = 128;
 
 __host__ __device__ __forceinline__ bool few_rows(int group, long long added) {
-  return group <= kRowsFew && added <= kFewItems * (kRowsFew / group);
+  return group * added <= kRowsFew * kFewItems;
 }
 
 // Units before item `item` of a request with `cached` tokens before its new ones: the tiles of
@@ -106,8 +107,7 @@ __host__ __device__ __forceinline__ long long attention_units(int group, long lo
                                                               long long added) {
   if (added == 0) return 0;
   if (few_rows(group, added)) {
-    const int per = kRowsFew / group;
-    return quotient(added + per - 1, per) * ((cached + added + kChunkKeys - 1) / kChunkKeys);
+    return quotient(added * group + kRowsFew - 1, kRowsFew) * ((cached + added + kChunkKeys - 1) / kChunkKeys);
   }
   const int per = kRowsMany / group;
   const long long items = quotient(added + per - 1, per);

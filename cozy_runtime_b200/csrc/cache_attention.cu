@@ -134,23 +134,23 @@ __device__ __forceinline__ int request_of(const CacheArgs& a, const long long* u
 }
 
 // ------------------------------------------------------------------------------- few rows
-// Matrix instructions are mma.sync m16n8k16: the query rows of an item (group · new tokens, at
-// most 16) are their 16 rows, keys their columns. HBM bounds this: a chunk is 2 · 64 · HD bytes
-// and 4 · 16 · 64 · HD operations on the tensor cores, an eighth of what even these instructions
-// do in the time. Codes are widened to f16 in registers (exact) straight from the swizzled tile
-// that TMA wrote. The operand layouts are chosen so that no shuffle or transposing load is
-// needed: the contraction over channels may run in any order, so a thread's 16 consecutive
-// channels of a key serve four instructions; the keys of a tile may be taken in any order
-// (column c is row (c & 1 ? c + 4 : c) mod 8 of 8, which keeps the 16-byte reads of both K and V
-// free of bank conflicts); and V's pairs of keys are joined by byte permutes before widening.
+// HBM bounds this: a chunk is 2 · 64 · HD bytes. The matrix instructions are mma.sync m16n8k16
+// with the keys as their 16 rows and the 8 query rows of an item as their columns (queries as the
+// 16 rows left half of every instruction, weight and accumulator of a decode step unused: 64
+// requests of 10000 keys 223 against 211 us in a loop under the power cap, 10 requests of 1800
+// keys and 24 heads 37 against 32). Codes are widened to f16 in registers (exact) straight from the swizzled tile
+// that TMA wrote. The operand layouts are chosen so that no transposing load is needed: the
+// contraction over channels may run in any order, so a thread's 16 consecutive channels of a key
+// serve four instructions; the keys of a tile may be taken in any order (row c is
+// (c & 1 ? c + 4 : c) mod 8 of 8, which keeps the 16-byte reads of both K and V free of bank
+// conflicts); V's pairs of keys are joined by byte permutes before widening; and movmatrix turns
+// the weights from a thread a key to a thread a row.
 template <int HD>
 struct Few {
-  // Warps by registers: heads of 128 need 255 a thread (at 168 they spill: 198 -> 273 us for 64
-  // requests of 10000 keys on a B200), heads of 64 run with 168 (64 requests of 4000 keys: 80 -> 69 us).
   static constexpr int kWarps = HD == 128 ? 8 : 12;
   static constexpr int kSlotBytes = kChunkKeys * HD;
   static constexpr int kSlots = 196608 / kWarps / kSlotBytes;  // rings of 192 KB an SM
-  static constexpr int kMeta = 8;                    // chunks whose scales are kept
+  static constexpr int kMeta = 8;                              // chunks whose scales are kept
   static constexpr int kBarOffset = kWarps * kSlots * kSlotBytes;
   static constexpr int kMetaOffset = kBarOffset + kWarps * kSlots * 8;
   static constexpr int kAlloc = kMetaOffset + kWarps * kMeta * 32 + 1024;
@@ -164,10 +164,11 @@ struct FewAt {
 };
 
 __device__ __forceinline__ void few_request(const CacheArgs& a, FewAt& at, int n) {
-  const int per = kRowsFew / a.group;  // tokens an item
   at.n = n;
   at.keys = a.lengths[n];
-  at.items = a.units_few[n + 1] == a.units_few[n] ? 0 : (a.starts[n + 1] - a.starts[n] + per - 1) / per;
+  at.items = a.units_few[n + 1] == a.units_few[n]
+                 ? 0
+                 : ((a.starts[n + 1] - a.starts[n]) * a.group + kRowsFew - 1) / kRowsFew;
   at.chunks = (at.keys + kChunkKeys - 1) / kChunkKeys;
 }
 
@@ -196,13 +197,19 @@ __device__ __forceinline__ bool few_next(const CacheArgs& a, FewAt& at) {
   return true;
 }
 
+__device__ __forceinline__ uint32_t transposed(uint32_t pair) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(pair));
+  return r;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(Few<HD>::kWarps * 32, 1)
     attend_few(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const CacheArgs a) {
   using L = Few<HD>;
-  constexpr int KSTEPS = HD / 16;  // k16 steps of Q·K
-  constexpr int XT = HD / 8;       // column tiles of the output
+  constexpr int KSTEPS = HD / 16;  // k16 steps of K·Q
+  constexpr int XT = HD / 16;      // 16-channel tiles of the output
   extern __shared__ uint8_t few_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(few_smem) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -314,64 +321,66 @@ __global__ void __launch_bounds__(Few<HD>::kWarps * 32, 1)
   unsigned u = 0;
   while (u < units && ok) {
     // ---- an item, or the part of it that this worker has
-    const int per = kRowsFew / a.group;
-    const int first_token = a.starts[at.n] + at.item * per;
-    const int left = a.starts[at.n + 1] - first_token;  // tokens from the item's first on
-    const int rows = min(left, per) * a.group;
-    const int seen0 = at.keys - left;  // keys before the item's own
+    const int first_token = a.starts[at.n], added = a.starts[at.n + 1] - first_token;
+    const int first_row = at.item * kRowsFew;
+    const int rows = min(kRowsFew, added * a.group - first_row);
+    const int seen0 = at.keys - added + first_row / a.group;  // keys before the first row's own
+    const int cached = at.keys - added;
     const int j0 = at.j;
     const int steps = static_cast<int>(min(units - u, static_cast<unsigned>(at.chunks - at.j)));
-    // rows g and g + 8: query times a power of two that puts its largest value in [2^14, 2^15)
-    uint32_t q[KSTEPS][4];
+    // Query row g times a power of two that puts their largest value in [2^14, 2^15),
+    // as the columns of K · Q; scores and outputs come to this thread for rows 2t and 2t + 1.
+    uint32_t q[KSTEPS][2];
     float mul[2];
-    int last[2];  // the last key that each row sees
+    int last[2], last_g;  // the last key that a row sees
+    const int row = g;
+    last_g = cached + (first_row + min(row, rows - 1)) / a.group;
+    uint4 x[HD / 64][2];
+    float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = g + 8 * i;
-      last[i] = seen0 + min(row, rows - 1) / a.group;
-      uint4 x[HD / 64][2];
-      float amax = 0.f;
+    for (int c = 0; c < HD / 64; ++c) {
 #pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
+      for (int k = 0; k < 2; ++k) {
+        x[c][k] = make_uint4(0, 0, 0, 0);
+        if (row < rows)
+          x[c][k] = *reinterpret_cast<const uint4*>(
+              a.query + (first_token + (first_row + row) / a.group) * a.q_token +
+              (at.h * a.group + (first_row + row) % a.group) * a.q_head + (t + 4 * c) * 16 + k * 8);
+        const uint32_t w[4] = {x[c][k].x, x[c][k].y, x[c][k].z, x[c][k].w};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          x[c][k] = make_uint4(0, 0, 0, 0);
-          if (row < rows)
-            x[c][k] = *reinterpret_cast<const uint4*>(
-                a.query + (first_token + row / a.group) * a.q_token +
-                (at.h * a.group + row % a.group) * a.q_head + (t + 4 * c) * 16 + k * 8);
-          const uint32_t w[4] = {x[c][k].x, x[c][k].y, x[c][k].z, x[c][k].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            amax = fmaxf(amax, fabsf(__uint_as_float(w[e] << 16)));
-            amax = fmaxf(amax, fabsf(__uint_as_float(w[e] & 0xffff0000u)));
-          }
+        for (int e = 0; e < 4; ++e) {
+          amax = fmaxf(amax, fabsf(__uint_as_float(w[e] << 16)));
+          amax = fmaxf(amax, fabsf(__uint_as_float(w[e] & 0xffff0000u)));
         }
       }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const int up = min(100, 14 + 127 - static_cast<int>(__float_as_uint(amax) >> 23));
-      const float s = exponent_scale(up);
-      mul[i] = a.scale_log2 * exponent_scale(-up);
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int up = min(100, 14 + 127 - static_cast<int>(__float_as_uint(amax) >> 23));
+    const float s = exponent_scale(up), back = a.scale_log2 * exponent_scale(-up);
 #pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
+    for (int i = 0; i < 2; ++i) {
+      mul[i] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + i));
+      last[i] = __shfl_sync(0xffffffffu, last_g, 4 * (2 * t + i));
+    }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t w[4] = {x[c][k].x, x[c][k].y, x[c][k].z, x[c][k].w};
+    for (int c = 0; c < HD / 64; ++c) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // words 2i, 2i + 1 of the 8 a chunk: registers {row, row + 8} × {low, high} of step i
-            const int word = k * 4 + e;
-            q[c * 4 + word / 2][(word & 1) * 2 + i] =
-                f16_pair(__uint_as_float(w[e] << 16) * s, __uint_as_float(w[e] & 0xffff0000u) * s);
-          }
-        }
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t w[4] = {x[c][k].x, x[c][k].y, x[c][k].z, x[c][k].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)  // words 2i, 2i + 1 of the 8 a chunk are step i's two registers
+          q[c * 4 + (k * 4 + e) / 2][e & 1] =
+              f16_pair(__uint_as_float(w[e] << 16) * s, __uint_as_float(w[e] & 0xffff0000u) * s);
       }
     }
     float o[XT][4];
 #pragma unroll
-    for (int x = 0; x < XT; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int x = 0; x < XT; ++x)
+      o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+    float m[2], l[2];
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
 
     for (int step = 0; step < steps; ++step, ++u) {
       const unsigned f = 2 * u;
@@ -379,20 +388,23 @@ __global__ void __launch_bounds__(Few<HD>::kWarps * 32, 1)
       if (!(ok = __all_sync(0xffffffffu, cache_wait(&full[slot], (f / L::kSlots) & 1, a.status)))) break;
       const float2* scales = meta + (f >> 1) % L::kMeta * 4;
       const int key0 = (j0 + step) * kChunkKeys;
-      // ---- scores
-      float s[8][4];
+      // ---- scores: tile kt of 16 keys; s[..][0, 1]: this lane's key of 8 for rows 2t, 2t + 1;
+      // [2, 3]: the key 8 behind
+      float s[4][4];
 #pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int kt = 0; kt < 4; ++kt) {
+        s[kt][0] = s[kt][1] = s[kt][2] = s[kt][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c) {
-          const uint4 k = lds128(base + slot * L::kSlotBytes + nt * 8 * HD + k_off[c]);
-          const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+          const uint32_t from = base + slot * L::kSlotBytes + kt * 16 * HD + k_off[c];
+          const uint4 lo = lds128(from), hi = lds128(from + 8 * HD);
+          const uint32_t w0[4] = {lo.x, lo.y, lo.z, lo.w}, w1[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            uint32_t b0, b1;
-            widen4(w[e], b0, b1);
-            mma16816(s[nt], q[c * 4 + e], b0, b1);
+            uint32_t k[4];
+            widen4(w0[e], k[0], k[2]);
+            widen4(w1[e], k[1], k[3]);
+            mma16816(s[kt], k, q[c * 4 + e][0], q[c * 4 + e][1]);
           }
         }
       }
@@ -400,67 +412,63 @@ __global__ void __launch_bounds__(Few<HD>::kWarps * 32, 1)
       // the scales are read before the ring of chunks moves on
       float2 sc[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sc[i] = scales[i < per_chunk ? i : 0];
+      for (int i = 0; i < 4; ++i) sc[i] = scales[i >> (box_shift - 4)];
       __syncwarp();
       load(f + L::kSlots);
       bool whole = key0 + kChunkKeys <= seen0 + 1;  // every row sees every key
 #pragma unroll
       for (int i = 0; i < 4; ++i) whole = whole && sc[i].x != 0.f;
-      float top[2] = {m[0], m[1]};
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        const float2 x = per_chunk == 4 ? sc[nt / 2] : per_chunk == 2 ? sc[nt / 4] : sc[0];
-        const float f0 = mul[0] * x.x, f1 = mul[1] * x.x;
-        s[nt][0] = fmaf(s[nt][0], f0, x.y);
-        s[nt][1] = fmaf(s[nt][1], f0, x.y);
-        s[nt][2] = fmaf(s[nt][2], f1, x.y);
-        s[nt][3] = fmaf(s[nt][3], f1, x.y);
-        if (!whole) {
-          const int ka = key0 + nt * 8 + row0, kb = key0 + nt * 8 + row1;
-          const bool gone = x.x == 0.f;
-          if (gone || ka > last[0]) s[nt][0] = -INFINITY;
-          if (gone || kb > last[0]) s[nt][1] = -INFINITY;
-          if (gone || ka > last[1]) s[nt][2] = -INFINITY;
-          if (gone || kb > last[1]) s[nt][3] = -INFINITY;
-        }
-        top[0] = fmaxf(top[0], fmaxf(s[nt][0], s[nt][1]));
-        top[1] = fmaxf(top[1], fmaxf(s[nt][2], s[nt][3]));
-      }
+      float top[2];
+      bool grew = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+        float most = m[i];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          const float f0 = mul[i] * sc[kt].x;
+          float& near = s[kt][i];
+          float& far = s[kt][2 + i];
+          near = fmaf(near, f0, sc[kt].y);
+          far = fmaf(far, f0, sc[kt].y);
+          if (!whole) {
+            const int key = key0 + kt * 16 + order;
+            const bool gone = sc[kt].x == 0.f;
+            if (gone || key > last[i]) near = -INFINITY;
+            if (gone || key + 8 > last[i]) far = -INFINITY;
+          }
+          most = fmaxf(most, fmaxf(near, far));
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        top[i] = most;
+        grew |= most > m[i];
       }
-      if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-        float w[2];
+      if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          w[i] = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - top[i]);
-          l[i] *= w[i];
+          const float w = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - top[i]);
+          l[i] *= w;
           m[i] = top[i];
-        }
 #pragma unroll
-        for (int x = 0; x < XT; ++x) {
-          o[x][0] *= w[0];
-          o[x][1] *= w[0];
-          o[x][2] *= w[1];
-          o[x][3] *= w[1];
+          for (int x = 0; x < XT; ++x) {
+            o[x][i] *= w;
+            o[x][2 + i] *= w;
+          }
         }
       }
+      // weights 2^(s + e - m), their sum without the value's 2^e; p: a thread a row (g)
+      uint32_t p[4][2];
       const float r0 = (m[0] == -INFINITY ? 0.f : m[0]) - kFewBias;
       const float r1 = (m[1] == -INFINITY ? 0.f : m[1]) - kFewBias;
-      // weights 2^(s + e - m), their sum without the value's 2^e
-      uint32_t p[4][4];
 #pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        const float2 x = per_chunk == 4 ? sc[nt / 2] : per_chunk == 2 ? sc[nt / 4] : sc[0];
-        const float back = exponent_scale(-static_cast<int>(x.y));
-        const float p0 = ex2_approx(s[nt][0] - r0), p1 = ex2_approx(s[nt][1] - r0);
-        const float p2 = ex2_approx(s[nt][2] - r1), p3 = ex2_approx(s[nt][3] - r1);
-        l[0] = fmaf(p0 + p1, back, l[0]);
-        l[1] = fmaf(p2 + p3, back, l[1]);
-        p[nt / 2][(nt & 1) * 2] = f16_pair(p0, p1);
-        p[nt / 2][(nt & 1) * 2 + 1] = f16_pair(p2, p3);
+      for (int kt = 0; kt < 4; ++kt) {
+        const float back = exponent_scale(-static_cast<int>(sc[kt].y));
+        const float p0 = ex2_approx(s[kt][0] - r0), p1 = ex2_approx(s[kt][1] - r1);
+        const float p2 = ex2_approx(s[kt][2] - r0), p3 = ex2_approx(s[kt][3] - r1);
+        l[0] = fmaf(p0 + p2, back, l[0]);
+        l[1] = fmaf(p1 + p3, back, l[1]);
+        p[kt][0] = transposed(f16_pair(p0, p1));
+        p[kt][1] = transposed(f16_pair(p2, p3));
       }
       // ---- values
       slot = (f + 1) % L::kSlots;
@@ -488,8 +496,7 @@ __global__ void __launch_bounds__(Few<HD>::kWarps * 32, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int at16 = kk * 16 + (i >> 1) * 8 + ((i & 1) ? row1 : row0);
-            const float2 x = per_chunk == 4 ? sc[kk] : per_chunk == 2 ? sc[kk / 2] : sc[0];
-            const bool gone = x.x == 0.f || key0 + at16 >= at.keys;
+            const bool gone = sc[kk].x == 0.f || key0 + at16 >= at.keys;
 #pragma unroll
             for (int w = 0; w < WORDS; ++w) {
               if (gone) v[i][w] = 0;
@@ -497,18 +504,16 @@ __global__ void __launch_bounds__(Few<HD>::kWarps * 32, 1)
             }
           }
           if (__any_sync(0xffffffffu, any != 0)) {
-            uint32_t see[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {  // a row's keys of the two column pairs
-              const int k = key0 + kk * 16 + (i >> 1) * 8, to_row = last[i & 1];
-              see[i] = f16_pair(k + row0 <= to_row ? 1.f : 0.f, k + row1 <= to_row ? 1.f : 0.f);
-            }
+            const int k = key0 + kk * 16, to_row = last_g;
+            const uint32_t see0 = f16_pair(k + row0 <= to_row ? 1.f : 0.f, k + row1 <= to_row ? 1.f : 0.f);
+            const uint32_t see1 = f16_pair(k + 8 + row0 <= to_row ? 1.f : 0.f, k + 8 + row1 <= to_row ? 1.f : 0.f);
 #pragma unroll
             for (int x = 0; x < XT; ++x) {
-              const int w = x / 4, sh = (x & 3) * 8;
-              auto one = [&](int i) { return (nan_bytes(v[i][w]) >> sh & 0xffu) ? 0x3c00u : 0u; };
+              auto one = [&](int i, int c) { return (nan_bytes(v[i][c / 4]) >> (c & 3) * 8 & 0xffu) ? 0x3c00u : 0u; };
+              const uint32_t n[4] = {one(0, 2 * x) | one(1, 2 * x) << 16, one(0, 2 * x + 1) | one(1, 2 * x + 1) << 16,
+                                     one(2, 2 * x) | one(3, 2 * x) << 16, one(2, 2 * x + 1) | one(3, 2 * x + 1) << 16};
               float hit[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816(hit, see, one(0) | one(1) << 16, one(2) | one(3) << 16);
+              mma16816(hit, n, see0, see1);
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 if (hit[i] > 0.f) o[x][i] = __uint_as_float(0x7fc00000u);
@@ -521,52 +526,49 @@ __global__ void __launch_bounds__(Few<HD>::kWarps * 32, 1)
         }
 #pragma unroll
         for (int w = 0; w < WORDS; ++w) {
-          uint32_t b0[4], b1[4];
-          widen4(__byte_perm(v[0][w], v[1][w], 0x5140), b0[0], b0[1]);
-          widen4(__byte_perm(v[0][w], v[1][w], 0x7362), b0[2], b0[3]);
-          widen4(__byte_perm(v[2][w], v[3][w], 0x5140), b1[0], b1[1]);
-          widen4(__byte_perm(v[2][w], v[3][w], 0x7362), b1[2], b1[3]);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) mma16816(o[w * 4 + x], p[kk], b0[x], b1[x]);
+          uint32_t x0[4], x1[4];  // channels 4w, 4w + 1 and 4w + 2, 4w + 3 of this lane's
+          widen4(__byte_perm(v[0][w], v[1][w], 0x5140), x0[0], x0[1]);
+          widen4(__byte_perm(v[2][w], v[3][w], 0x5140), x0[2], x0[3]);
+          widen4(__byte_perm(v[0][w], v[1][w], 0x7362), x1[0], x1[1]);
+          widen4(__byte_perm(v[2][w], v[3][w], 0x7362), x1[2], x1[3]);
+          mma16816(o[2 * w], x0, p[kk][0], p[kk][1]);
+          mma16816(o[2 * w + 1], x1, p[kk][0], p[kk][1]);
         }
       }
       __syncwarp();
       load(f + 1 + L::kSlots);
     }
     if (!ok) break;
-    // ---- the item's end: this thread has channels [t · HD / 4, + HD / 4) of rows g and g + 8
+    // ---- the item's end: this thread has channels [g · HD / 8, + HD / 8) of rows 2t and 2t + 1
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      const int row = g + 8 * i;
+      float sum = l[i];
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const int row = 2 * t + i;
       if (row >= rows) continue;
       if (steps == at.chunks) {
-        const int token = first_token + row / a.group, head = at.h * a.group + row % a.group;
-        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-        uint4* to_row = reinterpret_cast<uint4*>(a.out + token * a.o_token + head * a.o_head + t * (HD / 4));
+        const int token = first_token + (first_row + row) / a.group;
+        const int head = at.h * a.group + (first_row + row) % a.group;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        uint4* to_row = reinterpret_cast<uint4*>(a.out + token * a.o_token + head * a.o_head + g * (HD / 8));
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int x = 0; x < XT; x += 8)
-            to_row[(c * XT + x) / 8] = make_uint4(
-                pack_bf16x2(o[x][2 * i + c] * inv, o[x + 1][2 * i + c] * inv),
-                pack_bf16x2(o[x + 2][2 * i + c] * inv, o[x + 3][2 * i + c] * inv),
-                pack_bf16x2(o[x + 4][2 * i + c] * inv, o[x + 5][2 * i + c] * inv),
-                pack_bf16x2(o[x + 6][2 * i + c] * inv, o[x + 7][2 * i + c] * inv));
-        if (a.lse != nullptr && t == 0)
+        for (int x = 0; x < XT; x += 4)
+          to_row[x / 4] = make_uint4(
+              pack_bf16x2(o[x][i] * inv, o[x][2 + i] * inv),
+              pack_bf16x2(o[x + 1][i] * inv, o[x + 1][2 + i] * inv),
+              pack_bf16x2(o[x + 2][i] * inv, o[x + 2][2 + i] * inv),
+              pack_bf16x2(o[x + 3][i] * inv, o[x + 3][2 + i] * inv));
+        if (a.lse != nullptr && g == 0)
           a.lse[static_cast<long long>(token) * a.heads_kv * a.group + head] =
-              l[i] == 0.f ? -INFINITY : 0.6931471805599453f * (m[i] - kFewBias + __log2f(l[i]));
+              sum == 0.f ? -INFINITY : 0.6931471805599453f * (m[i] - kFewBias + __log2f(sum));
       } else {
         const long long part = (2LL * worker + (j0 == 0 ? 1 : 0)) * kRowsFew + row;
-        float4* to_row = reinterpret_cast<float4*>(a.ws_o + part * HD + t * (HD / 4));
+        float4* to_row = reinterpret_cast<float4*>(a.ws_o + part * HD + g * (HD / 8));
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int x = 0; x < XT; x += 4)
-            to_row[(c * XT + x) / 4] = make_float4(o[x][2 * i + c], o[x + 1][2 * i + c],
-                                                   o[x + 2][2 * i + c], o[x + 3][2 * i + c]);
-        if (t == 0) a.ws_ml[part] = make_float2(m[i], l[i]);
+        for (int x = 0; x < XT; x += 2)
+          to_row[x / 2] = make_float4(o[x][i], o[x][2 + i], o[x + 1][i], o[x + 1][2 + i]);
+        if (g == 0) a.ws_ml[part] = make_float2(m[i], sum);
       }
     }
     at.j += steps - 1;
@@ -590,19 +592,18 @@ __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
   __shared__ float sum_o[8][HD];
   __shared__ float warp_top[8], warp_sum[8];
   const int n = blockIdx.x / a.heads_kv, h = blockIdx.x % a.heads_kv;
-  const int per = kRowsFew / a.group, item = blockIdx.y / (per * a.group), row = blockIdx.y % (per * a.group);
+  const int item = blockIdx.y / kRowsFew, row = blockIdx.y % kRowsFew;
   const int start = a.starts[n], next = a.starts[n + 1], length = a.lengths[n];
   const long long before = a.units_few[n], behind = a.units_few[n + 1], all = a.units_few[a.requests];
-  const int first_token = start + item * per;
-  const int rows = behind == before ? 0 : (next - first_token) * a.group;
-  const int items = (next - start + per - 1) / per;
+  const int rows = behind == before ? 0 : (next - start) * a.group;
+  const int items = (rows + kRowsFew - 1) / kRowsFew;
   const long long chunks = (length + kChunkKeys - 1) / kChunkKeys;
   const long long total = all * a.heads_kv;
   const long long workers = min(static_cast<long long>(a.workers), total);
   const long long u0 = before * a.heads_kv + (static_cast<long long>(h) * items + item) * chunks;
   const int first = total == 0 ? 0 : static_cast<int>(quotient((u0 + 1) * workers - 1, total));
   const int last = total == 0 ? 0 : static_cast<int>(quotient((u0 + chunks) * workers - 1, total));
-  const bool split = row < rows && first != last;
+  const bool split = static_cast<int>(blockIdx.y) < rows && first != last;
   // one block at least waits, so that this grid does not end before the one it follows
   if (split || (blockIdx.x == 0 && blockIdx.y == 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!split) return;
@@ -670,7 +671,7 @@ __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
     value += sum_o[w][d];
     sum += warp_sum[w];
   }
-  const int token = first_token + row / a.group, head = h * a.group + row % a.group;
+  const int token = start + blockIdx.y / a.group, head = h * a.group + blockIdx.y % a.group;
   a.out[token * a.o_token + head * a.o_head + d] = __float2bfloat16(sum == 0.f ? 0.f : value / sum);
   if (a.lse != nullptr && d == 0)
     a.lse[static_cast<long long>(token) * a.heads_kv * a.group + head] =
@@ -1676,7 +1677,7 @@ static size_t many_bytes(int head_dim) {
 }
 
 // Which kernels a step needs, as far as the host knows: some request may have few rows, or many.
-static bool may_be_few(const CozyCachePlan& p) { return p.group <= kRowsFew; }
+static bool may_be_few(const CozyCachePlan& p) { return few_rows(p.group, 1); }
 static bool may_be_many(const CozyCachePlan& p) { return !few_rows(p.group, p.longest); }
 
 long long cache_workspace(const CozyCachePlan& p, const CozyCacheStore& c) {
@@ -1788,10 +1789,8 @@ int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyC
     a.ws_o = reinterpret_cast<float*>(space);
     a.ws_ml = reinterpret_cast<float2*>(a.ws_o + few_workers(c.head_dim) * 2 * kRowsFew * c.head_dim);
     space += few_bytes(c.head_dim);
-    // rows that an item of few rows can have: whole tokens
-    const int per = kRowsFew / p.group;
-    const long long tokens = p.longest < kFewItems * per ? p.longest : kFewItems * per;
-    const int rows = static_cast<int>(tokens) * p.group;
+    const int rows = static_cast<int>(std::min(static_cast<long long>(p.group) * p.longest,
+                                               static_cast<long long>(kRowsFew * kFewItems)));
     const int r = c.head_dim == 64 ? few_launch<64>(c, a, rows, stream) : few_launch<128>(c, a, rows, stream);
     if (r) return r;
   }

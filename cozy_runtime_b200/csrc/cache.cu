@@ -232,13 +232,14 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const CozyCach
   }
 }
 
-static int plan_check(const CozyCachePlan& p) {
+int cache_plan_check(const CozyCachePlan& p) {
   if (p.requests < 1 || p.requests > COZY_CACHE_MAX_REQUESTS || p.width < 1 || p.pages < 1)
     return cudaErrorInvalidValue;
   if (p.page != 16 && p.page != 32 && p.page != 64 && p.page != 128) return cudaErrorNotSupported;
   if (p.tokens < 0 || p.longest < 0 || p.group < 1 || p.table_stride < p.width)
     return cudaErrorInvalidValue;
-  if (static_cast<long long>(p.width) * p.page > 0x7fffffffLL) return cudaErrorInvalidValue;
+  // positions, and those up to a tile behind them, in 31 bits
+  if (static_cast<long long>(p.width) * p.page > (1LL << 30)) return cudaErrorInvalidValue;
   if (p.group > COZY_CACHE_MAX_GROUP) return cudaErrorNotSupported;
   const void* ptrs[] = {p.lengths, p.added, p.table, p.free_ring, p.cursor, p.lengths_after,
                         p.starts, p.cursor_after, p.units, p.status};
@@ -253,7 +254,7 @@ static int plan_check(const CozyCachePlan& p) {
 }
 
 int cache_plan(const CozyCachePlan& p, cudaStream_t stream) {
-  const int e = plan_check(p);
+  const int e = cache_plan_check(p);
   if (e) return e;
   const size_t smem = 4 * sizeof(int) * (static_cast<size_t>(p.requests) + 1);
   static bool configured[64] = {};
@@ -593,9 +594,9 @@ int cache_store_check(const CozyCacheStore& c, const CozyCachePlan& p) {
 
 int cache_append(const CozyCachePlan& p, const CozyCacheStore& c, const CozyCacheAppend& x,
                  cudaStream_t stream) {
-  int e = plan_check(p);
+  int e = cache_plan_check(p);
   if (e || (e = cache_store_check(c, p))) return e;
-  if (p.tokens == 0) return cudaSuccess;
+  if (p.tokens == 0 || p.longest == 0) return cudaSuccess;  // nobody brings a token
   AppendArgs a = {};
   a.blocks = reinterpret_cast<const int4*>(p.blocks);
   a.positions = p.positions;

@@ -21,6 +21,7 @@
 
 namespace cozy {
 
+int cache_plan_check(const CozyCachePlan& p);
 int cache_store_check(const CozyCacheStore& c, const CozyCachePlan& p);
 
 // What both kernels read: the plan's answers, the pool and the call.
@@ -1743,10 +1744,10 @@ static int many_launch(const CozyCacheStore& c, CacheArgs& a, cudaStream_t strea
 
 int cache_attention(const CozyCachePlan& p, const CozyCacheStore& c, const CozyCacheAttend& x,
                     cudaStream_t stream) {
-  const int e = cache_store_check(c, p);
-  if (e) return e;
-  if (p.tokens == 0) return cudaSuccess;
-  if (!(x.scale > 0.f) || x.scale > 3.0e38f) return cudaErrorInvalidValue;
+  int e = cache_plan_check(p);
+  if (e || (e = cache_store_check(c, p))) return e;
+  if (!(x.scale > 0.f) || x.scale > 2.0e38f) return cudaErrorInvalidValue;
+  if (p.tokens == 0 || p.longest == 0) return cudaSuccess;  // nobody brings a token
   const void* ptrs[] = {x.query, x.out};
   for (const void* ptr : ptrs)
     if (ptr == nullptr || reinterpret_cast<uintptr_t>(ptr) % 16) return cudaErrorInvalidValue;

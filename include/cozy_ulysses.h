@@ -471,7 +471,8 @@ COZY_API int cozy_ulysses_layer_end(CozyGroup* group, const CozyLayerCall* call,
  * brings added[n] new ones (0: none; -1: it is finished and its pages are released). Free page
  * numbers are the entries [cursor[0], cursor[1]) of a ring of `pages` entries (taken modulo
  * pages). Requests are given pages in order, from the ring's head; released pages go behind its
- * tail, to be given from the next plan on. Rows of the step's tokens: request n's are
+ * tail, to be given from the next plan on (every page of the row: a host that lets requests share
+ * pages counts them itself). Rows of the step's tokens: request n's are
  * [starts[n], starts[n + 1]); rows behind the last belong to nobody.
  * Writes the table (fresh entries only), the ring (behind the tail only), and the outputs;
  * lengths, added and cursor stay as they were, so the same plan can be made again.
@@ -488,7 +489,7 @@ typedef struct CozyCachePlan {
   long long table_stride;
   int* free_ring;          /* [pages] */
   const long long* cursor; /* [2] head, tail */
-  int requests, width, pages, page; /* page: 16, 32, 64 or 128 tokens */
+  int requests, width, pages, page; /* page: 16, 32, 64 or 128 tokens; width * page <= 2^30 */
   int tokens;              /* rows of the step's tensors */
   int longest;             /* no request brings more new tokens */
   int group;               /* query heads per key/value head, at most COZY_CACHE_MAX_GROUP */

@@ -63,12 +63,17 @@ def test_c_entries_refuse_without_a_gpu():
             setattr(p, name, value)
         return p
 
+    whole = _lib.CacheStore(1 << 20, 1 << 20, 1 << 20, 1 << 20, 9, 2, 16, 64)
+    bad_plan = (("cozy_cache_plan", ()),
+                ("cozy_cache_append", (ctypes.byref(whole), ctypes.byref(_lib.CacheAppend()))),
+                ("cozy_cache_attention", (ctypes.byref(whole), ctypes.byref(_lib.CacheAttend()))))
     for change, code in (({"requests": 0}, 1), ({"requests": 8193}, 1), ({"width": 0}, 1), ({"pages": 0}, 1),
                          ({"page": 48}, 801), ({"page": 0}, 801), ({"group": 0}, 1), ({"group": 129}, 801),
                          ({"tokens": -1}, 1), ({"longest": -1}, 1), ({"table_stride": 2}, 1), ({"max_blocks": 3}, 1),
                          ({"blocks": (1 << 20) + 8}, 1), ({"status": 0}, 1), ({"slots": 0}, 1),
                          ({"width": 1 << 28}, 1)):
-        assert lib.cozy_cache_plan(ctypes.byref(plan(**change)), 0) == code, change
+        for entry, more in bad_plan:
+            assert getattr(lib, entry)(ctypes.byref(plan(**change)), *more, 0) == code, (entry, change)
 
     def store(**change):
         s = _lib.CacheStore(1 << 20, 1 << 20, 1 << 20, 1 << 20, 9, 2, 16, 64)

@@ -581,6 +581,40 @@ def test_calls_side_by_side_on_two_streams(new):
         assert all(torch.equal(want, x) for x in got)
 
 
+def test_a_step_that_brings_nothing_with_rows_to_spare():
+    from cozy_runtime_b200 import cache
+
+    layout = cache.Layout(4, 2, 64, 16)
+    m = make([5, 0], [0, 0], 16, torch.Generator().manual_seed(1), tokens=7)
+    for longest in (0, 1, 60):
+        m["longest"] = longest
+        step, _ = on_gpu(m, layout)
+        store = cache.Cache.empty(layout, step.pages)
+        q, k = (torch.ones(7, h, 64, dtype=torch.bfloat16, device="cuda") for h in (4, 2))
+        assert cache.append(store, step, k, k, query=q, out=q).data_ptr() == q.data_ptr()
+        out = cache.attention(store, step, q, out=torch.full_like(q, 3))
+        assert (q == 1).all() and (out == 3).all()
+        step.check()
+
+
+def test_append_in_place():
+    from cozy_runtime_b200 import cache, rope
+
+    g = torch.Generator().manual_seed(2)
+    layout = cache.Layout(6, 2, 128, 16)
+    m = make([5, 40], [20, 3], 16, g)
+    step, t = on_gpu(m, layout)
+    store = cache.Cache.empty(layout, step.pages)
+    spec = rope.llama(t["table"].shape[1] * 16, 128).to("cuda")
+    qkv = torch.randn(23, 10, 128, generator=g).to(torch.bfloat16).cuda()
+    want = cache.append(store, step, qkv[:, 6:8], qkv[:, 8:], query=qkv[:, :6], rope=spec)
+    rest = qkv[:, 6:].clone()
+    got = cache.append(store, step, qkv[:, 6:8], qkv[:, 8:], query=qkv[:, :6], rope=spec, out=qkv[:, :6])
+    assert torch.equal(got, want) and torch.equal(qkv[:, 6:], rest)
+    with pytest.raises(ValueError):
+        cache.append(store, step, qkv[:, 6:8], qkv[:, 8:], query=qkv[:, :6], rope=spec, out=qkv[:, 1:7])
+
+
 def test_an_empty_step():
     from cozy_runtime_b200 import cache
 

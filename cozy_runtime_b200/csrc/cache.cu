@@ -440,7 +440,7 @@ __device__ __forceinline__ int exponent_of(float amax) {
 constexpr int kHeadsAThread = 4;
 
 template <int HD, int WARPS, int PASSES>
-__global__ void __launch_bounds__(256, 3) cache_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a) {
   constexpr int CHUNKS = HD / 8;         // threads a row
   constexpr int ROWS = 32 / CHUNKS;      // rows a warp and pass
   constexpr int UNITS = 8 / WARPS;       // units a CTA

@@ -1242,8 +1242,16 @@ __global__ void __launch_bounds__(512, 1)
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const long long part = 2LL * blockIdx.x + (at.j == 0 ? 1 : 0);
         const int head = at.h * a.group + row - (token - first_token) * a.group;
-        // whole rows leave through the tile's Q (free now, and of the same size), HD / 8 lanes a row
-        const uint32_t stage = smem_u32(smem + L::kQOffset + s * 2 * L::kCodeTile) + (warp & 3) * 32 * HD * 2;
+        // Whole rows leave through the tile's Q (free now, and of the same size), HD / 8 lanes a
+        // row. A row takes the bytes of its own two parts, which only its warp writes: the tile's
+        // other warps may be at the next item's Q already, or still at this one's rows. Chunk j
+        // stands where Q has it, so no two lanes of eight meet in a bank.
+        const uint32_t stage = smem_u32(smem + L::kQOffset + s * 2 * L::kCodeTile);
+        auto staged = [&](int r128, int j) {
+          constexpr int CODES = HD / 16;  // chunks of a row of codes
+          const uint32_t at = stage + (j / CODES) * L::kCodeTile + r128 * HD;
+          return at + (((j % CODES) ^ (HD == 128 ? r128 & 7 : r128 >> 1 & 3)) << 4);
+        };
         float4* ws = reinterpret_cast<float4*>(a.ws_o) + part * (HD / 4) * kRowsMany + row;
         const uint4 p = *poison;
         const bool nan = (p.x | p.y | p.z | p.w) != 0;
@@ -1267,8 +1275,7 @@ __global__ void __launch_bounds__(512, 1)
               for (int k = 0; k < 4; ++k)
                 w[k] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * k]) * inv,
                                    __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-              // chunk j of row r at j ^ (r mod 8): no two lanes of eight in a bank
-              sts128(stage + lane * HD * 2 + (((c * 4 + i) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+              sts128(staged(row128, c * 4 + i), make_uint4(w[0], w[1], w[2], w[3]));
             }
           } else if (row < rows) {
 #pragma unroll
@@ -1284,9 +1291,9 @@ __global__ void __launch_bounds__(512, 1)
           __syncwarp();
 #pragma unroll 4
           for (int i = 0; i < LANES; ++i) {
-            const int r32 = i * ROWS + lane / LANES, j = lane % LANES;
-            const int r = s * 128 + (warp & 3) * 32 + r32;
-            const uint4 v = lds128(stage + r32 * HD * 2 + ((j ^ (r32 & 7)) << 4));
+            const int r128 = (warp & 3) * 32 + i * ROWS + lane / LANES, j = lane % LANES;
+            const int r = s * 128 + r128;
+            const uint4 v = lds128(staged(r128, j));
             const int of = row_token(a, r);
             if (r < rows)
               *reinterpret_cast<uint4*>(a.out + (first_token + of) * a.o_token +

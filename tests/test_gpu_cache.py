@@ -339,6 +339,30 @@ def test_attention_over_long_contexts(lengths, new, page, hq, hkv, dim):
     check_attention(out, lse, want, m["tokens"], floor_of(max(lengths) + max(new), ve))
 
 
+@pytest.mark.parametrize("dim,hq", [(64, 20), (128, 20), (128, 24)])
+def test_attention_of_many_short_items(dim, hq):
+    """Items of one and two query tiles that follow one another in a worker, each with its output
+    staged where the next one's queries come: every repetition gives the same bits."""
+    from cozy_runtime_b200 import cache
+
+    hkv, page, requests = 4, 16, 240
+    g = torch.Generator().manual_seed(dim + hq)
+    lengths = torch.randint(0, 200, (requests,), generator=g).tolist()
+    new = torch.randint(7, 60, (requests,), generator=g).tolist()
+    m = make(lengths, new, page, g)
+    step, t = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    k, ke = fill(step.pages, hkv, page, dim, g)
+    v, ve = fill(step.pages, hkv, page, dim, g)
+    q = torch.randn(m["tokens"], hq, dim, generator=g).to(torch.bfloat16)
+    store, mine = store_on_gpu(k, ke, v, ve), q.cuda()
+    out, lse = cache.attention(store, step, mine, return_lse=True)
+    want = law.attend_step(values(k, ke), values(v, ve), t["table"].tolist(), lengths, new, q, page, dim**-0.5)
+    check_attention(out, lse, want, m["tokens"], floor_of(300, ve))
+    for _ in range(200):
+        again, again_lse = cache.attention(store, step, mine, return_lse=True)
+        assert torch.equal(again, out) and torch.equal(again_lse, lse)
+
+
 @pytest.mark.parametrize("lengths,new,hq,hkv,dim", [
     ([100, 30], [1, 1], 4, 2, 128), ([100, 30], [5, 3], 2, 1, 64), ([100, 30], [150, 90], 4, 2, 128),
     ([100, 30], [150, 90], 3, 1, 64),

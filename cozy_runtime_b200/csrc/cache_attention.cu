@@ -1129,7 +1129,13 @@ __global__ void __launch_bounds__(512, 1)
         for (int h = 0; h < halves; ++h) {
           const int b = h & 1, tile = block + (h >> 1), slot = tile % L::kScaleRing;
           const int tile_key0 = key0 + (h >> 1) * kTileKeys, half_key0 = tile_key0 + b * 64;
-          // the scales are there long before the scores
+          // The scales are there long before the scores. Not so for an item's first tile: rows that
+          // skipped items may be far ahead of the copies, and a parity two phases ahead reads as
+          // complete; its scores have arrived only behind its scales.
+          if (h == 0 && !many_wait(&s_full[2 * s], phase & 1, abort, a.status)) {
+            ok = false;
+            break;
+          }
           const float* scales =
               reinterpret_cast<const float*>(smem + L::kScaleOffset + slot * L::kScaleBytes) + b * 4;
           if (b == 0 && !many_wait(&scale_full[slot], (tile / L::kScaleRing) & 1, abort, a.status)) {
@@ -1144,7 +1150,7 @@ __global__ void __launch_bounds__(512, 1)
             back_of[c] = scales[16 + c * (4 / GROUPS)];
           }
           const int gone = reinterpret_cast<const int*>(scales)[24 - b * 4];
-          if (!many_wait(&s_full[2 * s + b], phase >> b & 1, abort, a.status)) {
+          if (h > 0 && !many_wait(&s_full[2 * s + b], phase >> b & 1, abort, a.status)) {
             ok = false;
             break;
           }

@@ -363,6 +363,31 @@ def test_attention_of_many_short_items(dim, hq):
         assert torch.equal(again, out) and torch.equal(again_lse, lse)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_whose_second_query_tile_skips_items(dim):
+    """Workers whose items are of one query tile for many tiles of keys, then of two: the second
+    tile's rows meet the scales of their own keys."""
+    from cozy_runtime_b200 import cache
+
+    hq, hkv, page, requests = 2, 2, 16, 200
+    g = torch.Generator().manual_seed(dim)
+    lengths = torch.randint(300, 700, (requests,), generator=g).tolist()
+    new = [142 if n % 13 == 12 else 30 + n % 60 for n in range(requests)]
+    m = make(lengths, new, page, g)
+    step, t = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    k, ke = fill(step.pages, hkv, page, dim, g)
+    v, ve = fill(step.pages, hkv, page, dim, g)
+    q = torch.randn(m["tokens"], hq, dim, generator=g).to(torch.bfloat16)
+    store, mine, table = store_on_gpu(k, ke, v, ve), q.cuda(), t["table"].tolist()
+    two = [n for n in range(requests) if new[n] > 128]
+    rows = torch.cat([sum(new[:n]) + torch.arange(new[n]) for n in two])
+    want = law.attend_step(values(k, ke), values(v, ve), [table[n] for n in two], [lengths[n] for n in two],
+                           [new[n] for n in two], q[rows], page, dim**-0.5)
+    for _ in range(5):
+        out, lse = cache.attention(store, step, mine, return_lse=True)
+        check_attention(out[rows], lse[rows], want, len(rows), floor_of(850, ve))
+
+
 @pytest.mark.parametrize("lengths,new,hq,hkv,dim", [
     ([100, 30], [1, 1], 4, 2, 128), ([100, 30], [5, 3], 2, 1, 64), ([100, 30], [150, 90], 4, 2, 128),
     ([100, 30], [150, 90], 3, 1, 64),

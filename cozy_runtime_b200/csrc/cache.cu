@@ -367,7 +367,8 @@ __device__ __forceinline__ void ready_row(float (&x)[8], int d0, unsigned mask, 
   if (!a.rotate || a.rope.rotary == 0) return;
   if (a.rope.interleaved) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {  // pairs behind the rotated ones have cos 1, sin 0
+    for (int i = 0; i < 4; ++i) {
+      if (d0 + 2 * i >= a.rope.rotary) break;  // channels of their own: an infinity stays in its place
       const float lo = x[2 * i], hi = x[2 * i + 1];
       x[2 * i] = lo * turn.c[i] - hi * turn.s[i];
       x[2 * i + 1] = hi * turn.c[i] + lo * turn.s[i];

@@ -220,6 +220,36 @@ def test_append_matches_the_law(lengths, new, page, hq, hkv, dim, norm, rotary, 
     step.check()
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_keeps_what_is_not_finite_to_its_pair(interleaved):
+    """NaN and infinities reach the channels that the rotation pairs them with, no others."""
+    from cozy_runtime_b200 import cache, rope
+
+    dim, rotary, page, hkv, tokens = 64, 32, 16, 2, 5
+    g = torch.Generator().manual_seed(14)
+    m = make([3], [tokens], page, g)
+    step, t = on_gpu(m, cache.Layout(4, hkv, dim, page))
+    columns = rotary // 2 if interleaved else rotary
+    angle = torch.rand(t["table"].shape[1] * page, columns, generator=g) + 0.3
+    spec = rope.RopeSpec(angle.cos().cuda(), angle.sin().cuda(), columns, 1, rotary, interleaved)
+    x = torch.randn(tokens, 4, dim, generator=g).to(torch.bfloat16)
+    spots = {0: math.inf, 1: math.nan, 9: -math.inf, 33: math.inf, 40: math.nan, 63: -math.inf}
+    touched = torch.zeros(dim, dtype=torch.bool)
+    for d, v in spots.items():
+        x[2, 1, d] = v
+        other = d if d >= rotary else d ^ 1 if interleaved else (d + rotary // 2) % rotary
+        touched[[d, other]] = True
+    k, ke = fill(step.pages, hkv, page, dim, g)
+    store = store_on_gpu(k, ke, k, ke)
+    out = cache.append(store, step, x[:, :hkv].cuda(), x[:, :hkv].cuda(), query=x.cuda(), rope=spec)
+    clean = torch.ones(tokens, 4, dim, dtype=torch.bool)
+    clean[2, 1] = ~touched
+    assert torch.equal(out.isfinite().cpu(), clean)
+    slot = int(step.slots[2])
+    stored = store.key[slot // page, :, slot % page].float().cpu()
+    assert torch.equal(stored.isnan(), ~clean[2, :hkv])
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_append_grows_a_block_token_by_token(dim):
     """A block filled by single tokens of growing and shrinking size: its exponent grows only, and

@@ -291,7 +291,7 @@ int cache_plan(const CozyCachePlan& p, cudaStream_t stream) {
 // HBM bounds the long form: a token reads (Hq + 2 Hkv) · D bf16 and writes Hq · D bf16 and
 // 2 · Hkv · D codes.
 struct AppendTensor {
-  int normalize;
+  int normalize, wide;  // wide: the weights can be read 16 bytes at a time
   const float* norm_weight;
   float norm_offset, norm_eps;
 };
@@ -313,45 +313,119 @@ struct AppendArgs {
   unsigned query_ctas;
 };
 
+// The 8 channels of a row that a thread holds: 4 at `low` and 4 at `high`. Split halves: each
+// channel's partner of the rotation beside it, so no shuffle is needed (eight a row and thread
+// cost 7 us of a prompt's 49). Otherwise 8 in a row, in one 16-byte access.
+struct Piece {
+  int low, high, turned;  // turned: rotated pairs, {i, 4 + i} or {2i, 2i + 1}
+};
+
+// APART: split halves are rotated, a row takes two accesses a thread.
+template <bool APART>
+__device__ __forceinline__ Piece piece_at(const AppendArgs& a, int chunk, bool rotate) {
+  const int rotary = rotate ? a.rope.rotary : 0;
+  if constexpr (APART) {
+    if (chunk * 8 < rotary) return {chunk * 4, chunk * 4 + rotary / 2, 4};
+    return {chunk * 8, chunk * 8 + 4, 0};
+  }
+  return {chunk * 8, chunk * 8 + 4, max(0, min(4, rotary / 2 - chunk * 4))};
+}
+
+template <bool APART>
+__device__ __forceinline__ uint4 load_piece(const __nv_bfloat16* row, const Piece& p) {
+  if constexpr (!APART) return *reinterpret_cast<const uint4*>(row + p.low);
+  const uint2 low = *reinterpret_cast<const uint2*>(row + p.low);
+  const uint2 high = *reinterpret_cast<const uint2*>(row + p.high);
+  return make_uint4(low.x, low.y, high.x, high.y);
+}
+
+template <bool APART>
+__device__ __forceinline__ void store_piece(__nv_bfloat16* row, const Piece& p, uint4 v) {
+  if constexpr (APART) {
+    *reinterpret_cast<uint2*>(row + p.low) = make_uint2(v.x, v.y);
+    *reinterpret_cast<uint2*>(row + p.high) = make_uint2(v.z, v.w);
+  } else {
+    *reinterpret_cast<uint4*>(row + p.low) = v;
+  }
+}
+
+template <bool APART>
+__device__ __forceinline__ void store_piece(uint8_t* row, const Piece& p, uint2 v) {
+  if constexpr (APART) {
+    *reinterpret_cast<uint32_t*>(row + p.low) = v.x;
+    *reinterpret_cast<uint32_t*>(row + p.high) = v.y;
+  } else {
+    *reinterpret_cast<uint2*>(row + p.low) = v;
+  }
+}
+
+// Four values of a table or a weight.
+__device__ __forceinline__ void load4(float* to, const float* from, long long stride, bool wide) {
+  if (wide) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(from));
+    to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = __ldg(from + i * stride);
+  }
+}
+
 // A thread's part of the rotation by one position: cos and sin of its 8 channels (split halves),
 // or of its 4 pairs (interleaved, the first 4). Read once for all heads of a token.
 struct Turn {
   float c[8], s[8];
 };
 
-template <int HD>
-__device__ __forceinline__ Turn turn_at(const AppendArgs& a, long long position, int d0) {
+template <bool APART>
+__device__ __forceinline__ Turn turn_at(const AppendArgs& a, long long position, const Piece& p) {
   Turn t;
   const CozyRope& r = a.rope;
   const float* cs = r.cos + position * r.stride_token;
   const float* sn = r.sin + position * r.stride_token;
-  const int first = r.interleaved ? d0 / 2 : d0, count = r.interleaved ? 4 : 8;
-  const int columns = r.interleaved ? r.rotary / 2 : r.rotary;
-  if (a.wide && first + count <= columns) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      if (i >= count) break;
-      const float4 c = __ldg(reinterpret_cast<const float4*>(cs + first + i));
-      const float4 s = __ldg(reinterpret_cast<const float4*>(sn + first + i));
-      t.c[i] = c.x; t.c[i + 1] = c.y; t.c[i + 2] = c.z; t.c[i + 3] = c.w;
-      t.s[i] = s.x; t.s[i + 1] = s.y; t.s[i + 2] = s.z; t.s[i + 3] = s.w;
+  if constexpr (APART) {
+    if (p.turned) {
+      load4(t.c, cs + p.low * r.stride_channel, r.stride_channel, a.wide);
+      load4(t.s, sn + p.low * r.stride_channel, r.stride_channel, a.wide);
+      load4(t.c + 4, cs + p.high * r.stride_channel, r.stride_channel, a.wide);
+      load4(t.s + 4, sn + p.high * r.stride_channel, r.stride_channel, a.wide);
     }
+  } else if (p.turned == 4) {
+    load4(t.c, cs + p.low / 2 * r.stride_channel, r.stride_channel, a.wide);
+    load4(t.s, sn + p.low / 2 * r.stride_channel, r.stride_channel, a.wide);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool in = i < count && first + i < columns;
-      t.c[i] = in ? __ldg(cs + (first + i) * r.stride_channel) : 1.f;
-      t.s[i] = in ? __ldg(sn + (first + i) * r.stride_channel) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      t.c[i] = i < p.turned ? __ldg(cs + (p.low / 2 + i) * r.stride_channel) : 1.f;
+      t.s[i] = i < p.turned ? __ldg(sn + (p.low / 2 + i) * r.stride_channel) : 0.f;
     }
   }
   return t;
 }
 
+// A norm's weights of a thread's channels, the offset in them.
+struct Weights {
+  float w[8];
+};
+
+__device__ __forceinline__ Weights weights_at(const AppendTensor& t, const Piece& p) {
+  Weights w;
+  if (t.normalize && t.norm_weight != nullptr) {
+    load4(w.w, t.norm_weight + p.low, 1, t.wide);
+    load4(w.w + 4, t.norm_weight + p.high, 1, t.wide);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.w[i] += t.norm_offset;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.w[i] = 1.f;
+  }
+  return w;
+}
+
 // Per-head RMSNorm, then the rotation, of a row held 8 channels a thread (the laws of
 // norm_rope.cuh, with the tables' values given): fp32, rounded by the caller.
-template <int HD>
-__device__ __forceinline__ void ready_row(float (&x)[8], int d0, unsigned mask, const AppendTensor& t,
-                                          const AppendArgs& a, const Turn& turn) {
+template <int HD, bool APART>
+__device__ __forceinline__ void ready_row(float (&x)[8], const Piece& p, unsigned mask, const AppendTensor& t,
+                                          const AppendArgs& a, const Turn& turn, const Weights& w) {
   constexpr int CHUNKS = HD / 8;
   if (t.normalize) {
     float ss = 0.f;
@@ -361,29 +435,24 @@ __device__ __forceinline__ void ready_row(float (&x)[8], int d0, unsigned mask, 
     for (int o = CHUNKS / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
     const float inv = rsqrtf(ss / HD + t.norm_eps);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = t.norm_weight ? x[i] * inv * (__ldg(t.norm_weight + d0 + i) + t.norm_offset) : x[i] * inv;
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w.w[i];
   }
-  if (!a.rotate || a.rope.rotary == 0) return;
-  if (a.rope.interleaved) {
+  if constexpr (APART) {
+    if (p.turned) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float lo = x[i], hi = x[4 + i];
+        x[i] = lo * turn.c[i] - hi * turn.s[i];
+        x[4 + i] = hi * turn.c[4 + i] + lo * turn.s[4 + i];
+      }
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (d0 + 2 * i >= a.rope.rotary) break;  // channels of their own: an infinity stays in its place
+      if (i >= p.turned) break;  // channels of their own: an infinity stays in its place
       const float lo = x[2 * i], hi = x[2 * i + 1];
       x[2 * i] = lo * turn.c[i] - hi * turn.s[i];
       x[2 * i + 1] = hi * turn.c[i] + lo * turn.s[i];
-    }
-  } else {
-    // channel j pairs with j ± rotary / 2: whole threads, rotary / 16 of them apart
-    const int half = a.rope.rotary / 16, chunk = d0 / 8, lane = threadIdx.x & 31;
-    const int other = chunk < half ? chunk + half : chunk < 2 * half ? chunk - half : chunk;
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(mask, x[i], lane - chunk + other);
-    if (chunk < 2 * half) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = chunk < half ? x[i] * turn.c[i] - y[i] * turn.s[i] : x[i] * turn.c[i] + y[i] * turn.s[i];
     }
   }
 }
@@ -440,52 +509,50 @@ __device__ __forceinline__ int exponent_of(float amax) {
 // Heads of a token that a thread group readies: the tables' values are read once for them.
 constexpr int kHeadsAThread = 4;
 
-template <int HD, int WARPS, int PASSES>
-__global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a) {
+template <int HD, bool APART>
+__device__ __forceinline__ void append_query(const AppendArgs& a) {
+  constexpr int CHUNKS = HD / 8, ROWS = 32 / CHUNKS;  // threads a row, rows a warp
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunk = lane % CHUNKS, sub = lane / CHUNKS;
+  const unsigned mask = row_group_mask<CHUNKS>();
+  const int sets = (a.heads_q + kHeadsAThread - 1) / kHeadsAThread;
+  const unsigned at = (blockIdx.x * 8 + warp) * ROWS + sub;
+  const int token = at / sets, head0 = at % sets * kHeadsAThread;
+  if (token >= a.tokens) return;
+  const int position = a.positions[token];
+  const Piece p = piece_at<APART>(a, chunk, a.rotate);
+  uint4 v[kHeadsAThread];
+#pragma unroll
+  for (int i = 0; i < kHeadsAThread; ++i)
+    if (head0 + i < a.heads_q)
+      v[i] = load_piece<APART>(a.src[0] + token * a.src_token[0] + (head0 + i) * a.src_head[0], p);
+  if (position < 0) return;
+  Turn turn = {};
+  if (a.rotate) turn = turn_at<APART>(a, position, p);
+  const Weights w = weights_at(a.t[0], p);
+#pragma unroll
+  for (int i = 0; i < kHeadsAThread; ++i) {
+    if (head0 + i >= a.heads_q) break;
+    float x[8];
+    widen8(v[i], x);
+    ready_row<HD, APART>(x, p, mask, a.t[0], a, turn, w);
+    store_piece<APART>(a.out + token * a.out_token + (head0 + i) * a.out_head, p, narrow8(x));
+  }
+}
+
+// READY: the rows are normed or rotated first (keys).
+template <int HD, int WARPS, int PASSES, bool READY, bool APART>
+__device__ __forceinline__ void append_unit(const AppendArgs& a, int which, int head, int4 entry,
+                                            float* largest) {
   constexpr int CHUNKS = HD / 8;         // threads a row
   constexpr int ROWS = 32 / CHUNKS;      // rows a warp and pass
-  constexpr int UNITS = 8 / WARPS;       // units a CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int chunk = lane % CHUNKS, sub = lane / CHUNKS, d0 = chunk * 8;
+  const int chunk = lane % CHUNKS, slot = (warp % WARPS) * ROWS + lane / CHUNKS;
   const unsigned mask = row_group_mask<CHUNKS>();
-
-  if (blockIdx.x < a.query_ctas) {  // queries: some heads of a token a group of threads
-    const int sets = (a.heads_q + kHeadsAThread - 1) / kHeadsAThread;
-    const unsigned at = (blockIdx.x * 8 + warp) * ROWS + sub;
-    const int token = at / sets, head0 = at % sets * kHeadsAThread;
-    if (token >= a.tokens) return;
-    const int position = a.positions[token];
-    uint4 v[kHeadsAThread];
-#pragma unroll
-    for (int i = 0; i < kHeadsAThread; ++i)
-      if (head0 + i < a.heads_q)
-        v[i] = *reinterpret_cast<const uint4*>(a.src[0] + token * a.src_token[0] +
-                                               (head0 + i) * a.src_head[0] + d0);
-    if (position < 0) return;
-    Turn turn = {};
-    if (a.rotate) turn = turn_at<HD>(a, position, d0);
-#pragma unroll
-    for (int i = 0; i < kHeadsAThread; ++i) {
-      if (head0 + i >= a.heads_q) break;
-      float x[8];
-      widen8(v[i], x);
-      ready_row<HD>(x, d0, mask, a.t[0], a, turn);
-      *reinterpret_cast<uint4*>(a.out + token * a.out_token + (head0 + i) * a.out_head + d0) = narrow8(x);
-    }
-    return;
-  }
-
-  __shared__ float largest[8];
-  const long long unit = static_cast<long long>(blockIdx.x - a.query_ctas) * UNITS + warp / WARPS;
-  const int which = static_cast<int>(unit & 1);  // 0 keys, 1 values
-  const int head = static_cast<int>((unit >> 1) % a.heads_kv);
-  const long long at = (unit >> 1) / a.heads_kv;
-  const int4 entry = at < a.max_blocks ? a.blocks[at] : make_int4(-1, 0, 0, 0);
-  if (entry.x < 0) return;  // all warps of the unit alike
-  const int slot = (warp % WARPS) * ROWS + sub;
   const AppendTensor& t = a.t[1 + which];
   const __nv_bfloat16* src = a.src[1 + which] + entry.w * a.src_token[1 + which] +
-                             head * a.src_head[1 + which] + d0;
+                             head * a.src_head[1 + which];
+  const Piece p = piece_at<APART>(a, chunk, READY && a.rotate);
   const long long block = static_cast<long long>(entry.x) * a.heads_kv + head;
   int8_t* exponent = a.exponents[which] + block;
   const int before = entry.y > 0 ? *exponent : kExponentFloor;
@@ -493,20 +560,25 @@ __global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int r = slot + i * (WARPS * ROWS);
-    if (r < entry.z) held[i] = *reinterpret_cast<const uint4*>(src + r * a.src_token[1 + which]);
+    if (r < entry.z) held[i] = load_piece<APART>(src + r * a.src_token[1 + which], p);
   }
   float amax = 0.f;
-  const int position = a.positions[entry.w];
+  int position = 0;
+  Weights w;
+  if constexpr (READY) {
+    position = a.positions[entry.w];
+    w = weights_at(t, p);
+  }
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int r = slot + i * (WARPS * ROWS);
     if (r < entry.z) {
       float x[8];
       widen8(held[i], x);
-      if (which == 0 && (t.normalize || a.rotate)) {
+      if constexpr (READY) {
         Turn turn = {};
-        if (a.rotate) turn = turn_at<HD>(a, position + r, d0);
-        ready_row<HD>(x, d0, mask, t, a, turn);
+        if (a.rotate) turn = turn_at<APART>(a, position + r, p);
+        ready_row<HD, APART>(x, p, mask, t, a, turn, w);
         held[i] = narrow8(x);
         widen8(held[i], x);
       }
@@ -524,13 +596,13 @@ __global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a
     // the unit's own barrier: other units of the CTA may have left
     asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / WARPS), "n"(WARPS * 32) : "memory");
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) amax = fmaxf(amax, largest[warp / WARPS * WARPS + w]);
+    for (int i = 0; i < WARPS; ++i) amax = fmaxf(amax, largest[warp / WARPS * WARPS + i]);
   } else {
     __syncwarp();
   }
   const int e = max(before, exponent_of(amax));
   if (chunk == 0 && slot == 0) *exponent = static_cast<int8_t>(e);
-  uint8_t* codes = a.codes[which] + block * a.page * HD + d0;
+  uint8_t* codes = a.codes[which] + block * a.page * HD;
   const float scale = exponent_scale(-e);
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
@@ -541,13 +613,13 @@ __global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         x[k] = fabsf(x[k]) <= kLargestStored ? x[k] * scale : __uint_as_float(0x7fc00000u);
-      *reinterpret_cast<uint2*>(codes + (entry.y + r) * HD) = encode8(x);
+      store_piece<APART>(codes + (entry.y + r) * HD, p, encode8(x));
     }
   }
   if (e > before && entry.y > 0) {  // the scale grew: shift what the block holds already
     const float shift = exponent_scale(max(before - e, -126));
     for (int r = slot; r < entry.y; r += WARPS * ROWS) {
-      uint2* row = reinterpret_cast<uint2*>(codes + r * HD);
+      uint2* row = reinterpret_cast<uint2*>(codes + r * HD + chunk * 8);
       float x[8];
       decode8(*row, x);
 #pragma unroll
@@ -555,6 +627,27 @@ __global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a
       *row = encode8(x);
     }
   }
+}
+
+template <int HD, int WARPS, int PASSES, bool APART>
+__global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a) {
+  constexpr int UNITS = 8 / WARPS;       // units a CTA
+  __shared__ float largest[8];
+  if (blockIdx.x < a.query_ctas) {  // queries: some heads of a token a group of threads
+    append_query<HD, APART>(a);
+    return;
+  }
+  const int warp = threadIdx.x >> 5;
+  const long long unit = static_cast<long long>(blockIdx.x - a.query_ctas) * UNITS + warp / WARPS;
+  const int which = static_cast<int>(unit & 1);  // 0 keys, 1 values
+  const int head = static_cast<int>((unit >> 1) % a.heads_kv);
+  const long long at = (unit >> 1) / a.heads_kv;
+  const int4 entry = at < a.max_blocks ? a.blocks[at] : make_int4(-1, 0, 0, 0);
+  if (entry.x < 0) return;  // all warps of the unit alike
+  if (which == 0 && (a.t[1].normalize || a.rotate))
+    append_unit<HD, WARPS, PASSES, true, APART>(a, 0, head, entry, largest);
+  else
+    append_unit<HD, WARPS, PASSES, false, false>(a, which, head, entry, largest);
 }
 
 template <int HD>
@@ -573,11 +666,16 @@ static int append_launch(AppendArgs& a, int longest, cudaStream_t stream) {
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
   a.query_ctas = static_cast<unsigned>(query_ctas);
   const unsigned grid = static_cast<unsigned>(ctas);
-  if (warps == 1) cache_append_kernel<HD, 1, 4><<<grid, 256, 0, stream>>>(a);
-  else if (warps == 2) cache_append_kernel<HD, 2, 4><<<grid, 256, 0, stream>>>(a);
-  else if (warps == 4) cache_append_kernel<HD, 4, 4><<<grid, 256, 0, stream>>>(a);
-  else if (most <= 32 * kRows) cache_append_kernel<HD, 8, 4><<<grid, 256, 0, stream>>>(a);
-  else cache_append_kernel<HD, 8, 128 / 8 / kRows><<<grid, 256, 0, stream>>>(a);
+  const bool apart = a.rotate && !a.rope.interleaved && a.rope.rotary > 0;
+  const auto launch = [&](auto* split, auto* whole) { (apart ? split : whole)<<<grid, 256, 0, stream>>>(a); };
+  if (warps == 1) launch(cache_append_kernel<HD, 1, 4, true>, cache_append_kernel<HD, 1, 4, false>);
+  else if (warps == 2) launch(cache_append_kernel<HD, 2, 4, true>, cache_append_kernel<HD, 2, 4, false>);
+  else if (warps == 4) launch(cache_append_kernel<HD, 4, 4, true>, cache_append_kernel<HD, 4, 4, false>);
+  else if (most <= 32 * kRows)
+    launch(cache_append_kernel<HD, 8, 4, true>, cache_append_kernel<HD, 8, 4, false>);
+  else
+    launch(cache_append_kernel<HD, 8, 128 / 8 / kRows, true>,
+           cache_append_kernel<HD, 8, 128 / 8 / kRows, false>);
   return cudaGetLastError();
 }
 
@@ -635,6 +733,7 @@ int cache_append(const CozyCachePlan& p, const CozyCacheStore& c, const CozyCach
     a.t[i].norm_weight = x.norm_weight[i];
     a.t[i].norm_offset = x.norm_offset[i];
     a.t[i].norm_eps = x.norm_eps[i];
+    a.t[i].wide = reinterpret_cast<uintptr_t>(x.norm_weight[i]) % 16 == 0;
   }
   if (x.rope != nullptr) {
     a.rope = *x.rope;

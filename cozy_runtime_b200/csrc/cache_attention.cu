@@ -135,12 +135,13 @@ __device__ __forceinline__ int request_of(const CacheArgs& a, const long long* u
 }
 
 // ------------------------------------------------------------------------------- few rows
-// HBM bounds this: a chunk is 2 · 64 · HD bytes. The matrix instructions are mma.sync m16n8k16
+// HBM bounds this: a chunk is 2 · 64 · HD bytes (64 requests of 2000 to 16384 keys, 32/8 heads of
+// 128: 1.16 GB in 199 us, 0.89 of the measured copy rate). The matrix instructions are mma.sync m16n8k16
 // with the keys as their 16 rows and the 8 query rows of an item as their columns (queries as the
 // 16 rows left half of every instruction, weight and accumulator of a decode step unused: 64
 // requests of 10000 keys 223 against 211 us in a loop under the power cap, 10 requests of 1800
-// keys and 24 heads 37 against 32). Codes are widened to f16 in registers (exact) straight from the swizzled tile
-// that TMA wrote. The operand layouts are chosen so that no transposing load is needed: the
+// keys and 24 heads 37 against 32). Codes are widened to f16 in registers (exact) straight from the
+// swizzled tile that TMA wrote. The operand layouts are chosen so that no transposing load is needed: the
 // contraction over channels may run in any order, so a thread's 16 consecutive channels of a key
 // serve four instructions; the keys of a tile may be taken in any order (row c is
 // (c & 1 ? c + 4 : c) mod 8 of 8, which keeps the 16-byte reads of both K and V free of bank
@@ -701,7 +702,9 @@ __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
 // A tile of keys is taken in two halves of 64 with a buffer of S each, so that the next half's
 // Q·Kᵀ is done when a half's softmax ends: neither the tensor cores nor the softmax wait for the
 // other's round trip. (With one buffer of 128 a unit took 3823 clocks, 2129 of them on the tensor
-// cores.) Tensor memory: S/P of tile s, half b at column 128 s + 64 b, O at 256 + HD s.
+// cores.) A chunk of 1024 tokens behind 130047 keys (32/8 heads of 128) takes 2.33 ms: 941 TFLOP/s,
+// 0.56 of the measured bf16 rate, under the power cap; the exponentials and the tensor cores take
+// about half of it each and overlap in part. Tensor memory: S/P of tile s, half b at column 128 s + 64 b, O at 256 + HD s.
 template <int HD>
 struct Many {
   static constexpr int kThreads = 512;

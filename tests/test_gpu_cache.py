@@ -221,6 +221,47 @@ def test_append_matches_the_law(lengths, new, page, hq, hkv, dim, norm, rotary, 
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
+def test_append_reads_tables_and_weights_of_any_alignment(interleaved):
+    """Tables and weights 4 bytes behind a 16-byte boundary, strided tables: the same bits."""
+    from cozy_runtime_b200 import cache, rope, ulysses
+
+    dim, page, hkv, hq, new = 64, 32, 2, 6, [70, 1, 9]
+    g = torch.Generator().manual_seed(15)
+    m = make([3, 40, 0], new, page, g)
+    layout = cache.Layout(hq, hkv, dim, page)
+    step, t = on_gpu(m, layout)
+    columns = dim // 2 if interleaved else dim
+    angle = torch.rand(t["table"].shape[1] * page, columns, generator=g).cuda() * 6
+    weight = torch.randn(dim, generator=g).cuda()
+    q, k = (torch.randn(m["tokens"], h, dim, generator=g).to(torch.bfloat16).cuda() for h in (hq, hkv))
+
+    def behind(x):
+        whole = x.new_empty(x.numel() + 1)
+        whole[1:] = x.flatten()
+        return whole[1:].view(x.shape)
+
+    def apart(x):
+        whole = x.new_zeros(x.shape[0], 2 * x.shape[1] + 3)
+        whole[:, 0:2 * x.shape[1]:2] = x
+        return whole
+
+    cos, sin = angle.cos(), angle.sin()
+    got = []
+    for c, s, strides, w in ((cos, sin, (columns, 1), weight),
+                             (behind(cos), behind(sin), (columns, 1), behind(weight)),
+                             (apart(cos), apart(sin), (2 * columns + 3, 2), behind(weight))):
+        spec = rope.RopeSpec(c, s, *strides, dim, interleaved)
+        store = cache.Cache.empty(layout, step.pages)
+        for codes in (store.key, store.value):
+            codes.view(torch.uint8).zero_()
+        norm = ulysses.Norm(w, offset=0.25, eps=1e-6)
+        out = cache.append(store, step, k, k, query=q, rope=spec, norm_q=norm, norm_k=norm)
+        got.append((out, store.key.view(torch.uint8), store.key_exponent, store.value.view(torch.uint8)))
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
 def test_append_keeps_what_is_not_finite_to_its_pair(interleaved):
     """NaN and infinities reach the channels that the rotation pairs them with, no others."""
     from cozy_runtime_b200 import cache, rope

@@ -157,7 +157,8 @@ class Cache:
 class Plan:
     """A step's plan on the GPU. `lengths` [requests] int32 after the step, `cursor` [2] int64
     after it, `starts` [requests + 1] int32, `positions` [tokens] int32 and `slots` [tokens] int64
-    (page number · page + row; both -1 in rows of nobody), `status` [1] int32."""
+    (page number · page + row; both -1 in rows of nobody and of tokens whose page number is outside
+    the pool), `status` [1] int32."""
 
     def __init__(self, layout: Layout, table: Tensor, lengths: Tensor, new: Tensor, free: Tensor,
                  cursor: Tensor, tokens: int, longest: int):
@@ -348,7 +349,9 @@ def append(
     dimension contiguous. Query and key are normed (`norm_q`, `norm_k`: per-head RMSNorm) and
     rotated (`rope`: row = position in the request; the tables must reach the table's width) in
     fp32 and rounded once to bf16, the laws of `rope.head_norm_rope`. Returns the ready queries
-    (`out`, or a new tensor; rows of nobody are left as they were), None without `query`.
+    (`out`, or a new tensor; rows of nobody are left as they were), None without `query`. A token
+    whose page number is outside the pool (the plan's status says so) is not stored, its ready query
+    is zero.
 
     A block's exponent is the smallest e ≥ -60 with max |x| ≤ 448 · 2^e over the tokens put into it
     so far. It only grows; the codes a block holds are then rounded to the grown scale, which is

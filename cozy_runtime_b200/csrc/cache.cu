@@ -300,6 +300,7 @@ struct AppendTensor {
 struct AppendArgs {
   const int4* blocks;
   const int* positions;
+  const int* used;  // tokens of the step's requests: rows from there on belong to nobody
   int max_blocks, tokens;
   int pages, page, heads_q, heads_kv;
   const __nv_bfloat16* src[3];  // query, key, value
@@ -527,7 +528,12 @@ __device__ __forceinline__ void append_query(const AppendArgs& a) {
   for (int i = 0; i < kHeadsAThread; ++i)
     if (head0 + i < a.heads_q)
       v[i] = load_piece<APART>(a.src[0] + token * a.src_token[0] + (head0 + i) * a.src_head[0], p);
-  if (position < 0) return;
+  if (position < 0) {  // a token of a page outside the pool has no place: a query of zeros
+    if (token < *a.used)
+      for (int i = 0; i < kHeadsAThread && head0 + i < a.heads_q; ++i)
+        store_piece<APART>(a.out + token * a.out_token + (head0 + i) * a.out_head, p, make_uint4(0, 0, 0, 0));
+    return;
+  }
   Turn turn = {};
   if (a.rotate) turn = turn_at<APART>(a, position, p);
   const Weights w = weights_at(a.t[0], p);
@@ -703,6 +709,7 @@ int cache_append(const CozyCachePlan& p, const CozyCacheStore& c, const CozyCach
   AppendArgs a = {};
   a.blocks = reinterpret_cast<const int4*>(p.blocks);
   a.positions = p.positions;
+  a.used = p.starts + p.requests;
   a.max_blocks = p.max_blocks;
   a.tokens = p.tokens;
   a.pages = c.pages;

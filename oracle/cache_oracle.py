@@ -106,6 +106,8 @@ def append_step(codes, exponents, table, lengths, new, rows, page):
         a = max(a, 0)
         for b in range(length // page, -(-(length + a) // page) if a else 0):
             low, high, p = max(length, b * page), min(length + a, (b + 1) * page), table[n][b]
+            if not 0 <= p < codes.shape[0]:  # tokens of a page that is not there are left out
+                continue
             for h in range(codes.shape[1]):
                 x = rows[t + low - length:t + high - length, h].double()
                 fits = x.abs() <= LARGEST

@@ -521,6 +521,49 @@ def test_attention_leaves_out_bad_pages(new, dim):
     assert int(step.status) == 16
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_a_step_with_bad_pages_among_good_ones(interleaved):
+    """Tokens whose own page number is outside the pool: nothing of them is stored, their ready
+    queries are zeros, and every other row and block is what the law gives."""
+    from cozy_runtime_b200 import cache, rope
+
+    lengths, new, page, hq, hkv, dim = [20, 40, 7], [40, 2, 1], 16, 4, 2, 64
+    g = torch.Generator().manual_seed(2)
+    m = make(lengths, new, page, g)
+    used = m["tokens"]
+    m["tokens"] += 2
+    m["table"][0][1] = 10**6  # the page that the first request is filling
+    m["free"][m["cursor"][0] % len(m["free"])] = -7  # and the first that it is given
+    step, t = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    positions, table = step.positions.cpu().long()[:used], t["table"].tolist()
+    bad = positions < 0
+    assert bad.tolist() == [i < 28 for i in range(used)]
+    k0, ke0 = fill(step.pages, hkv, page, dim, g)
+    v0, ve0 = fill(step.pages, hkv, page, dim, g)
+    store = store_on_gpu(k0, ke0, v0, ve0)
+    columns = dim // 2 if interleaved else dim
+    angle = torch.rand(t["table"].shape[1] * page, columns, generator=g) * 6
+    spec = rope.RopeSpec(angle.cos().cuda(), angle.sin().cuda(), columns, 1, dim, interleaved)
+    q, k, v = (torch.randn(m["tokens"], h, dim, generator=g).to(torch.bfloat16) for h in (hq, hkv, hkv))
+    kept = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    got = cache.append(store, step, k.cuda(), v.cuda(), query=q.cuda(), rope=spec, out=kept)
+    assert (got[:used][bad.cuda()] == 0).all() and (got[used:] == 7).all()
+    cos, sin = angle.cos()[positions.clamp_min(0)], angle.sin()[positions.clamp_min(0)]
+    want_q, want_k = (law.ready(x[:used], None, 0.0, None, cos, sin, interleaved, dim) for x in (q, k))
+    err = (got[:used].cpu().double() - want_q).abs()
+    assert (err <= 2**-8 * want_q.abs() + 2**-18 * want_q.abs().amax(-1, keepdim=True))[~bad].all()
+    kc, ke = law.append_step(k0.double(), ke0, table, lengths, new, want_k.to(torch.bfloat16).double(), page)
+    vc, ve = law.append_step(v0.double(), ve0, table, lengths, new, v[:used].double(), page)
+    assert torch.equal(store.value.cpu().double(), vc) and torch.equal(store.value_exponent.cpu().long(), ve)
+    assert torch.equal(store.key_exponent.cpu().long(), ke)
+    assert ((store.key.cpu().double() - kc).abs() <= 2**-3 * kc.abs() + 2**-9).all()
+    out, lse = cache.attention(store, step, got, return_lse=True)
+    stored = [values(c.cpu(), e.cpu()) for c, e in ((store.key, store.key_exponent), (store.value, store.value_exponent))]
+    want = law.attend_step(*stored, table, lengths, new, got.cpu(), page, dim**-0.5)
+    check_attention(out, lse, want, used, floor_of(60, store.value_exponent))
+    assert int(step.status) == 16
+
+
 @pytest.mark.parametrize("new", [[1, 2], [70, 90]])
 def test_attention_over_the_whole_range_of_scales(new):
     """Value exponents from the floor to the ceiling in one row, keys of tiny blocks, zero queries."""

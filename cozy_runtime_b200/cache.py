@@ -36,6 +36,7 @@ from cozy_runtime_b200.ulysses import Norm
 PAGES = (16, 32, 64, 128)
 MAX_REQUESTS = 8192
 MAX_GROUP = 128
+MAX_TOKENS = 2**30
 #: the range of a block's exponent; larger magnitudes than 448 · 2^40 are stored as NaN
 EXPONENT_RANGE = (-60, 40)
 
@@ -279,8 +280,8 @@ def plan(
         raise ValueError("an empty table or pool")
     if width * layout.page > 2**30:
         raise ValueError("a request holds at most 2^30 tokens")
-    if not 0 <= tokens < 2**31 or not 0 <= longest < 2**31:
-        raise ValueError("tokens and longest must be counts below 2^31")
+    if not 0 <= tokens <= MAX_TOKENS or not 0 <= longest < 2**31:
+        raise ValueError("tokens must be a count up to 2^30, longest one below 2^31")
     index = table.get_device()
     _one_device(table.device, index, lengths, new, free, cursor)
     made = Plan(layout, table, lengths, new, free, cursor, tokens, longest)

@@ -238,8 +238,10 @@ int cache_plan_check(const CozyCachePlan& p) {
   if (p.page != 16 && p.page != 32 && p.page != 64 && p.page != 128) return cudaErrorNotSupported;
   if (p.tokens < 0 || p.longest < 0 || p.group < 1 || p.table_stride < p.width)
     return cudaErrorInvalidValue;
-  // positions, and those up to a tile behind them, in 31 bits
+  // positions, and those up to a tile behind them, in 31 bits; rows, and those a grid behind them
   if (static_cast<long long>(p.width) * p.page > (1LL << 30)) return cudaErrorInvalidValue;
+  if (p.tokens > COZY_CACHE_MAX_TOKENS || p.max_blocks > COZY_CACHE_MAX_TOKENS)
+    return cudaErrorInvalidValue;
   if (p.group > COZY_CACHE_MAX_GROUP) return cudaErrorNotSupported;
   const void* ptrs[] = {p.lengths, p.added, p.table, p.free_ring, p.cursor, p.lengths_after,
                         p.starts, p.cursor_after, p.units, p.status};

@@ -466,6 +466,7 @@ COZY_API int cozy_ulysses_layer_end(CozyGroup* group, const CozyLayerCall* call,
  * into a graph. */
 #define COZY_CACHE_MAX_REQUESTS 8192
 #define COZY_CACHE_MAX_GROUP 128
+#define COZY_CACHE_MAX_TOKENS (1 << 30)
 
 /* A step's plan. Inputs: request n holds lengths[n] tokens in the pages of its table row and
  * brings added[n] new ones (0: none; -1: it is finished and its pages are released). Free page
@@ -492,10 +493,11 @@ typedef struct CozyCachePlan {
   int* free_ring;          /* [pages] */
   const long long* cursor; /* [2] head, tail */
   int requests, width, pages, page; /* page: 16, 32, 64 or 128 tokens; width * page <= 2^30 */
-  int tokens;              /* rows of the step's tensors */
+  int tokens;              /* rows of the step's tensors, at most COZY_CACHE_MAX_TOKENS */
   int longest;             /* no request brings more new tokens */
   int group;               /* query heads per key/value head, at most COZY_CACHE_MAX_GROUP */
-  int max_blocks;          /* entries of `blocks`: min(tokens, tokens / page + 2 * requests) */
+  int max_blocks;          /* entries of `blocks`: min(tokens, tokens / page + 2 * requests) or more, at most
+                              COZY_CACHE_MAX_TOKENS */
   int* lengths_after;      /* [requests] */
   int* starts;             /* [requests + 1] */
   long long* cursor_after; /* [2] */

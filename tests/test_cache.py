@@ -100,6 +100,34 @@ def test_c_entries_refuse_without_a_gpu():
         assert lib.cozy_cache_attention(ctypes.byref(plan()), ctypes.byref(store()), ctypes.byref(y), 0) == 1, change
 
 
+def plan_struct(**change):
+    from cozy_runtime_b200 import _lib
+
+    p = _lib.CachePlan()
+    fields = dict(requests=2, width=3, table_stride=3, pages=9, page=16, tokens=4, longest=2, group=2, max_blocks=4)
+    for name in ("lengths", "added", "table", "free_ring", "cursor", "lengths_after", "starts", "cursor_after",
+                 "positions", "slots", "blocks", "units", "status"):
+        fields[name] = 1 << 20
+    for name, value in (fields | change).items():
+        setattr(p, name, value)
+    return p
+
+
+def test_more_tokens_than_a_grids_indices_reach_are_refused():
+    """A thread's index is one of a row and of a row a grid behind: both stay in 31 bits."""
+    from cozy_runtime_b200 import _lib, cache
+
+    good = [torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.ones(2, dtype=torch.int32),
+            torch.zeros(9, dtype=torch.int32), torch.tensor([0, 9])]
+    for tokens in (2**30 + 1, 2**31 - 8192, 2**31 - 1):
+        with pytest.raises(ValueError, match="2\\^30"):
+            cache.plan(cache.Layout(4, 2, 64, 16), *good, tokens=tokens, longest=1)
+    lib = _lib.load()
+    for change in ({"tokens": 2**31 - 1, "max_blocks": 1 << 28}, {"tokens": 2**30 + 1, "max_blocks": 1 << 28},
+                   {"max_blocks": 2**31 - 1}):
+        assert lib.cozy_cache_plan(ctypes.byref(plan_struct(**change)), 0) == _lib.INVALID_VALUE, change
+
+
 def test_oracle_rounds_as_e4m3_does():
     g = torch.Generator().manual_seed(1)
     x = torch.cat([torch.randn(4000, generator=g) * 2.0 ** torch.randint(-12, 8, (4000,), generator=g),

@@ -278,6 +278,8 @@ def plan(
         raise ValueError(f"{requests} requests are not served (1 to {MAX_REQUESTS})")
     if width < 1 or free.shape[0] < 1:
         raise ValueError("an empty table or pool")
+    if free.shape[0] * layout.page >= 2**31:
+        raise ValueError(f"a ring of {free.shape[0]} pages: a pool holds at most 2^31 - 1 rows")
     if width * layout.page > 2**30:
         raise ValueError("a request holds at most 2^30 tokens")
     if not 0 <= tokens <= MAX_TOKENS or not 0 <= longest < 2**31:

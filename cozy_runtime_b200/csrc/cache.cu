@@ -240,6 +240,7 @@ int cache_plan_check(const CozyCachePlan& p) {
     return cudaErrorInvalidValue;
   // positions, and those up to a tile behind them, in 31 bits; rows, and those a grid behind them
   if (static_cast<long long>(p.width) * p.page > (1LL << 30)) return cudaErrorInvalidValue;
+  if (p.pages > 0x7fffffff / p.page) return cudaErrorInvalidValue;  // what no pool can hold
   if (p.tokens > COZY_CACHE_MAX_TOKENS || p.max_blocks > COZY_CACHE_MAX_TOKENS)
     return cudaErrorInvalidValue;
   if (p.group > COZY_CACHE_MAX_GROUP) return cudaErrorNotSupported;

@@ -492,7 +492,8 @@ typedef struct CozyCachePlan {
   long long table_stride;
   int* free_ring;          /* [pages] */
   const long long* cursor; /* [2] head, tail */
-  int requests, width, pages, page; /* page: 16, 32, 64 or 128 tokens; width * page <= 2^30 */
+  int requests, width, pages, page; /* page: 16, 32, 64 or 128 tokens; width * page <= 2^30,
+                                       pages * page < 2^31 */
   int tokens;              /* rows of the step's tensors, at most COZY_CACHE_MAX_TOKENS */
   int longest;             /* no request brings more new tokens */
   int group;               /* query heads per key/value head, at most COZY_CACHE_MAX_GROUP */

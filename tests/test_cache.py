@@ -128,6 +128,20 @@ def test_more_tokens_than_a_grids_indices_reach_are_refused():
         assert lib.cozy_cache_plan(ctypes.byref(plan_struct(**change)), 0) == _lib.INVALID_VALUE, change
 
 
+def test_a_ring_longer_than_any_pool_is_refused():
+    """Also one whose length, cut to 32 bits, would be that of a short ring."""
+    from cozy_runtime_b200 import _lib, cache
+
+    for pages, page in ((2**27, 16), (2**24, 128), (2**32 + 9, 16), (2**31 + 5, 64)):
+        free = torch.empty(pages, dtype=torch.int32, device="meta")  # a shape without memory
+        with pytest.raises(ValueError, match="rows"):
+            cache.plan(cache.Layout(4, 2, 64, page), torch.zeros(2, 3, dtype=torch.int32),
+                       torch.zeros(2, dtype=torch.int32), torch.ones(2, dtype=torch.int32), free,
+                       torch.tensor([0, 9]), tokens=2, longest=1)
+        if pages < 2**31:
+            assert _lib.load().cozy_cache_plan(ctypes.byref(plan_struct(pages=pages, page=page)), 0) == _lib.INVALID_VALUE
+
+
 def test_oracle_rounds_as_e4m3_does():
     g = torch.Generator().manual_seed(1)
     x = torch.cat([torch.randn(4000, generator=g) * 2.0 ** torch.randint(-12, 8, (4000,), generator=g),

@@ -328,6 +328,31 @@ def _overlap(a: Tensor, b: Tensor) -> bool:
     return a.numel() > 0 and a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
 
 
+def _rows_meet(a: Tensor, at: tuple[int, int], b: Tensor, bt: tuple[int, int]) -> bool:
+    """Whether a row of `a` and a row of `b` [tokens, heads, head_dim] share memory; `at`, `bt`:
+    their strides {token, head}. Slices of one packed projection lie in each other's span without
+    sharing a row. Spans that meet count as sharing where the token strides differ or rows overlap
+    their own tensor's."""
+    (tokens, heads_a, dim), heads_b, token = a.shape, b.shape[1], at[0]
+    apart = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    end_a = (tokens - 1) * token + (heads_a - 1) * at[1] + dim
+    end_b = apart + (tokens - 1) * bt[0] + (heads_b - 1) * bt[1] + dim
+    if tokens == 0 or apart >= end_a or end_b <= 0:
+        return False
+    if token != bt[0] or token < dim:
+        return True
+    behind = apart % token
+    if behind >= (heads_a - 1) * at[1] + dim and behind + (heads_b - 1) * bt[1] + dim <= token:
+        return False  # a token's rows of b between two tokens' of a
+    for offset in {apart + j * bt[1] - i * at[1] for i in range(heads_a) for j in range(heads_b)}:
+        # two rows that lie `offset` and some tokens apart, of which the nearest are looked at
+        near = -offset // token
+        for k in (near, near + 1):
+            if -tokens < k < tokens and abs(offset + k * token) < dim:
+                return True
+    return False
+
+
 def _fits(store: Cache, step: Plan) -> None:
     if store._blocks != step._blocks:
         raise ValueError(f"a cache of {store._blocks} [pages, heads, page, head_dim] "
@@ -352,7 +377,8 @@ def append(
     dimension contiguous. Query and key are normed (`norm_q`, `norm_k`: per-head RMSNorm) and
     rotated (`rope`: row = position in the request; the tables must reach the table's width) in
     fp32 and rounded once to bf16, the laws of `rope.head_norm_rope`. Returns the ready queries
-    (`out`, or a new tensor; rows of nobody are left as they were), None without `query`. A token
+    (`out`, or a new tensor; rows of nobody are left as they were), None without `query`. `out` is
+    the query itself or shares no memory with it, and none with a row of `key` or `value`. A token
     whose page number is outside the pool (the plan's status says so) is not stored, its ready query
     is zero.
 
@@ -378,6 +404,9 @@ def append(
             # in place is fine: a thread reads its rows before it writes them
             if _overlap(query, out) and (out.data_ptr() != query.data_ptr() or strides != tuple(a.query_strides)):
                 raise ValueError("out overlaps the query and is not the query")
+            # other blocks of threads read keys and values while these rows are written
+            if _rows_meet(out, strides, key, tuple(a.key_strides)) or _rows_meet(out, strides, value, tuple(a.value_strides)):
+                raise ValueError("out shares memory with the key or the value")
         a.query, a.out = query.data_ptr(), out.data_ptr()
         a.out_strides[:] = strides
     elif norm_q is not None or out is not None:

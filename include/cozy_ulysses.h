@@ -530,7 +530,8 @@ typedef struct CozyCacheStore {
  * e >= -60 with max |x| <= 448 * 2^e over the tokens put into it so far: it only grows, and the
  * codes that the block holds are then rounded to the grown scale (exact down to subnormals). A
  * magnitude over 448 * 2^40 or a NaN is stored as NaN and does not count for the exponent. Rows
- * of `out` that belong to nobody are left as they were. Strides in elements {token, head},
+ * of `out` that belong to nobody are left as they were. `out` is the query itself (pointer and
+ * strides) or shares no memory with it, and shares none with key and value. Strides in elements {token, head},
  * multiples of 8; pointers 16-byte aligned. Index 0 of the norm arrays is the query's, 1 the
  * key's. rope->token0 is not used; the tables must hold every position up to width * page. */
 typedef struct CozyCacheAppend {

@@ -142,6 +142,36 @@ def test_a_ring_longer_than_any_pool_is_refused():
             assert _lib.load().cozy_cache_plan(ctypes.byref(plan_struct(pages=pages, page=page)), 0) == _lib.INVALID_VALUE
 
 
+def test_rows_that_share_memory_are_found():
+    """Against the sets of elements themselves, for slices of packed projections and odd strides."""
+    import random
+
+    from cozy_runtime_b200 import cache
+
+    r, whole, met = random.Random(3), torch.zeros(6000, dtype=torch.bfloat16), 0
+    index = torch.arange(6000)
+    cases = []
+    for _ in range(3000):
+        dim, tokens = 8, r.randint(1, 5)
+        token = 8 * r.randint(1, 30)
+        shapes = [(tokens, r.randint(1, 4), dim) for _ in "ab"]
+        strides = [(token, 8 * r.randint(0, 8), 1) for _ in "ab"]
+        cases.append((shapes, strides, [8 * r.randint(0, 40) for _ in "ab"]))
+    # q, k and v of a packed row, in its own place and over one another's
+    cases += [([(4, 4, 8), (4, 2, 8)], [(64, 8, 1)] * 2, list(at)) for at in ((0, 32), (0, 48), (32, 32), (16, 32), (40, 32), (64, 48))]
+    for shapes, strides, starts in cases:
+        a, b = (torch.as_strided(whole, s, t, o) for s, t, o in zip(shapes, strides, starts))
+        sets = [set(torch.as_strided(index, s, t, o).flatten().tolist()) for s, t, o in zip(shapes, strides, starts)]
+        want = bool(sets[0] & sets[1])
+        # strides as the calls take them: of one token or one head, any will do
+        given = [(s[2] if s[0] <= 1 else t[0], s[2] if s[1] == 1 else t[1]) for s, t in zip(shapes, strides)]
+        assert cache._rows_meet(a, given[0], b, given[1]) == want, (shapes, strides, starts)
+        met += want
+    assert 500 < met < 2500
+    a, b = torch.as_strided(whole, (3, 2, 8), (64, 8, 1), 0), torch.as_strided(whole, (3, 2, 8), (80, 8, 1), 16)
+    assert cache._rows_meet(a, (64, 8), b, (80, 8))  # not shown to be apart
+
+
 def test_oracle_rounds_as_e4m3_does():
     g = torch.Generator().manual_seed(1)
     x = torch.cat([torch.randn(4000, generator=g) * 2.0 ** torch.randint(-12, 8, (4000,), generator=g),

@@ -778,6 +778,31 @@ def test_append_in_place():
         cache.append(store, step, qkv[:, 6:8], qkv[:, 8:], query=qkv[:, :6], rope=spec, out=qkv[:, 1:7])
 
 
+def test_append_refuses_an_out_over_keys_or_values():
+    """Keys and values are read while queries are written: an `out` over a row of theirs is refused
+    and nothing is stored; one between their rows is served."""
+    from cozy_runtime_b200 import cache
+
+    g = torch.Generator().manual_seed(2)
+    layout = cache.Layout(4, 4, 64, 16)
+    m = make([5, 40], [20, 3], 16, g)
+    step, _ = on_gpu(m, layout)
+    k0, ke0 = fill(step.pages, 4, 16, 64, g)
+    store = store_on_gpu(k0, ke0, k0, ke0)
+    qkv = torch.randn(23, 16, 64, generator=g).to(torch.bfloat16).cuda()
+    q, k, v, rest = qkv.split(4, dim=1)
+    was = qkv.clone()
+    for out in (k, v, qkv[:, 6:10], qkv[:, 11:15], qkv[:, 5:13:2]):
+        for query in (q, q.clone()):
+            with pytest.raises(ValueError, match="out"):
+                cache.append(store, step, k, v, query=query, out=out)
+    assert torch.equal(qkv, was) and torch.equal(store.key.cpu().view(torch.uint8), k0.view(torch.uint8))
+    got = cache.append(store, step, k, v, query=q.clone(), out=rest)
+    assert torch.equal(got, q) and torch.equal(qkv[:, :12], was[:, :12])
+    want = cache.append(store, step, k, v, query=q)
+    assert torch.equal(want, q)
+
+
 def test_an_empty_step():
     from cozy_runtime_b200 import cache
 

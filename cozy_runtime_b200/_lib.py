@@ -390,6 +390,7 @@ SIGNATURES = {
     "cozy_ulysses_layer_attend": ([c_void_p, POINTER(LayerCall), c_uint64], c_int),
     "cozy_ulysses_layer_end": ([c_void_p, POINTER(LayerCall), c_uint64], c_int),
     "cozy_cache_plan": ([POINTER(CachePlan), c_uint64], c_int),
+    "cozy_cache_plan_back": ([POINTER(CachePlan), c_void_p, c_uint64], c_int),
     "cozy_cache_append": (
         [POINTER(CachePlan), POINTER(CacheStore), POINTER(CacheAppend), c_uint64], c_int,
     ),

@@ -10,6 +10,12 @@ A step is one `plan` for all layers, then for each layer an `append` and an `att
         out = cache.attention(store, step, query)
     lengths, cursor = step.lengths, step.cursor
 
+Where a step's tokens are drafts of which some are rejected, the next step starts from shorter
+lengths and says how far the last one went, so that pages behind them come back:
+
+    step = cache.plan(layout, table, step.lengths - rejected, new, free, step.cursor, tokens=T,
+                      longest=L, reached=step.lengths)
+
 The step's tokens are packed: request n's rows of `query`, `key` and `value` [tokens, heads,
 head_dim] are `step.starts[n]` to `step.starts[n + 1]`. Lengths, page numbers and the plan's answer
 stay on the GPU: no call here synchronizes, and a step can be captured into a CUDA graph (each
@@ -258,6 +264,7 @@ def plan(
     *,
     tokens: int,
     longest: int,
+    reached: Tensor | None = None,
 ) -> Plan:
     """Gives pages to the requests of a step and says where its tokens go, in one launch.
 
@@ -267,8 +274,13 @@ def plan(
     numbers of which entries `cursor` = [head, tail) int64 (counted on, taken modulo pages) are
     free. Pages are given from the head in the requests' order; released ones go behind the tail
     and are given from the next plan on (every page of the row: who lets requests share pages counts
-    them, and sets a length to 0 instead of finishing the request). `tokens`: rows of the step's tensors (at least the sum of
-    `new`; rows behind it belong to nobody). `longest`: no request brings more than that.
+    them, and sets a length to 0 instead of finishing the request). `tokens`: rows of the step's tensors
+    (at least the sum of `new`; rows behind it belong to nobody). `longest`: no request brings more
+    than that. `reached` [requests] int32: the lengths that the last plan left (`Plan.lengths`),
+    where `lengths` may have been set back since: a row holds the pages of the larger of the two,
+    and those behind its tokens of this step are released like a finished request's. Without
+    `reached` such pages would be lost; with it, a row handed on with a length of 0 needs 0 there
+    too, and a step behind a refused one the refused one's `reached`.
 
     `table` and `free` are written in place, only where they held nothing; the new lengths and
     cursor are the plan's, so planning the same tensors again gives the same plan. A step that
@@ -284,11 +296,22 @@ def plan(
         raise ValueError("a request holds at most 2^30 tokens")
     if not 0 <= tokens <= MAX_TOKENS or not 0 <= longest < 2**31:
         raise ValueError("tokens must be a count up to 2^30, longest one below 2^31")
-    index = table.get_device()
-    _one_device(table.device, index, lengths, new, free, cursor)
+    if reached is not None:
+        _need(reached, "reached", torch.int32, (requests,))
+        if not reached.is_contiguous():
+            raise ValueError("reached must be contiguous")
+    index, device = table.get_device(), table.device
+    _one_device(device, index, lengths, new, free, cursor)
+    if reached is not None:
+        _one_device(device, index, reached)
     made = Plan(layout, table, lengths, new, free, cursor, tokens, longest)
+    made._inputs += (reached,)
+    lib = _lib.load()
     with _on(index):
-        code = _lib.load().cozy_cache_plan(ctypes.byref(made._c), _stream(index))
+        if reached is None:
+            code = lib.cozy_cache_plan(ctypes.byref(made._c), _stream(index))
+        else:
+            code = lib.cozy_cache_plan_back(ctypes.byref(made._c), reached.data_ptr(), _stream(index))
     _lib.check("cozy_cache_plan", code)
     return made
 
@@ -383,7 +406,8 @@ def append(
     is zero.
 
     A block's exponent is the smallest e ≥ -60 with max |x| ≤ 448 · 2^e over the tokens put into it
-    so far. It only grows; the codes a block holds are then rounded to the grown scale, which is
+    so far, those among them that were rejected later. It only grows until a token starts the block
+    anew; the codes a block holds are then rounded to the grown scale, which is
     exact down to e4m3's subnormals. NaN, infinities and magnitudes over 448 · 2^40 are stored as
     NaN and leave the exponent alone. The same step can be appended again: it stores the same.
     A page that requests share must be full: two writers of one block are not ordered."""

@@ -49,25 +49,34 @@ __device__ __forceinline__ long long pages_of(long long length, int page) {
   return (length + page - 1) / page;
 }
 
+// Pages that a request's row holds before the step: those of its length, or of the length that it
+// was set back from.
+__device__ __forceinline__ long long held_pages(const CozyCachePlan& p, const int* reached, int n) {
+  return pages_of(reached == nullptr ? p.lengths[n] : max(p.lengths[n], reached[n]), p.page);
+}
+
+// Pages that it holds behind the step.
+__device__ __forceinline__ long long kept_pages(const CozyCachePlan& p, int n) {
+  const long long added = p.added[n];
+  return added < 0 ? 0 : pages_of(p.lengths[n] + added, p.page);
+}
+
 // One request's part of the sums, and the status bits it raises.
-__device__ __forceinline__ PlanSums request_sums(const CozyCachePlan& p, int n, int* flags) {
+__device__ __forceinline__ PlanSums request_sums(const CozyCachePlan& p, const int* reached, int n,
+                                                 int* flags) {
   const long long length = p.lengths[n], added = p.added[n];
   PlanSums s = {};
-  if (length < 0 || added < -1) {
+  if (length < 0 || added < -1 || (reached != nullptr && reached[n] < 0)) {
     *flags |= kPlanLengths;
     return s;
   }
-  const long long held = pages_of(length, p.page);
-  if (added < 0) {
-    if (held > p.width) *flags |= kPlanNarrow;
-    s.back = held;
-    return s;
-  }
-  const long long want = pages_of(length + added, p.page);
-  if (want > p.width) *flags |= kPlanNarrow;
+  const long long held = held_pages(p, reached, n), want = kept_pages(p, n);
+  if (held > p.width || want > p.width) *flags |= kPlanNarrow;
+  s.back = max(0LL, held - want);
+  if (added < 0) return s;
   if (added > p.longest) *flags |= kPlanTokens;
   s.tokens = added;
-  s.need = want - held;
+  s.need = max(0LL, want - held);
   if (added > 0) {
     s.blocks = want - length / p.page;
     const long long units = attention_units(p.group, length, added);
@@ -92,7 +101,8 @@ __device__ __forceinline__ int span_of(const int* starts, int n, int at) {
   return low;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const CozyCachePlan p) {
+__global__ void __launch_bounds__(kPlanThreads)
+    cache_plan_kernel(const CozyCachePlan p, const int* reached) {
   extern __shared__ int plan_smem[];
   __shared__ PlanSums warp_sums[32];
   __shared__ int any_flags;
@@ -111,7 +121,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const CozyCach
   PlanSums carry = {};
   for (int base = 0; base < p.requests; base += kPlanThreads) {
     const int n = base + threadIdx.x;
-    PlanSums mine = n < p.requests ? request_sums(p, n, &flags) : PlanSums{};
+    PlanSums mine = n < p.requests ? request_sums(p, reached, n, &flags) : PlanSums{};
     PlanSums upto = mine;
 #pragma unroll
     for (int by = 1; by < 32; by <<= 1) {
@@ -186,7 +196,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const CozyCach
   // the page of block `b` of request n: fresh ones straight from the ring
   bool bad = false;
   auto page_of = [&](int n, int b) {
-    const int held = static_cast<int>(pages_of(p.lengths[n], p.page));
+    const int held = static_cast<int>(held_pages(p, reached, n));
     const int id = b < held ? p.table[n * p.table_stride + b]
                             : p.free_ring[ring_at(head + needs[n] + (b - held), p.pages)];
     if (id >= 0 && id < p.pages) return id;
@@ -223,11 +233,12 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const CozyCach
   if (bad) atomicOr(p.status, kPlanBadPage);
   for (int i = first; i < carry.back; i += step) {
     const int n = span_of(backs, p.requests, i);
-    p.free_ring[ring_at(tail + i, p.pages)] = p.table[n * p.table_stride + (i - backs[n])];
+    p.free_ring[ring_at(tail + i, p.pages)] =
+        p.table[n * p.table_stride + kept_pages(p, n) + (i - backs[n])];
   }
   for (int i = first; i < carry.need; i += step) {
     const int n = span_of(needs, p.requests, i);
-    const int held = static_cast<int>(pages_of(p.lengths[n], p.page));
+    const long long held = held_pages(p, reached, n);
     p.table[n * p.table_stride + held + (i - needs[n])] = p.free_ring[ring_at(head + i, p.pages)];
   }
 }
@@ -256,7 +267,7 @@ int cache_plan_check(const CozyCachePlan& p) {
   return cudaSuccess;
 }
 
-int cache_plan(const CozyCachePlan& p, cudaStream_t stream) {
+int cache_plan(const CozyCachePlan& p, const int* reached, cudaStream_t stream) {
   const int e = cache_plan_check(p);
   if (e) return e;
   const size_t smem = 4 * sizeof(int) * (static_cast<size_t>(p.requests) + 1);
@@ -284,7 +295,7 @@ int cache_plan(const CozyCachePlan& p, cudaStream_t stream) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, cache_plan_kernel, p);
+  return cudaLaunchKernelEx(&cfg, cache_plan_kernel, p, reached);
 }
 
 // -------------------------------------------------------------------------------- the append

@@ -167,7 +167,7 @@ int cozy_attention_fwd_fp8(const void* q, const void* k, const void* v, const fl
 }  // extern "C"
 
 namespace cozy {
-int cache_plan(const CozyCachePlan& plan, cudaStream_t stream);
+int cache_plan(const CozyCachePlan& plan, const int* reached, cudaStream_t stream);
 int cache_append(const CozyCachePlan& plan, const CozyCacheStore& store,
                  const CozyCacheAppend& append, cudaStream_t stream);
 long long cache_workspace(const CozyCachePlan& plan, const CozyCacheStore& store);
@@ -179,7 +179,12 @@ extern "C" {
 
 int cozy_cache_plan(const CozyCachePlan* plan, uintptr_t stream) {
   if (!plan) return cudaErrorInvalidValue;
-  return cozy::cache_plan(*plan, as_stream(stream));
+  return cozy::cache_plan(*plan, nullptr, as_stream(stream));
+}
+
+int cozy_cache_plan_back(const CozyCachePlan* plan, const int* reached, uintptr_t stream) {
+  if (!plan || !reached) return cudaErrorInvalidValue;
+  return cozy::cache_plan(*plan, reached, as_stream(stream));
 }
 
 int cozy_cache_append(const CozyCachePlan* plan, const CozyCacheStore* store,

@@ -513,6 +513,14 @@ typedef struct CozyCachePlan {
 
 COZY_API int cozy_cache_plan(const CozyCachePlan* plan, uintptr_t stream);
 
+/* The same for requests whose lengths may have been set back since the last step (rejected drafts):
+ * request n's row holds the pages of max(lengths[n], reached[n]) tokens, reached [requests] being
+ * the last plan's lengths_after. Pages behind lengths[n] + added[n] tokens go behind the ring's
+ * tail, as those of a finished request do; after the step a row holds its lengths_after's pages
+ * again. Through cozy_cache_plan such pages would be in neither the table nor the ring. A row that
+ * is handed on by setting its length to 0 has reached 0 too, or its pages are released. */
+COZY_API int cozy_cache_plan_back(const CozyCachePlan* plan, const int* reached, uintptr_t stream);
+
 /* One layer's blocks: codes [pages][heads_kv][page][head_dim] (e4m3, 128-byte aligned) and one
  * exponent a block ([pages][heads_kv], int8 in [-60, 40]): value = code * 2^exponent. */
 typedef struct CozyCacheStore {

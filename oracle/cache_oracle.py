@@ -14,22 +14,23 @@ FLOOR = -60
 LARGEST = 448.0 * 2.0**40
 
 
-def plan_step(table, lengths, new, free, cursor, *, tokens, longest, page):
-    """Lists in (table: list of rows; copies are changed), a dict out."""
+def plan_step(table, lengths, new, free, cursor, *, tokens, longest, page, reached=None):
+    """Lists in (table: list of rows; copies are changed), a dict out. `reached`: lengths that the
+    rows held pages for, where they were set back since."""
+    reached = lengths if reached is None else reached
     table, free = [list(r) for r in table], list(free)
     pages, width, (head, tail) = len(free), len(table[0]), cursor
     up = lambda x: -(-x // page)  # noqa: E731
     status, need, back, total = 0, 0, 0, 0
-    for length, a in zip(lengths, new):
-        if length < 0 or a < -1:
+    for length, a, r in zip(lengths, new, reached):
+        held, want = up(max(length, r)), up(length + a) if a >= 0 else 0
+        if length < 0 or a < -1 or r < 0:
             status |= 8
-        elif a < 0:
-            status |= 2 * (up(length) > width)
-            back += up(length)
-        else:
-            status |= 2 * (up(length + a) > width) | 4 * (a > longest)
-            need += up(length + a) - up(length)
-            total += a
+            continue
+        status |= 2 * (max(held, want) > width) | 4 * (a > longest)
+        need += max(0, want - held)
+        back += max(0, held - want)
+        total += max(a, 0)
     if head < 0 or tail < head or tail - head > pages:
         status |= 8
     elif need > tail - head:
@@ -43,14 +44,15 @@ def plan_step(table, lengths, new, free, cursor, *, tokens, longest, page):
     if status:
         return out
     before, t = [list(r) for r in table], 0
-    for n, (length, a) in enumerate(zip(lengths, new)):
+    for n, (length, a, r) in enumerate(zip(lengths, new, reached)):
+        held = up(max(length, r))
+        for i in range(up(length + a) if a >= 0 else 0, held):
+            free[tail % pages] = before[n][i]
+            tail += 1
         if a < 0:
-            for i in range(up(length)):
-                free[tail % pages] = before[n][i]
-                tail += 1
             out["lengths"][n] = 0
         else:
-            for b in range(up(length), up(length + a)):
+            for b in range(held, up(length + a)):
                 table[n][b] = free[head % pages]
                 head += 1
             for x in range(length, length + a):

@@ -172,6 +172,29 @@ def test_rows_that_share_memory_are_found():
     assert cache._rows_meet(a, (64, 8), b, (80, 8))  # not shown to be apart
 
 
+def test_what_was_reached_is_checked_before_the_device():
+    from cozy_runtime_b200 import _lib, cache
+
+    good = [torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.ones(2, dtype=torch.int32),
+            torch.zeros(9, dtype=torch.int32), torch.tensor([0, 9])]
+    for reached in (torch.zeros(3, dtype=torch.int32), torch.zeros(2), torch.zeros(4, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="reached"):
+            cache.plan(cache.Layout(4, 2, 64, 16), *good, tokens=2, longest=1, reached=reached)
+    lib = _lib.load()
+    assert lib.cozy_cache_plan_back(ctypes.byref(plan_struct()), None, 0) == _lib.INVALID_VALUE
+    assert lib.cozy_cache_plan_back(None, 1 << 20, 0) == _lib.INVALID_VALUE
+    assert lib.cozy_cache_plan_back(ctypes.byref(plan_struct(requests=0)), 1 << 20, 0) == _lib.INVALID_VALUE
+
+
+def test_the_law_keeps_every_page_when_drafts_are_rejected():
+    table, free, cursor, reached = [[0, -1, -1]], [0, 1, 2], [1, 3], [15]
+    for _ in range(20):
+        made = law.plan_step(table, [15], [5], free, cursor, tokens=5, longest=5, page=16, reached=reached)
+        assert made["status"] == 0
+        table, free, cursor, reached = (made[k] for k in ("table", "free", "cursor", "lengths"))
+        assert sorted(table[0][:2] + [free[i % 3] for i in range(*cursor)]) == [0, 1, 2]
+
+
 def test_oracle_rounds_as_e4m3_does():
     g = torch.Generator().manual_seed(1)
     x = torch.cat([torch.randn(4000, generator=g) * 2.0 ** torch.randint(-12, 8, (4000,), generator=g),

@@ -668,6 +668,103 @@ def test_requests_come_grow_and_go():
         assert int(cursor[1] - cursor[0]) == pages - free_now
 
 
+def test_a_draft_over_a_pages_end_is_rejected_again_and_again():
+    from cozy_runtime_b200 import cache
+
+    layout, pages = cache.Layout(2, 1, 64, 16), 3
+    table, free, new = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[0, -1, -1]], [0, 1, 2], [5]))
+    lengths = reached = torch.tensor([15], dtype=torch.int32, device="cuda")
+    cursor = torch.tensor([1, 3], device="cuda")
+    for _ in range(50):
+        step = cache.plan(layout, table, lengths, new, free, cursor, tokens=5, longest=5, reached=reached)
+        step.check()
+        reached, cursor = step.lengths, step.cursor
+        held = table[0, :2].tolist()
+        left = [int(free[i % pages]) for i in range(*cursor.tolist())]
+        assert sorted(held + left) == [0, 1, 2] and step.slots.tolist()[1] == held[1] * 16
+    step = cache.plan(layout, table, lengths, new - 6, free, cursor, tokens=5, longest=5, reached=reached)
+    step.check()
+    assert int(step.cursor[1] - step.cursor[0]) == pages and sorted(free.tolist()) == [0, 1, 2]
+
+
+@pytest.mark.parametrize("page,longest", [(16, 40), (32, 7), (64, 200)])
+def test_lengths_set_back_give_their_pages_back(page, longest):
+    """Steps whose requests come, bring drafts, lose some of them (whole pages too) and go: each plan
+    is the law's, eager and captured, the rows and the ring hold every page once, and the attention
+    sees what was accepted."""
+    import random
+
+    from cozy_runtime_b200 import cache
+
+    r, g = random.Random(page), torch.Generator().manual_seed(page)
+    layout, requests, tokens = cache.Layout(4, 2, 64, page), 5, 300
+    width = 6 * longest // page + 8
+    pages = requests * width
+    state = {"table": torch.full((requests, width), -1, dtype=torch.int32), "lengths": torch.zeros(requests, dtype=torch.int32),
+             "new": torch.zeros(requests, dtype=torch.int32), "reached": torch.zeros(requests, dtype=torch.int32),
+             "free": torch.randperm(pages, generator=g).to(torch.int32), "cursor": torch.tensor([0, pages])}
+    state = {k: x.cuda() for k, x in state.items()}
+    captured = {k: x.clone() for k, x in state.items()}
+
+    def plan(s):
+        return cache.plan(layout, s["table"], s["lengths"], s["new"], s["free"], s["cursor"], tokens=tokens,
+                          longest=longest, reached=s["reached"])
+
+    plan({k: x.clone() for k, x in state.items()})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured_plan = plan(captured)
+    store = cache.Cache.empty(layout, pages)
+    lengths = [0] * requests
+    for i in range(40):
+        reached = state["reached"].tolist()
+        # what was rejected of the last step, and what this one brings
+        lengths = [0 if not x else x - r.choice([0, 0, 1, r.randint(0, min(x, longest))]) for x in reached]
+        new = [-1 if x and r.random() < 0.1 else r.choice([0, 1, r.randint(1, longest)]) if x + longest <= page * (width - 1) else -1
+               for x in lengths]
+        while sum(max(a, 0) for a in new) > tokens:
+            new[r.randrange(requests)] = 0
+        want = law.plan_step(state["table"].tolist(), lengths, new, state["free"].tolist(), state["cursor"].tolist(),
+                             tokens=tokens, longest=longest, page=page, reached=reached)
+        assert want["status"] == 0
+        for s in (state, captured):
+            s["lengths"].copy_(torch.tensor(lengths, dtype=torch.int32))
+            s["new"].copy_(torch.tensor(new, dtype=torch.int32))
+        graph.replay()
+        step = plan(state)
+        for p, s in ((step, state), (captured_plan, captured)):
+            p.check()
+            for name in ("lengths", "starts", "cursor", "positions", "slots"):
+                assert getattr(p, name).tolist() == want[name], (i, name)
+            assert s["table"].tolist() == want["table"] and s["free"].tolist() == want["free"]
+        head, tail = want["cursor"]
+        rows = [p for row, x in zip(want["table"], want["lengths"]) for p in row[:-(-x // page)]]
+        assert sorted(rows + [want["free"][j % pages] for j in range(head, tail)]) == list(range(pages))
+        qkv = torch.randn(tokens, 8, 64, generator=g).to(torch.bfloat16).cuda()
+        cache.append(store, step, qkv[:, 4:6], qkv[:, 6:])
+        out, lse = cache.attention(store, step, qkv[:, :4], return_lse=True)
+        if i % 8 == 7:
+            kv = [values(c.cpu(), e.cpu()) for c, e in ((store.key, store.key_exponent), (store.value, store.value_exponent))]
+            ref = law.attend_step(*kv, want["table"], lengths, new, qkv[:, :4].cpu(), page, 0.125)
+            check_attention(out, lse, ref, sum(max(a, 0) for a in new), floor_of(pages * page, store.value_exponent))
+        for p, s in ((step, state), (captured_plan, captured)):
+            s["reached"].copy_(p.lengths)
+            s["cursor"].copy_(p.cursor)
+
+
+@pytest.mark.parametrize("reached,bit", [([-1, 40], 8), ([16 * 8, 40], 2), ([20, 2**31 - 1], 2)])
+def test_plan_refuses_an_impossible_reach(reached, bit):
+    from cozy_runtime_b200 import cache
+
+    m = make([20, 40], [40, 2], 16, torch.Generator().manual_seed(2))
+    t = {k: torch.tensor(m[k], dtype=torch.int64 if k == "cursor" else torch.int32, device="cuda")
+         for k in ("table", "lengths", "new", "free", "cursor")}
+    step = cache.plan(cache.Layout(4, 4, 64, 16), *t.values(), tokens=m["tokens"], longest=m["longest"],
+                      reached=torch.tensor(reached, dtype=torch.int32, device="cuda"))
+    assert int(step.status) & bit and step.starts.tolist() == [0, 0, 0]
+    assert t["table"].tolist() == m["table"] and t["free"].tolist() == m["free"]
+
+
 def test_a_captured_step_plans_anew_at_each_replay():
     from cozy_runtime_b200 import cache, rope
 

@@ -284,7 +284,8 @@ def plan(
 
     `table` and `free` are written in place, only where they held nothing; the new lengths and
     cursor are the plan's, so planning the same tensors again gives the same plan. A step that
-    cannot be served (see `STATUS_NAMES`) changes nothing: its plan has no rows."""
+    cannot be served (see `STATUS_NAMES`; a page number outside the pool among those to be released
+    is one such) changes nothing: its plan has no rows."""
     requests, width = _check_plan(table, lengths, new, free, cursor)
     if not 1 <= requests <= MAX_REQUESTS:
         raise ValueError(f"{requests} requests are not served (1 to {MAX_REQUESTS})")

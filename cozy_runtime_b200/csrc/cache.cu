@@ -1,6 +1,7 @@
 // The 8-bit paged cache's bookkeeping: a step's plan (block tables and slot maps from request
 // lengths) and the append (per-head RMSNorm and RoPE of the step's queries and keys, keys and
 // values into e4m3 blocks).
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -11,6 +12,8 @@
 #include "norm_rope.cuh"
 
 namespace cozy {
+
+namespace cg = cooperative_groups;
 
 // ---------------------------------------------------------------------------------- the plan
 // One cluster. Every CTA scans all requests (a few loads a thread, two barriers a round: cheaper
@@ -101,11 +104,17 @@ __device__ __forceinline__ int span_of(const int* starts, int n, int at) {
   return low;
 }
 
+// Released page number `i` of the step: its request's table entries behind what it keeps.
+__device__ __forceinline__ int released_page(const CozyCachePlan& p, const int* backs, int i) {
+  const int n = span_of(backs, p.requests, i);
+  return p.table[n * p.table_stride + kept_pages(p, n) + (i - backs[n])];
+}
+
 __global__ void __launch_bounds__(kPlanThreads)
     cache_plan_kernel(const CozyCachePlan p, const int* reached) {
   extern __shared__ int plan_smem[];
   __shared__ PlanSums warp_sums[32];
-  __shared__ int any_flags;
+  __shared__ int any_flags, bad_release;
   const int n1 = p.requests + 1;
   int* starts = plan_smem;        // [requests + 1] each: tokens, fresh pages, released pages, blocks
   int* needs = starts + n1;
@@ -113,8 +122,11 @@ __global__ void __launch_bounds__(kPlanThreads)
   int* blocks = backs + n1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool lead = blockIdx.x == 0;
-  if (threadIdx.x == 0) any_flags = 0;
+  if (threadIdx.x == 0) any_flags = bad_release = 0;
   __syncthreads();
+  cg::cluster_group cluster = cg::this_cluster();
+  const bool alone = gridDim.x == 1;
+  if (!alone) cluster.barrier_arrive();
 
   // checks first: a step that cannot be served gets nothing at all
   int flags = 0;
@@ -163,29 +175,53 @@ __global__ void __launch_bounds__(kPlanThreads)
   else if (tail - head + carry.back > p.pages) flags |= kPlanLengths;
   if (carry.tokens > p.tokens) flags |= kPlanTokens;
   if (flags) atomicOr(&any_flags, flags);
+  if (threadIdx.x == 0) {
+    starts[0] = needs[0] = backs[0] = blocks[0] = 0;
+    if (lead) p.units[0] = p.units[n1] = 0;
+  }
   __syncthreads();
-  const int status = any_flags;
+  int status = any_flags;  // alike in all CTAs
+  if (lead && threadIdx.x == 0) *p.status = status;
+  const int first = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
+  // A number outside the pool must not come into the ring, from where another request would be
+  // given it: each CTA looks at its share and tells all. A thread's first numbers stay in registers.
+  constexpr int kGiven = 4;
+  int given[kGiven];
+  if (!alone) cluster.barrier_wait();  // every bad_release is set
+  if (status == 0 && carry.back > 0) {
+    bool out = false;
+    auto look = [&](int i) {
+      const int id = i < carry.back ? released_page(p, backs, i) : 0;
+      out |= id < 0 || id >= p.pages;
+      return id;
+    };
+#pragma unroll
+    for (int j = 0; j < kGiven; ++j) given[j] = look(first + j * step);
+    for (int i = first + kGiven * step; i < carry.back; i += step) look(i);
+    if (out)
+      for (unsigned r = 0; r < gridDim.x; ++r) *cluster.map_shared_rank(&bad_release, r) = 1;
+  }
+  // the status word is also set before any CTA adds the bad-page bit to it
+  if (alone) __syncthreads();
+  else cluster.sync();
+  if (bad_release) {
+    status = kPlanBadPage;
+    if (lead && threadIdx.x == 0) *p.status = status;  // nobody adds to it: the step has no rows
+  }
   const bool refused = status != 0;
   if (refused) {
     for (int n = threadIdx.x; n < n1; n += kPlanThreads) {
       starts[n] = 0;
       if (lead) p.units[n] = p.units[n1 + n] = 0;
     }
+    __syncthreads();
     carry = PlanSums{};
-  } else if (threadIdx.x == 0) {
-    starts[0] = needs[0] = backs[0] = blocks[0] = 0;
-    if (lead) p.units[0] = p.units[n1] = 0;
   }
   if (lead && threadIdx.x == 0) {
-    *p.status = status;
     p.cursor_after[0] = head + carry.need;
     p.cursor_after[1] = tail + carry.back;
   }
-  // the status word is set before any CTA adds the bad-page bit to it
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
 
-  const int first = blockIdx.x * kPlanThreads + threadIdx.x, step = gridDim.x * kPlanThreads;
   for (int n = first; n < n1; n += step) {
     p.starts[n] = starts[n];
     if (n < p.requests) {
@@ -231,11 +267,11 @@ __global__ void __launch_bounds__(kPlanThreads)
     reinterpret_cast<int4*>(p.blocks)[i] = entry;
   }
   if (bad) atomicOr(p.status, kPlanBadPage);
-  for (int i = first; i < carry.back; i += step) {
-    const int n = span_of(backs, p.requests, i);
-    p.free_ring[ring_at(tail + i, p.pages)] =
-        p.table[n * p.table_stride + kept_pages(p, n) + (i - backs[n])];
-  }
+#pragma unroll
+  for (int j = 0; j < kGiven; ++j)
+    if (first + j * step < carry.back) p.free_ring[ring_at(tail + first + j * step, p.pages)] = given[j];
+  for (int i = first + kGiven * step; i < carry.back; i += step)
+    p.free_ring[ring_at(tail + i, p.pages)] = released_page(p, backs, i);
   for (int i = first; i < carry.need; i += step) {
     const int n = span_of(needs, p.requests, i);
     const long long held = held_pages(p, reached, n);

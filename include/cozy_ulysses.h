@@ -480,8 +480,9 @@ COZY_API int cozy_ulysses_layer_end(CozyGroup* group, const CozyLayerCall* call,
  * *status: 0, or the sum of 1 (too few free pages), 2 (a request longer than its table row), 4
  * (more new tokens than `tokens`, or than `longest` in one request), 8 (a negative length,
  * added < -1, or an impossible cursor) - with any of these nothing is given or released, starts
- * are all 0 and append and attention do nothing - and 16 (a page number outside [0, pages): the
- * tokens in such a page have position and slot -1, append stores nothing of them and writes zeros
+ * are all 0 and append and attention do nothing - and 16 (a page number outside [0, pages)). Among
+ * pages that would be released 16 refuses the step in the same way: such a number must not come
+ * into the ring. Elsewhere the tokens in such a page have position and slot -1, append stores nothing of them and writes zeros
  * for their queries; they stay rows of their request, so attention gives what their query finds in
  * the pages that are there). A later call that meets such a page in the table sets 16
  * too, and one whose on-chip wait times out sets 32 (its output is then incomplete). */

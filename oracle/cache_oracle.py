@@ -38,6 +38,10 @@ def plan_step(table, lengths, new, free, cursor, *, tokens, longest, page, reach
     elif tail - head + back > pages:
         status |= 8
     status |= 4 * (total > tokens)
+    if not status:  # numbers outside the pool do not come into the ring
+        gone = (p for row, length, a, r in zip(table, lengths, new, reached)
+                for p in row[up(length + a) if a >= 0 else 0:up(max(length, r))])
+        status = 16 * any(not 0 <= p < pages for p in gone)
     out = {"status": status, "table": table, "free": free, "lengths": [max(x, 0) for x in lengths],
            "cursor": [head, tail], "starts": [0] * (len(new) + 1), "positions": [-1] * tokens,
            "slots": [-1] * tokens}

@@ -153,6 +153,39 @@ def test_plan_leaves_out_bad_pages():
     assert step.slots.tolist() == want["slots"] and step.positions.tolist() == want["positions"]
 
 
+@pytest.mark.parametrize("requests", [3, 1500])
+def test_plan_refuses_to_release_what_is_not_in_the_pool(requests):
+    """A finished or shortened row with a number outside the pool: the step changes nothing, and
+    the ring holds pages of the pool only; without that row it is served."""
+    from cozy_runtime_b200 import cache
+
+    layout = cache.Layout(4, 4, 64, 16)
+    lengths = [20 + 37 * i % 90 for i in range(requests)]
+    for bad, new_there in ((-1, -1), (10**6, -1), (-1, 0)):
+        new = [-1 if i % 7 == 0 else 1 for i in range(requests)]
+        m = make(lengths, new, 16, torch.Generator().manual_seed(2))
+        who = requests - 2
+        new[who] = new_there
+        m["new"], set_back = new, list(lengths)
+        if new_there == 0:  # a row set back to where its last page is not needed
+            set_back[who] = 16 * ((lengths[who] - 1) // 16)
+        m["table"][who][(lengths[who] - 1) // 16] = bad
+        t = {k: torch.tensor(m[k], dtype=torch.int64 if k == "cursor" else torch.int32, device="cuda")
+             for k in ("table", "lengths", "new", "free", "cursor")}
+        t["lengths"].copy_(torch.tensor(set_back, dtype=torch.int32))
+        reached = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        want = law.plan_step(m["table"], set_back, new, m["free"], m["cursor"], tokens=requests, longest=1, page=16,
+                             reached=lengths)
+        step = cache.plan(layout, *t.values(), tokens=requests, longest=1, reached=reached)
+        assert int(step.status) == want["status"] == 16
+        assert t["table"].tolist() == m["table"] and t["free"].tolist() == m["free"]
+        assert step.starts.tolist() == [0] * (requests + 1) and step.cursor.tolist() == m["cursor"]
+        assert step.lengths.tolist() == set_back
+        t["lengths"][who] = reached[who] = 0  # the host hands the row on instead
+        step = cache.plan(layout, *t.values(), tokens=requests, longest=1, reached=reached)
+        step.check()
+
+
 # ---------------------------------------------------------------------------------------- append
 APPENDS = [
     # lengths, new, page, heads_q, heads_kv, dim, norm, rotary, interleaved

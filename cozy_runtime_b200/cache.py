@@ -18,8 +18,9 @@ lengths and says how far the last one went, so that pages behind them come back:
 
 The step's tokens are packed: request n's rows of `query`, `key` and `value` [tokens, heads,
 head_dim] are `step.starts[n]` to `step.starts[n + 1]`. Lengths, page numbers and the plan's answer
-stay on the GPU: no call here synchronizes, and a step can be captured into a CUDA graph (each
-replay plans anew from the lengths the tensors then hold). A plan that cannot be served gives no
+stay on the GPU: no call here synchronizes (but an `append` whose norm weights are not on that GPU),
+and a step can be captured into a CUDA graph (each replay plans anew from the lengths the tensors
+then hold). A plan that cannot be served gives no
 pages and its append and attention do nothing; `Plan.check()` says why. As with every torch tensor,
 a plan or a cache used on another stream than the one that wrote it is ordered by the caller.
 """
@@ -400,17 +401,19 @@ def append(
     `key`, `value` [tokens, heads_kv, head_dim] and `query` [tokens, heads_q, head_dim] bf16, head
     dimension contiguous. Query and key are normed (`norm_q`, `norm_k`: per-head RMSNorm) and
     rotated (`rope`: row = position in the request; the tables must reach the table's width) in
-    fp32 and rounded once to bf16, the laws of `rope.head_norm_rope`. Returns the ready queries
-    (`out`, or a new tensor; rows of nobody are left as they were), None without `query`. `out` is
-    the query itself or shares no memory with it, and none with a row of `key` or `value`. A token
-    whose page number is outside the pool (the plan's status says so) is not stored, its ready query
-    is zero.
+    fp32 and rounded once to bf16, the laws of `rope.head_norm_rope`. Norm weights are read as they
+    are where they are fp32, contiguous and on the cache's GPU. Others are converted in every call,
+    one more launch each; those on the host or another GPU are copied, which waits for the copy and
+    is refused in a captured step. Returns the ready queries (`out`, or a new tensor; rows of nobody
+    are left as they were), None without `query`. `out` is the query itself or shares no memory with
+    it, and none with a row of `key` or `value`. A token whose page number is outside the pool (the
+    plan's status says so) is not stored, its ready query is zero.
 
     A block's exponent is the smallest e ≥ -60 with max |x| ≤ 448 · 2^e over the tokens put into it
-    so far, those among them that were rejected later. It only grows until a token starts the block
-    anew; the codes a block holds are then rounded to the grown scale, which is
-    exact down to e4m3's subnormals. NaN, infinities and magnitudes over 448 · 2^40 are stored as
-    NaN and leave the exponent alone. The same step can be appended again: it stores the same.
+    so far, those among them that were rejected later. Until a token starts the block anew it only
+    grows; the codes the block holds are then rounded to the grown scale, which is exact down to
+    e4m3's subnormals. NaN, infinities and magnitudes over 448 · 2^40 are stored as NaN and leave the
+    exponent alone. The same step can be appended again: it stores the same.
     A page that requests share must be full: two writers of one block are not ordered."""
     _fits(store, step)
     layout, index, tokens = step.layout, store._index, step.tokens
@@ -462,6 +465,10 @@ def append(
         if norm.weight is not None:
             if norm.weight.shape != (layout.head_dim,):
                 raise ValueError("a norm's weight has one value for each channel of a head")
+            if norm.weight.get_device() != index:
+                with _on(index):
+                    if torch.cuda.is_current_stream_capturing():
+                        raise ValueError(f"a norm's weight on {norm.weight.device} in a captured step on {device}")
             w = norm.weight.to(device=device, dtype=torch.float32).contiguous()
             weights.append(w)
             a.norm_weight[i] = w.data_ptr()

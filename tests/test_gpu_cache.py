@@ -846,6 +846,37 @@ def test_a_captured_step_plans_anew_at_each_replay():
             assert (out[sum(new):] == 0).all()
 
 
+def test_norm_weights_as_models_ship_them():
+    """bf16 and strided weights give what their fp32 values give, captured too; a weight that is not
+    on the GPU is refused in a captured step, which goes on without it."""
+    from cozy_runtime_b200 import cache, ulysses
+
+    g = torch.Generator().manual_seed(16)
+    layout = cache.Layout(4, 2, 128, 16)
+    m = make([5, 40], [20, 3], 16, g)
+    step, _ = on_gpu(m, layout)
+    store = cache.Cache.empty(layout, step.pages)
+    q, k = (torch.randn(23, h, 128, generator=g).to(torch.bfloat16).cuda() for h in (4, 2))
+    weight = torch.randn(128, generator=g).to(torch.bfloat16)
+    strided = weight.float().repeat_interleave(2).cuda()[::2]
+
+    def append(w):
+        return cache.append(store, step, k, k, query=q, norm_q=ulysses.Norm(w, 0.5), norm_k=ulysses.Norm(w, 0.5))
+
+    want, codes = append(weight.float().cuda()), store.key.view(torch.uint8).clone()
+    on_cuda = weight.cuda()
+    for w in (on_cuda, strided, weight, weight.double()):
+        assert torch.equal(append(w), want) and torch.equal(store.key.view(torch.uint8), codes)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="captured"):
+            append(weight)
+        got = append(on_cuda)
+    got.zero_()
+    graph.replay()
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("new", [[1] * 20, [60, 1, 9] + [1] * 17])
 def test_calls_side_by_side_on_two_streams(new):
     """Two layers of one step on two streams: the same plan, caches of their own."""

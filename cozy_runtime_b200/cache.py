@@ -495,7 +495,8 @@ def attention(
     the natural log of each row's sum of exponentials [tokens, heads_q] fp32, by which outputs
     over parts of the keys can be joined. Rows of nobody are left as they were.
 
-    What stands in blocks behind a row's last key, NaN among it, does not reach the row. Keys in a
+    What stands in blocks behind a row's last key, NaN among it, does not reach the row. A query row
+    with an infinity or a NaN gives a row of NaN. Keys in a
     page whose number is outside the pool are left out, and the plan's status says so."""
     _fits(store, step)
     layout, index = step.layout, store._index

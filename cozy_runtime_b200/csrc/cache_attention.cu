@@ -359,7 +359,8 @@ __global__ void __launch_bounds__(Few<HD>::kWarps * 32, 1)
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const int up = min(100, 14 + 127 - static_cast<int>(__float_as_uint(amax) >> 23));
-    const float s = exponent_scale(up), back = a.scale_log2 * exponent_scale(-up);
+    // scores of an infinity have no softmax: under a scale of zero it is NaN, and its row with it
+    const float s = amax == INFINITY ? 0.f : exponent_scale(up), back = a.scale_log2 * exponent_scale(-up);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mul[i] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + i));

@@ -531,6 +531,33 @@ def test_attention_nan_reaches_the_rows_that_see_it(lengths, new, hq, hkv, dim):
     assert torch.equal(lse.cpu()[~rows], plain_lse.cpu()[~rows]) and lse.cpu()[rows].isnan().all()
 
 
+@pytest.mark.parametrize("spot", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("lengths,new,dim", [
+    ([100, 30], [1, 1], 128), ([100, 30], [3, 2], 64), ([20000, 30], [1, 1], 128),  # the last: joined parts
+    ([100, 30], [150, 90], 128), ([100, 30], [80, 1], 64),
+])
+def test_attention_of_a_query_that_is_not_finite_is_nan(lengths, new, dim, spot):
+    """An infinity's scores are infinite or NaN, of one sign too where the keys are: no softmax."""
+    from cozy_runtime_b200 import cache
+
+    page, hq, hkv = 32, 4, 2
+    g = torch.Generator().manual_seed(3)
+    m = make(lengths, new, page, g)
+    step, _ = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    k, ke = fill(step.pages, hkv, page, dim, g)
+    v, ve = fill(step.pages, hkv, page, dim, g)
+    k[..., 5] = 3.0  # every key's share of an infinity here has its sign
+    q = torch.randn(m["tokens"], hq, dim, generator=g).to(torch.bfloat16)
+    store = store_on_gpu(k, ke, v, ve)
+    plain, plain_lse = cache.attention(store, step, q.cuda(), return_lse=True)
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool)
+    for t, h in ((0, 1), (m["tokens"] - 1, 3), (m["tokens"] // 2, 2)):
+        q[t, h, 5], hit[t, h] = spot, True
+    out, lse = cache.attention(store, step, q.cuda(), return_lse=True)
+    assert torch.equal(out.isnan().cpu(), hit[..., None].expand(q.shape)) and torch.equal(lse.isnan().cpu(), hit)
+    assert torch.equal(out.cpu()[~hit], plain.cpu()[~hit]) and torch.equal(lse.cpu()[~hit], plain_lse.cpu()[~hit])
+
+
 @pytest.mark.parametrize("new,dim", [([1, 1, 1], 128), ([4, 1, 2], 64), ([200, 1, 60], 128), ([70, 70, 1], 64)])
 def test_attention_leaves_out_bad_pages(new, dim):
     """Page numbers outside the pool (written into the table behind the plan): their keys are left

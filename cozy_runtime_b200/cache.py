@@ -495,6 +495,11 @@ def attention(
     the natural log of each row's sum of exponentials [tokens, heads_q] fp32, by which outputs
     over parts of the keys can be joined. Rows of nobody are left as they were.
 
+    Arithmetic: fp32 sums and softmax; weights are rounded to f16's 11 bits. A query row alone or
+    among few (up to 24 rows a key head) is read to 2^-28 of its largest value; in a longer chunk as
+    two e4m3 parts, exactly from 2^-9.8 of its largest value on and to 2^-17.8 of it below, so the
+    same row may differ there in bf16's last bit.
+
     What stands in blocks behind a row's last key, NaN among it, does not reach the row. A query row
     with an infinity or a NaN gives a row of NaN. Keys in a
     page whose number is outside the pool are left out, and the plan's status says so."""

@@ -16,7 +16,7 @@ namespace cozy {
 
 // Exponents: the floor keeps 2^(s - m + e) of the attention above fp32's smallest normal for
 // every key within 2^-26 of its row's largest term, whatever mixture of scales a row meets
-// (floor to ceiling is a factor of 2^100); magnitudes under 2^-69 are stored as zero, those over
+// (floor to ceiling is a factor of 2^100); magnitudes up to 2^-70 are stored as zero, those over
 // 448 · 2^40 (infinities among them) as NaN.
 constexpr int kExponentFloor = -60;
 constexpr int kExponentCeiling = 40;

@@ -694,8 +694,9 @@ __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
 //                   the issuer waits once for both
 //
 // S = Q·Kᵀ runs in 8 bits on K's codes as they are stored, with Q split into two e4m3 parts
-// under one power of two a row: q = hi + lo holds all 8 bits of a bf16 that is not below 2^-11 of
-// its row's largest value, and a smaller one to 2^-19 of that. Two 8-bit products cost what one
+// under one power of two a row that puts its largest value in (224, 448]: q = hi + lo holds all 8
+// bits of a bf16 from 2^-2 on, which is at most 2^-9.8 of the largest, and a smaller one to half of
+// e4m3's smallest step, 2^-10: 2^-17.8 of the largest or less. Two 8-bit products cost what one
 // 16-bit product costs, and K needs neither widening nor more than its stored bytes of shared
 // memory. P stays in f16 (11 bits; two 8-bit parts would lose the weights under 2^-17 of a row's
 // largest, which a long context has many of), so V is widened.

@@ -647,6 +647,42 @@ def test_attention_over_the_whole_range_of_scales(new):
     check_attention(out, lse, want, m["tokens"], floor_of(300, ve))
 
 
+@pytest.mark.parametrize("new,dim", [([1, 3], 128), ([2, 1], 64), ([60, 90], 128), ([130, 40], 64)])
+def test_attention_of_queries_with_one_large_channel(new, dim):
+    """One channel of a query 2000 times the others and the keys zero in it. In a chunk a query is two
+    e4m3 parts whose largest value is scaled into (224, 448]: each channel is off by half a
+    subnormal step, 2^-10, or less, so a score by amax(q) · 2^-10 / 224 · sum |k| · scale on top of
+    the usual 2^-16 of its sum of magnitudes. Single tokens and drafts do without that."""
+    from cozy_runtime_b200 import cache
+
+    lengths, page, hq, hkv = [150, 77], 16, 4, 2
+    g = torch.Generator().manual_seed(dim + len(new))
+    m = make(lengths, new, page, g)
+    step, t = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    k, ke = fill(step.pages, hkv, page, dim, g, outliers=False)
+    v, ve = fill(step.pages, hkv, page, dim, g)
+    k[..., 7] = 0
+    q = torch.randn(m["tokens"], hq, dim, generator=g) * 0.05
+    q[..., 7] = torch.where(torch.rand(q.shape[:2], generator=g) < 0.5, -1, 1) * (60 + 60 * torch.rand(q.shape[:2], generator=g))
+    q = q.to(torch.bfloat16)
+    out, lse = cache.attention(store_on_gpu(k, ke, v, ve), step, q.cuda(), return_lse=True)
+    scale, kv, table = dim**-0.5, values(k, ke), t["table"].tolist()
+    ref, rlse, weight, size = law.attend_step(kv, values(v, ve), table, lengths, new, q, page, scale)
+    off, t0 = 2**-16 * size, 0
+    for n, (length, a) in enumerate(zip(lengths, new)):
+        if a * hq // hkv > 24:
+            rows = kv[table[n][:-(-(length + a) // page)]].abs().sum(-1).amax((0, 2))  # of each key head
+            amax = q[t0:t0 + a].double().abs().amax(-1)
+            off[t0:t0 + a] += amax * 2**-10 / 224 * rows.repeat_interleave(hq // hkv) * scale
+        t0 += a
+    assert off.max() < 0.04  # e^(2 off) - 1 < 2.1 off
+    err = (out.cpu().double() - ref).abs()
+    bound = 2**-8 * ref.abs() + (2**-10 + 2.1 * off[..., None]) * weight + floor_of(300, ve)
+    assert (err <= bound).all(), (err / bound).max()
+    err = (lse.cpu().double() - rlse).abs()
+    assert (err <= off + 2**-20 * (8 + rlse.abs())).all(), err.max()
+
+
 def test_attention_far_into_a_large_pool():
     """Blocks behind the first 4 GB of a pool, rows of a packed projection, a strided output."""
     from cozy_runtime_b200 import cache

@@ -647,6 +647,32 @@ def test_attention_over_the_whole_range_of_scales(new):
     check_attention(out, lse, want, m["tokens"], floor_of(300, ve))
 
 
+@pytest.mark.parametrize("new", [[2, 1, 3], [70, 90, 60]])
+def test_attention_over_the_scales_of_a_rows_own_blocks(new):
+    """Requests and heads whose values are all tiny, all ordinary or all huge, in one step: the
+    absolute error of a row is that of the scales it sees, not of the pool's largest."""
+    from cozy_runtime_b200 import cache
+
+    lengths, page, hq, hkv, dim = [200, 90, 133], 16, 4, 2, 64
+    g = torch.Generator().manual_seed(21)
+    m = make(lengths, new, page, g)
+    step, t = on_gpu(m, cache.Layout(hq, hkv, dim, page))
+    k, ke = fill(step.pages, hkv, page, dim, g)
+    v, ve = fill(step.pages, hkv, page, dim, g)
+    floor, table, t0 = torch.zeros(m["tokens"], hq, 1, dtype=torch.float64), t["table"].tolist(), 0
+    for n, (length, a) in enumerate(zip(lengths, new)):
+        for h in range(hkv):
+            low = [-60, -8, 34][(n + h) % 3]
+            pages = table[n][:-(-(length + a) // page)]
+            ve[pages, h] = torch.randint(low, low + 7, (len(pages),), generator=g).to(torch.int8)
+            floor[t0:t0 + a, h * hq // hkv:(h + 1) * hq // hkv] = floor_of(length + a, ve[pages, h])
+        t0 += a
+    q = torch.randn(m["tokens"], hq, dim, generator=g).to(torch.bfloat16)
+    out, lse = cache.attention(store_on_gpu(k, ke, v, ve), step, q.cuda(), return_lse=True)
+    want = law.attend_step(values(k, ke), values(v, ve), table, lengths, new, q, page, dim**-0.5)
+    check_attention(out, lse, want, m["tokens"], floor)
+
+
 @pytest.mark.parametrize("new,dim", [([1, 3], 128), ([2, 1], 64), ([60, 90], 128), ([130, 40], 64)])
 def test_attention_of_queries_with_one_large_channel(new, dim):
     """One channel of a query 2000 times the others and the keys zero in it. In a chunk a query is two

@@ -19,8 +19,9 @@ namespace cg = cooperative_groups;
 // One cluster. Every CTA scans all requests (a few loads a thread, two barriers a round: cheaper
 // than handing the sums over), keeps the running sums in shared memory, and then takes its share
 // of the tokens, fresh pages, released pages and touched blocks, each found by bisection.
-// Nothing here is bandwidth: a step of 4 requests moves 112 bytes, one of 1000 requests 170 KB;
-// the time is the launch, one load of the lengths, the scan and the bisection's chain.
+// Nothing here is bandwidth: a step of 4 requests moves 112 bytes (6.1 us), one of 1000 requests
+// 170 KB (13.3 us, 1 us of it the look at released page numbers); the time is the launch, one load
+// of the lengths, the scan and the bisection's chain.
 constexpr int kPlanThreads = 1024;
 
 struct PlanSums {
@@ -339,7 +340,7 @@ int cache_plan(const CozyCachePlan& p, const int* reached, cudaStream_t stream) 
 // registers), normed and rotated, their largest magnitude sets or grows the block's exponent,
 // and their codes are written. WARPS warps share a unit. Queries take CTAs of the same launch.
 // HBM bounds the long form: a token reads (Hq + 2 Hkv) · D bf16 and writes Hq · D bf16 and
-// 2 · Hkv · D codes. 8192 tokens (32/8 heads of 128) take 43.6 us, 0.66 of the measured copy rate
+// 2 · Hkv · D codes. 8192 tokens (32/8 heads of 128) take 42.8 us, 0.67 of the measured copy rate
 // (32.4 us, 0.84, without a rotation: each head's keys read the tables from L2 again).
 struct AppendTensor {
   int normalize, wide;  // wide: the weights can be read 16 bytes at a time
@@ -715,7 +716,7 @@ static int append_launch(AppendArgs& a, int longest, cudaStream_t stream) {
   const long long units = 2LL * a.heads_kv * a.max_blocks;
   // Four passes of rows a warp, and as many warps a unit as its rows then take (a page of 128 rows
   // of 128 channels: eight passes of 8 warps); two passes of twice the warps took 49.4 us for 8192
-  // tokens instead of 43.6. A decode step has one row a unit: one pass, 4.9 us for 256 tokens
+  // tokens instead of 42.8. A decode step has one row a unit: one pass, 4.9 us for 256 tokens
   // instead of 5.7 (device time; 32/8 heads of 128, pages of 64).
   const int most = longest < a.page ? longest : a.page;
   const int warps = most <= 4 * kRows ? 1 : most <= 8 * kRows ? 2 : most <= 16 * kRows ? 4 : 8;

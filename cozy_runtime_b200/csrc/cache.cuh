@@ -28,10 +28,10 @@ enum : int {
   kPlanNarrow = 2,      // a request longer than its table row
   kPlanTokens = 4,      // more new tokens than `tokens`, or than `longest` in one request
   kPlanLengths = 8,     // a negative length, new < -1, or a ring whose cursor is not possible
-  kPlanBadPage = 16,    // a page number outside [0, pages): its tokens are left out
+  kPlanBadPage = 16,    // a page number outside [0, pages): its tokens are left out; among pages
+                        // to be released: the step is refused
   kPlanTimeout = 32,    // an on-chip wait of a call of this step ran past its limit
 };
-constexpr int kPlanRefused = kPlanNoPages | kPlanNarrow | kPlanTokens | kPlanLengths;
 
 // 2^e of an exponent byte; any byte is valid (uninitialised blocks behind a sequence are read).
 __host__ __device__ __forceinline__ float exponent_scale(int e) {
@@ -51,8 +51,9 @@ __host__ __device__ __forceinline__ long long quotient(long long a, long long b)
   return a / b;
 }
 
-// Σ floor((a·i + b) / 128) for i in [0, n), 0 ≤ a ≤ 256, 0 ≤ b, n < 2^24: the Euclid-like recursion
-// on the divisor and a; behind its first step everything is below 2^31.
+// Σ floor((a·i + b) / 128) for i in [0, n), 0 ≤ a ≤ 256, 0 ≤ b, n < 2^24: the floor sum of lattice
+// points under a line by its well-known recursion, which swaps the divisor and a as Euclid's
+// algorithm does; behind its first step everything is below 2^31.
 __host__ __device__ inline long long floor_sum_128(uint32_t n, uint32_t a, long long b) {
   if (n == 0) return 0;
   long long sum = static_cast<long long>(n) * (n - 1) / 2 * (a >> 7) + n * (b >> 7);

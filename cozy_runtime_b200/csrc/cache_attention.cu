@@ -4,8 +4,10 @@
 // of one head of one request) stand in one order, requests outermost, and every warp of the GPU
 // takes an equal run of them, whatever the lengths are. A run that covers an item (one head of
 // one request) writes its output; pieces of items leave fp32 rows and (max, sum) in the
-// workspace, and a second kernel, already resident when the first ends, joins them in order: no
-// atomics, the same bits every time.
+// workspace, and a second kernel joins them in order: no atomics, the same bits every time. The
+// join is launched while the first kernel runs, which hides the launch; its blocks start as SMs
+// come free, since the first leaves none the registers (8192 of an SM with heads of 128, and a
+// join's block takes 12288).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -704,9 +706,10 @@ __global__ void __launch_bounds__(256) join_few(const CacheArgs a) {
 // A tile of keys is taken in two halves of 64 with a buffer of S each, so that the next half's
 // Q·Kᵀ is done when a half's softmax ends: neither the tensor cores nor the softmax wait for the
 // other's round trip. (With one buffer of 128 a unit took 3823 clocks, 2129 of them on the tensor
-// cores.) A chunk of 1024 tokens behind 130047 keys (32/8 heads of 128) takes 2.33 ms: 941 TFLOP/s,
-// 0.56 of the measured bf16 rate, under the power cap; the exponentials and the tensor cores take
-// about half of it each and overlap in part. Tensor memory: S/P of tile s, half b at column 128 s + 64 b, O at 256 + HD s.
+// cores.) A chunk of 1024 tokens behind 130047 keys (32/8 heads of 128) takes 4.1 M clocks: 2.12 ms
+// at 1965 MHz, and in a loop under the power cap 2.48 ms at 1657 MHz, 885 TFLOP/s, 0.53 of the
+// measured bf16 rate. That is 4650 clocks a unit, of which the exponentials take 2092 and the matrix
+// instructions 2448: as much as both, one after the other. Tensor memory: S/P of tile s, half b at column 128 s + 64 b, O at 256 + HD s.
 template <int HD>
 struct Many {
   static constexpr int kThreads = 512;
@@ -1703,7 +1706,7 @@ long long cache_workspace(const CozyCachePlan& p, const CozyCacheStore& c) {
   return (may_be_few(p) ? few_bytes(c.head_dim) : 0) + (may_be_many(p) ? many_bytes(c.head_dim) : 0);
 }
 
-// A join starts while its attention runs and waits for that one's end on the device.
+// A join is launched while its attention runs and waits for that one's end on the device.
 static int join_launch(void (*kernel)(CacheArgs), dim3 grid, const CacheArgs& a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;

@@ -496,9 +496,9 @@ def attention(
     over parts of the keys can be joined. Rows of nobody are left as they were.
 
     Arithmetic: fp32 sums and softmax; weights are rounded to f16's 11 bits. A query row alone or
-    among few (up to 24 rows a key head) is read to 2^-28 of its largest value; in a longer chunk as
-    two e4m3 parts, exactly from 2^-9.8 of its largest value on and to 2^-17.8 of it below, so the
-    same row may differ there in bf16's last bit.
+    among few (up to 24 rows a key head) is read exactly from 2^-28 of its largest value on; in a
+    longer chunk, as two e4m3 parts, exactly from 2^-9.8 of it on and to 2^-17.8 of it below, so the
+    same row may come out a little different there.
 
     What stands in blocks behind a row's last key, NaN among it, does not reach the row. A query row
     with an infinity or a NaN gives a row of NaN. Keys in a
